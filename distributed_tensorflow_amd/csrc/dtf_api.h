@@ -250,6 +250,31 @@ int dtf_dense_step_begin(float* loss_sum, int32_t* correct, float* global_step, 
 int dtf_softmax_xent(const float* logits, const float* labels, int M, int C, float* dz, float grad_scale,
                      float* loss_sum, int32_t* correct, float* row_loss, void* stream);
 
+// --- a model over tokens: table lookup with gradient and row update (embed.hip) ----------------------------------
+// dtype: 0 fp32, 1 bf16, 2 fp16.  ids: int32 (ids_wide 0) or int64 (1); an id outside [0, rows) is padding (a row of zeros,
+// no gradient).  Leading dimensions in elements; workspace: dtf_embed_workspace bytes, 16-byte aligned, contents unimportant.
+// out[t][:] = scale * table[ids[t]][:]
+int dtf_embed_lookup(const void* table, int dtype, int64_t rows, int dim, int64_t ld, const void* ids, int ids_wide,
+                     int64_t tokens, float scale, void* out, int64_t ldo, void* stream);
+int64_t dtf_embed_workspace(int64_t tokens, int dim);
+// grad[v][:] = scale * sum of g[t][:] over the t with id v, for every row v
+int dtf_embed_grad(const void* ids, int ids_wide, int64_t tokens, const void* g, int64_t ldg, void* grad, int dtype,
+                   int64_t rows, int dim, int64_t ldt, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+// table[v][:] -= lr[0] * scale * sum of g[t][:]; rows that do not occur are not touched
+int dtf_embed_sgd(const void* ids, int ids_wide, int64_t tokens, const void* g, int64_t ldg, void* table, int dtype,
+                  int64_t rows, int dim, int64_t ldt, float scale, const float* lr, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+// Softmax cross-entropy against integer labels (xent.hip).  row_loss[t] = logsumexp(z[t]) - z[t][label]; dz (may be null;
+// may be the logits themselves) = grad_scale * d(row loss)/dz; stats[t][2] (may be null): maximum and sum of exponentials
+// relative to it, what dtf_sparse_xent_grad needs.  A negative label is padding (loss 0, gradient 0), one >= classes gives NaN.
+int dtf_sparse_xent(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                    int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats, void* stream);
+// dz = g[t * g_stride] * d(row loss t)/dz
+int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                         int labels_wide, const float* stats, const float* g, int64_t g_stride, void* dz, int64_t ldz,
+                         void* stream);
+
 int dtf_abi_sizeof(int which);   // sizeof of DtfMlpDesc (0), DtfPipeDesc (1), DtfXgDesc (2)
 const char* dtf_hip_build_info(void);
 

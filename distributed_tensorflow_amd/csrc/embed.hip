@@ -1,0 +1,576 @@
+// Table lookup by token, its gradient, and the sparse row update (an embedding in front of a dense stack).
+//
+//   lookup    out[t][:]   = scale * table[ids[t]][:]
+//   gradient  grad[v][:]  = scale * sum over t with ids[t] = v of g[t][:]           (every row of the table is written)
+//   update    table[v][:] -= lr * scale * sum over t with ids[t] = v of g[t][:]     (only rows that occur are touched)
+//
+// An id outside [0, rows) is padding: a row of zeros, no gradient.  Storage fp32, bf16 or fp16; sums in fp32, rounded once.
+//
+// All three are bound by memory.  The gradient must not depend on the order in which atomics land, and a frequent token
+// must not serialise on its row, so the tokens are SORTED by id (stable, least significant digit first) and equal ids are
+// summed as runs of the sorted order, in ascending t:
+//
+//   sort      digits of up to 9 bits, two launches per digit: counts of every block, then the scatter, each block of which
+//             adds up the counts in front of it by itself (at most 128 blocks, so that is at most 128 coalesced rows).
+//             Ranks inside a wave come from ballots over the digit's bits.  Up to 4096 tokens: one workgroup, all digits
+//             in LDS, one launch.
+//   sums      a group of lanes owns a chunk of consecutive sorted positions and a slice of columns, walks the chunk with
+//             the loads of four positions in flight, and stores each run that lies inside the chunk.  The pieces of a run
+//             that crosses chunks go to an fp32 workspace row of their chunk.  Further blocks of the same launch look up
+//             (binary search in the sorted ids) which rows of the table do not occur and store their zeros, so no row of
+//             the gradient is written twice.
+//   joins     one group of waves per run that crosses chunks adds its pieces in order.  The chunk borders depend on the
+//             sizes alone: the result is the same bits every time.
+#include "dtf_api.h"
+#include "dtf_types.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kSmall = 4096;        // tokens sorted by one workgroup
+constexpr int kSortThreads = 1024;
+constexpr int kWaves = kSortThreads / 64;
+constexpr int kMaxDigit = 9;        // bits
+constexpr int kMaxSortBlocks = 128;
+constexpr int kThreads = 256;
+constexpr int kFillRows = 32;       // rows of the table per zero-filling block
+constexpr int kJoinChunks = 4;      // chunks whose crossing runs one block joins
+
+__device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t t) {
+  return wide ? static_cast<const int64_t*>(ids)[t] : (int64_t) static_cast<const int32_t*>(ids)[t];
+}
+// Sort key: the row, or `rows` (behind every row) for padding.
+__device__ __forceinline__ uint32_t load_key(const void* ids, int wide, int64_t t, uint32_t rows) {
+  const int64_t id = load_id(ids, wide, t);
+  return (id >= 0 && id < (int64_t)rows) ? (uint32_t)id : rows;
+}
+
+// --- lookup ------------------------------------------------------------------------------------------------------------
+// 1 << lanes_log2 lanes per row, as many rows per block as fit; the grid strides over the tokens.
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void lookup_kernel(const T* __restrict__ table, int64_t ld, int64_t rows,
+                                                          const void* __restrict__ ids, int wide, int64_t tokens, int packs,
+                                                          int lanes_log2, float scale, T* __restrict__ out, int64_t ldo) {
+  const int group = threadIdx.x >> lanes_log2, groups = kThreads >> lanes_log2;
+  const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
+  for (int64_t t = (int64_t)blockIdx.x * groups + group; t < tokens; t += (int64_t)gridDim.x * groups) {
+    const int64_t id = load_id(ids, wide, t);
+    const bool inside = id >= 0 && id < rows;
+    const T* src = table + (inside ? id : 0) * ld;
+    T* dst = out + t * ldo;
+    for (int c = lane; c < packs; c += 1 << lanes_log2) {
+      Pack<T, N> p;
+      if (inside) {
+        p = *reinterpret_cast<const Pack<T, N>*>(src + (int64_t)c * N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) p.v[e] = (T)(scale * (float)p.v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) p.v[e] = (T)0.0f;
+      }
+      *reinterpret_cast<Pack<T, N>*>(dst + (int64_t)c * N) = p;
+    }
+  }
+}
+
+// --- sort --------------------------------------------------------------------------------------------------------------
+// Lanes of the wave with the same digit as this one (among `valid` lanes).
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool valid) {
+  uint64_t mask = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot((digit >> b) & 1u);
+    mask &= ((digit >> b) & 1u) ? set : ~set;
+  }
+  return mask;
+}
+
+// Stable places of one batch of kSortThreads items.  `base[d]` is where the next item with digit d goes; it is advanced.
+// `wave_at[w][d]` is zero on entry and on exit.  Every thread of the block calls it.
+__device__ __forceinline__ uint32_t place(uint32_t digit, int bits, bool valid, uint32_t* base, uint32_t* wave_at) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << bits;
+  const uint64_t mask = same_digit(digit, bits, valid);
+  const uint32_t rank = __popcll(mask & ((1ull << lane) - 1));
+  const bool leader = valid && rank == 0;
+  if (leader) wave_at[wave * digits + digit] = __popcll(mask);
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+    uint32_t at = base[d];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t n = wave_at[w * digits + d];
+      wave_at[w * digits + d] = at;
+      at += n;
+    }
+    base[d] = at;
+  }
+  __syncthreads();
+  const uint32_t to = valid ? wave_at[wave * digits + digit] + rank : 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
+  __syncthreads();
+  return to;
+}
+
+// Exclusive prefix sum over `digits` (<= 512) totals, one per thread; every thread of the block calls it.
+__device__ __forceinline__ uint32_t digit_prefix(uint32_t v, uint32_t* wave_sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t inc = v;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t up = __shfl_up(inc, s);
+    if (lane >= s) inc += up;
+  }
+  if (lane == 63) wave_sum[wave] = inc;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += wave_sum[w];
+  __syncthreads();
+  return before + inc - v;
+}
+
+// The whole sort in one workgroup, items and counters in LDS.
+__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void* __restrict__ ids, int wide, int tokens,
+                                                                  uint32_t rows, int key_bits, uint32_t* __restrict__ keys,
+                                                                  uint32_t* __restrict__ order) {
+  __shared__ uint2 item[2][kSmall];
+  __shared__ uint32_t wave_at[kWaves * 256];
+  __shared__ uint32_t base[256], wave_sum[kWaves];
+  for (int i = threadIdx.x; i < tokens; i += kSortThreads) item[0][i] = make_uint2(load_key(ids, wide, i, rows), (uint32_t)i);
+  for (int i = threadIdx.x; i < kWaves * 256; i += kSortThreads) wave_at[i] = 0;
+  const int passes = (key_bits + 7) / 8, bits = (key_bits + passes - 1) / passes, digits = 1 << bits;
+  int cur = 0;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    if (threadIdx.x < digits) base[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens; i += kSortThreads) atomicAdd(&base[(item[cur][i].x >> shift) & (digits - 1)], 1u);
+    __syncthreads();
+    const uint32_t total = threadIdx.x < digits ? base[threadIdx.x] : 0;
+    const uint32_t at = digit_prefix(total, wave_sum);
+    if (threadIdx.x < digits) base[threadIdx.x] = at;
+    __syncthreads();
+    for (int i0 = 0; i0 < tokens; i0 += kSortThreads) {
+      const int i = i0 + threadIdx.x;
+      const bool valid = i < tokens;
+      const uint2 it = valid ? item[cur][i] : make_uint2(0, 0);
+      const uint32_t to = place((it.x >> shift) & (digits - 1), bits, valid, base, wave_at);
+      if (valid) item[cur ^ 1][to] = it;
+    }
+    __syncthreads();
+    cur ^= 1;
+  }
+  for (int i = threadIdx.x; i < tokens; i += kSortThreads) {
+    keys[i] = item[cur][i].x;
+    order[i] = item[cur][i].y;
+  }
+}
+
+struct SortPass {
+  const void* ids;         // first pass: the ids themselves
+  const uint2* in;         // later passes: {key, position}
+  int wide;
+  uint32_t rows;
+  int64_t tokens, tile;    // items per block, a multiple of kSortThreads
+  int shift, bits;
+};
+
+__device__ __forceinline__ uint2 sort_item(const SortPass& a, int64_t i) {
+  return a.in ? a.in[i] : make_uint2(load_key(a.ids, a.wide, i, a.rows), (uint32_t)i);
+}
+
+// counts[block][digit]
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortPass a, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t hist[1 << kMaxDigit];
+  const int digits = 1 << a.bits, lane = threadIdx.x & 63;
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * a.tile, last = min(first + a.tile, a.tokens);
+  for (int64_t i0 = first; i0 < last; i0 += kSortThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    const bool valid = i < last;
+    const uint32_t digit = valid ? (sort_item(a, i).x >> a.shift) & (digits - 1) : 0;
+    // one LDS atomic per distinct digit of the wave: a frequent token would make its lanes queue on one counter
+    const uint64_t mask = same_digit(digit, a.bits, valid);
+    if (valid && (mask & ((1ull << lane) - 1)) == 0) atomicAdd(&hist[digit], (uint32_t)__popcll(mask));
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kSortThreads) counts[(int64_t)blockIdx.x * digits + d] = hist[d];
+}
+
+// `pairs` (not the last pass) or `keys` and `order` (the last pass) receive the items in order of this digit.
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass a, const uint32_t* __restrict__ counts,
+                                                                    int blocks, uint2* __restrict__ pairs,
+                                                                    uint32_t* __restrict__ keys, uint32_t* __restrict__ order) {
+  __shared__ uint32_t wave_at[kWaves << kMaxDigit];
+  __shared__ uint32_t base[1 << kMaxDigit], wave_sum[kWaves];
+  const int digits = 1 << a.bits;
+  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
+  uint32_t total = 0, before = 0;
+  if (threadIdx.x < digits) {
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) {
+      const uint32_t n = counts[(int64_t)b * digits + threadIdx.x];
+      total += n;
+      before += b < (int)blockIdx.x ? n : 0;
+    }
+  }
+  const uint32_t at = digit_prefix(total, wave_sum);
+  if (threadIdx.x < digits) base[threadIdx.x] = at + before;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * a.tile, last = min(first + a.tile, a.tokens);
+  for (int64_t i0 = first; i0 < last; i0 += kSortThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    const bool valid = i < last;
+    const uint2 it = valid ? sort_item(a, i) : make_uint2(0, 0);
+    const uint32_t to = place((it.x >> a.shift) & (digits - 1), a.bits, valid, base, wave_at);
+    if (valid) {
+      if (pairs) {
+        pairs[to] = it;
+      } else {
+        keys[to] = it.x;
+        order[to] = it.y;
+      }
+    }
+  }
+}
+
+// --- sums --------------------------------------------------------------------------------------------------------------
+struct SumArgs {
+  const uint32_t* keys;      // sorted
+  const uint32_t* order;     // token of every sorted position
+  int64_t tokens;
+  uint32_t rows;
+  int chunk;                 // sorted positions per chunk
+  int64_t chunks;
+  int dim, packs, lanes_log2;
+  int64_t ldg, ldt;          // row strides of g and of the table / gradient, in elements
+  float scale;
+  const float* lr;           // row update: device learning rate
+  float* pieces;             // [chunks][2][piece_ld]: the run that began before the chunk, the run that goes on behind it
+  int64_t piece_ld;
+  int64_t sum_blocks;        // blocks past these write the zeros of rows that do not occur
+};
+
+template <typename T, int N, bool UPDATE>
+__device__ __forceinline__ void store_row(const SumArgs& a, T* table, uint32_t row, int pack, const float (&acc)[N], float f) {
+  Pack<T, N>* at = reinterpret_cast<Pack<T, N>*>(table + (int64_t)row * a.ldt + (int64_t)pack * N);
+  Pack<T, N> p;
+  if (UPDATE) {
+    p = *at;
+#pragma unroll
+    for (int e = 0; e < N; ++e) p.v[e] = (T)((float)p.v[e] - f * acc[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) p.v[e] = (T)(f * acc[e]);
+  }
+  *at = p;
+}
+
+template <typename T, int N, bool UPDATE>
+__global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __restrict__ g, T* __restrict__ table) {
+  const int lanes = 1 << a.lanes_log2, groups = kThreads >> a.lanes_log2;
+  const int group = threadIdx.x >> a.lanes_log2;
+  const int pack = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+  const bool in_row = pack < a.packs;
+  if ((int64_t)blockIdx.x >= a.sum_blocks) {
+    // Rows that do not occur: which of kFillRows rows are missing from the sorted ids, then their zeros.
+    __shared__ int missing[kFillRows];
+    const int64_t row0 = ((int64_t)blockIdx.x - a.sum_blocks) * kFillRows;
+    if (threadIdx.x < kFillRows) {
+      const int64_t row = row0 + threadIdx.x;
+      int64_t low = 0, high = a.tokens;                    // first position whose key is >= row
+      while (low < high) {
+        const int64_t mid = (low + high) >> 1;
+        if ((int64_t)a.keys[mid] < row) low = mid + 1; else high = mid;
+      }
+      missing[threadIdx.x] = row < (int64_t)a.rows && !(low < a.tokens && (int64_t)a.keys[low] == row);
+    }
+    __syncthreads();
+    Pack<T, N> zero;
+#pragma unroll
+    for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
+    for (int r = group; r < kFillRows; r += groups)
+      if (missing[r] && in_row) *reinterpret_cast<Pack<T, N>*>(table + (row0 + r) * a.ldt + (int64_t)pack * N) = zero;
+    return;
+  }
+  const int64_t chunk = (int64_t)blockIdx.x * groups + group;
+  if (chunk >= a.chunks || !in_row) return;
+  const float f = UPDATE ? a.lr[0] * a.scale : a.scale;
+  const int64_t first = chunk * a.chunk, last = min(first + a.chunk, a.tokens);
+  const T* column = g + (int64_t)pack * N;
+  uint32_t run = a.keys[first];
+  bool from_before = first > 0 && a.keys[first - 1] == run;
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  float* piece = a.pieces + chunk * 2 * a.piece_ld + (int64_t)pack * N;
+  constexpr int kAhead = 4;
+  for (int64_t i0 = first; i0 < last && run < a.rows; i0 += kAhead) {
+    uint32_t key[kAhead];
+    Pack<T, N> v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) key[j] = i0 + j < last ? a.keys[i0 + j] : a.rows;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (key[j] < a.rows) v[j] = *reinterpret_cast<const Pack<T, N>*>(column + (int64_t)a.order[i0 + j] * a.ldg);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + j >= last) break;
+      if (key[j] != run) {
+        if (from_before) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) piece[e] = acc[e];
+        } else {
+          store_row<T, N, UPDATE>(a, table, run, pack, acc, f);
+        }
+        from_before = false;
+        run = key[j];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = 0.f;
+      }
+      if (run < a.rows) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += (float)v[j].v[e];
+      }
+    }
+  }
+  if (run >= a.rows) return;                               // padding sits behind every row
+  const bool goes_on = last < a.tokens && a.keys[last] == run;
+  if (from_before || goes_on) {
+    float* to = from_before ? piece : piece + a.piece_ld;
+#pragma unroll
+    for (int e = 0; e < N; ++e) to[e] = acc[e];
+  } else {
+    store_row<T, N, UPDATE>(a, table, run, pack, acc, f);
+  }
+}
+
+// Runs that cross chunks: the chunk a run begins in names it; its pieces are that chunk's second workspace row and the
+// first rows of the chunks behind it.  Four waves take every fourth piece each; their sums meet in order.
+template <typename T, bool UPDATE>
+__global__ __launch_bounds__(kThreads) void join_kernel(SumArgs a, T* __restrict__ table) {
+  __shared__ f32x4 part[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = (blockIdx.y * 64 + lane) * 4;
+  const float f = UPDATE ? a.lr[0] * a.scale : a.scale;
+  for (int k = 0; k < kJoinChunks; ++k) {
+    const int64_t chunk = (int64_t)blockIdx.x * kJoinChunks + k;
+    if (chunk >= a.chunks) break;
+    const int64_t first = chunk * a.chunk, last = first + a.chunk;
+    if (last >= a.tokens) break;
+    const uint32_t run = a.keys[last - 1];
+    if (run >= a.rows || a.keys[last] != run) continue;
+    if (a.keys[first] == run && first > 0 && a.keys[first - 1] == run) continue;    // it began before this chunk
+    // how many chunks behind this one begin with the run: the ids are sorted, so the first that does not ends the count
+    int64_t pieces = 0;
+    for (int64_t c0 = chunk + 1;; c0 += 64) {
+      const int64_t c = c0 + lane;
+      const uint64_t same = __ballot(c < a.chunks && a.keys[min(c, a.chunks - 1) * a.chunk] == run);
+      pieces += __popcll(same);
+      if (same != ~0ull) break;
+    }
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (col < a.dim) {
+      const float* src = a.pieces + chunk * 2 * a.piece_ld + col;
+      if (wave == 0) sum = *reinterpret_cast<const f32x4*>(src + a.piece_ld);
+#pragma unroll 8
+      for (int64_t p = wave + 1; p <= pieces; p += 4) sum += *reinterpret_cast<const f32x4*>(src + p * 2 * a.piece_ld);
+    }
+    __syncthreads();
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && col < a.dim) {
+      sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+      T* row = table + (int64_t)run * a.ldt + col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < a.dim) row[e] = UPDATE ? (T)((float)row[e] - f * sum[e]) : (T)(f * sum[e]);
+    }
+  }
+}
+
+inline int log2_lanes(int packs) {
+  int l = 0;
+  while ((1 << l) < packs && (1 << l) < kThreads) ++l;
+  return l;
+}
+
+// Sorted positions per chunk: enough chunks for 256 CUs x 1024 threads, at least 4 and at most 32 positions.
+inline int chunk_of(int64_t tokens, int64_t lanes) {
+  const int64_t c = tokens * lanes / (256 * 1024);
+  return c < 4 ? 4 : c > 32 ? 32 : (int)c;
+}
+
+struct Workspace {
+  int64_t keys, order, pairs, counts, pieces, total;    // byte offsets
+  int64_t chunks, piece_ld;
+  int chunk;
+};
+
+// The chunk length goes by the element count of a row and not by the access width: the workspace does not depend on
+// alignment.
+Workspace plan(int64_t tokens, int dim) {
+  Workspace w;
+  auto up = [](int64_t n) { return (n + 255) & ~(int64_t)255; };
+  w.chunk = chunk_of(tokens, (dim + 3) / 4);
+  w.chunks = (tokens + w.chunk - 1) / w.chunk;
+  w.piece_ld = (dim + 7) / 8 * 8;
+  const int64_t big = tokens > kSmall ? 1 : 0;
+  w.keys = 0;
+  w.order = up(w.keys + 4 * tokens);
+  w.pairs = up(w.order + 4 * tokens);
+  w.counts = up(w.pairs + big * 16 * tokens);
+  w.pieces = up(w.counts + big * 4 * kMaxSortBlocks * (1 << kMaxDigit));
+  w.total = up(w.pieces + w.chunks * 2 * w.piece_ld * 4) + 256;
+  return w;
+}
+
+int sort_tokens(const void* ids, int wide, int64_t tokens, uint32_t rows, const Workspace& w, char* ws, hipStream_t s) {
+  uint32_t* keys = reinterpret_cast<uint32_t*>(ws + w.keys);
+  uint32_t* order = reinterpret_cast<uint32_t*>(ws + w.order);
+  int key_bits = 1;
+  while ((1ull << key_bits) <= (uint64_t)rows) ++key_bits;       // keys 0 .. rows
+  if (tokens <= kSmall) {
+    sort_small_kernel<<<1, kSortThreads, 0, s>>>(ids, wide, (int)tokens, rows, key_bits, keys, order);
+    return 0;
+  }
+  uint2* pairs[2] = {reinterpret_cast<uint2*>(ws + w.pairs), reinterpret_cast<uint2*>(ws + w.pairs) + tokens};
+  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + w.counts);
+  int64_t tile = (tokens + kMaxSortBlocks - 1) / kMaxSortBlocks;
+  tile = (tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+  const int blocks = (int)((tokens + tile - 1) / tile);
+  const int passes = (key_bits + kMaxDigit - 1) / kMaxDigit;
+  const int bits = (key_bits + passes - 1) / passes;
+  for (int p = 0; p < passes; ++p) {
+    SortPass a{p == 0 ? ids : nullptr, p == 0 ? nullptr : pairs[(p - 1) & 1], wide, rows, tokens, tile, p * bits, bits};
+    sort_count_kernel<<<blocks, kSortThreads, 0, s>>>(a, counts);
+    sort_scatter_kernel<<<blocks, kSortThreads, 0, s>>>(a, counts, blocks, p + 1 < passes ? pairs[p & 1] : nullptr, keys, order);
+  }
+  return 0;
+}
+
+template <typename T, int N, bool UPDATE>
+void launch_sums(SumArgs a, const T* g, T* table, int64_t fill_rows, hipStream_t s) {
+  a.packs = a.dim / N;
+  a.lanes_log2 = log2_lanes(a.packs);
+  const int lanes = 1 << a.lanes_log2, groups = kThreads / lanes;
+  a.sum_blocks = (a.chunks + groups - 1) / groups;
+  const int64_t fill = (fill_rows + kFillRows - 1) / kFillRows;
+  const dim3 grid((unsigned)(a.sum_blocks + fill), (a.packs + lanes - 1) / lanes);
+  if (grid.x) sum_kernel<T, N, UPDATE><<<grid, kThreads, 0, s>>>(a, g, table);
+  if (a.chunks > 1)
+    join_kernel<T, UPDATE><<<dim3((unsigned)((a.chunks + kJoinChunks - 1) / kJoinChunks), (a.dim + 255) / 256), kThreads, 0, s>>>(a, table);
+}
+
+template <typename T>
+int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const void* g, int64_t ldg, void* table, int64_t ldt,
+                 int64_t rows, int dim, float scale, const float* lr, void* workspace, hipStream_t s) {
+  const Workspace w = plan(tokens, dim);
+  char* ws = static_cast<char*>(workspace);
+  if (tokens > 0) sort_tokens(ids, wide, tokens, (uint32_t)rows, w, ws, s);
+  SumArgs a{};
+  a.keys = reinterpret_cast<uint32_t*>(ws + w.keys);
+  a.order = reinterpret_cast<uint32_t*>(ws + w.order);
+  a.tokens = tokens;
+  a.rows = (uint32_t)rows;
+  a.chunk = w.chunk;
+  a.chunks = w.chunks;
+  a.dim = dim;
+  a.ldg = ldg;
+  a.ldt = ldt;
+  a.scale = scale;
+  a.lr = lr;
+  a.pieces = reinterpret_cast<float*>(ws + w.pieces);
+  a.piece_ld = w.piece_ld;
+  const T* gp = static_cast<const T*>(g);
+  T* tp = static_cast<T*>(table);
+  const int bytes = dtf_access_bytes((uint64_t)g | (uint64_t)table | (uint64_t)(ldg * sizeof(T)) | (uint64_t)(ldt * sizeof(T)) |
+                                     (uint64_t)(dim * sizeof(T)));
+  const int64_t fill = update ? 0 : rows;
+  auto go = [&](auto n) {
+    constexpr int N = decltype(n)::value;
+    if (update) launch_sums<T, N, true>(a, gp, tp, fill, s); else launch_sums<T, N, false>(a, gp, tp, fill, s);
+  };
+  if (bytes == 16) go(std::integral_constant<int, 16 / sizeof(T)>());
+  else if (bytes == 8) go(std::integral_constant<int, 8 / sizeof(T)>());
+  else if (bytes == 4 || sizeof(T) == 4) go(std::integral_constant<int, 4 / sizeof(T)>());
+  else go(std::integral_constant<int, 1>());
+  return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_lookup(const void* table, int64_t ld, int64_t rows, const void* ids, int wide, int64_t tokens, int dim, float scale,
+                  void* out, int64_t ldo, hipStream_t s) {
+  const T* tp = static_cast<const T*>(table);
+  T* op = static_cast<T*>(out);
+  const int bytes = dtf_access_bytes((uint64_t)table | (uint64_t)out | (uint64_t)(ld * sizeof(T)) | (uint64_t)(ldo * sizeof(T)) |
+                                     (uint64_t)(dim * sizeof(T)));
+  auto go = [&](auto n) {
+    constexpr int N = decltype(n)::value;
+    const int packs = dim / N, l = log2_lanes(packs), groups = kThreads >> l;
+    int64_t grid = (tokens + groups - 1) / groups;
+    if (grid > (1 << 20)) grid = 1 << 20;       // (blocks x threads stays below 2^32)
+    lookup_kernel<T, N><<<(unsigned)grid, kThreads, 0, s>>>(tp, ld, rows, ids, wide, tokens, packs, l, scale, op, ldo);
+  };
+  if (bytes == 16) go(std::integral_constant<int, 16 / sizeof(T)>());
+  else if (bytes == 8) go(std::integral_constant<int, 8 / sizeof(T)>());
+  else if (bytes == 4 || sizeof(T) == 4) go(std::integral_constant<int, 4 / sizeof(T)>());
+  else go(std::integral_constant<int, 1>());
+  return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
+}
+
+// grids stay below 2^32 threads
+constexpr int64_t kMaxTokens = (int64_t)1 << 26, kMaxRows = (int64_t)1 << 28;
+constexpr int kMaxDim = 1 << 20;
+
+bool bad_shape(int64_t tokens, int64_t rows, int dim, int dtype) {
+  return tokens < 0 || tokens > kMaxTokens || rows < 1 || rows > kMaxRows || dim < 1 || dim > kMaxDim || dtype < 0 || dtype > 2;
+}
+
+}  // namespace
+
+extern "C" int dtf_embed_lookup(const void* table, int dtype, int64_t rows, int dim, int64_t ld, const void* ids, int ids_wide,
+                                int64_t tokens, float scale, void* out, int64_t ldo, void* stream) {
+  if (bad_shape(tokens, rows, dim, dtype) || ld < dim || ldo < dim) return DTF_ERR_SHAPE;
+  if (tokens == 0) return DTF_OK;
+  if (!table || !ids || !out) return DTF_ERR_NULL;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DTF_F32) return launch_lookup<float>(table, ld, rows, ids, ids_wide, tokens, dim, scale, out, ldo, s);
+  if (dtype == DTF_BF16) return launch_lookup<bf16_t>(table, ld, rows, ids, ids_wide, tokens, dim, scale, out, ldo, s);
+  return launch_lookup<f16_t>(table, ld, rows, ids, ids_wide, tokens, dim, scale, out, ldo, s);
+}
+
+extern "C" int64_t dtf_embed_workspace(int64_t tokens, int dim) {
+  if (tokens < 0 || tokens > kMaxTokens || dim < 1 || dim > kMaxDim) return -1;
+  return plan(tokens, dim).total;
+}
+
+static int embed_scatter(bool update, const void* ids, int ids_wide, int64_t tokens, const void* g, int64_t ldg, void* table,
+                         int dtype, int64_t rows, int dim, int64_t ldt, float scale, const float* lr, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  if (bad_shape(tokens, rows, dim, dtype) || ldt < dim || (tokens > 0 && ldg < dim)) return DTF_ERR_SHAPE;
+  if (!table || !workspace || (tokens > 0 && (!ids || !g)) || (update && !lr)) return DTF_ERR_NULL;
+  if (workspace_bytes < plan(tokens, dim).total || ((uintptr_t)workspace & 15u)) return DTF_ERR_SHAPE;
+  if (update && tokens == 0) return DTF_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DTF_F32)
+    return scatter_sums<float>(update, ids, ids_wide, tokens, g, ldg, table, ldt, rows, dim, scale, lr, workspace, s);
+  if (dtype == DTF_BF16)
+    return scatter_sums<bf16_t>(update, ids, ids_wide, tokens, g, ldg, table, ldt, rows, dim, scale, lr, workspace, s);
+  return scatter_sums<f16_t>(update, ids, ids_wide, tokens, g, ldg, table, ldt, rows, dim, scale, lr, workspace, s);
+}
+
+extern "C" int dtf_embed_grad(const void* ids, int ids_wide, int64_t tokens, const void* g, int64_t ldg, void* grad, int dtype,
+                              int64_t rows, int dim, int64_t ldt, float scale, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+  return embed_scatter(false, ids, ids_wide, tokens, g, ldg, grad, dtype, rows, dim, ldt, scale, nullptr, workspace,
+                       workspace_bytes, stream);
+}
+
+extern "C" int dtf_embed_sgd(const void* ids, int ids_wide, int64_t tokens, const void* g, int64_t ldg, void* table, int dtype,
+                             int64_t rows, int dim, int64_t ldt, float scale, const float* lr, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  return embed_scatter(true, ids, ids_wide, tokens, g, ldg, table, dtype, rows, dim, ldt, scale, lr, workspace, workspace_bytes,
+                       stream);
+}

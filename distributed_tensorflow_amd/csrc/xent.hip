@@ -1,0 +1,351 @@
+// Softmax cross-entropy over a vocabulary against INTEGER labels, loss and gradient: the output end of a model over tokens,
+// where a one-hot label matrix would be as large as the logits.
+//
+//   loss[t]  = log(sum_c exp z[t][c]) - z[t][l_t]
+//   dz[t][c] = w_t * (exp(z[t][c]) / sum_c' exp z[t][c'] - [c = l_t])        w_t = grad_scale, or the row's upstream gradient
+//
+// l_t < 0 is padding: loss 0, a gradient row of zeros, the logits are not looked at.  l_t >= classes: NaN loss and gradient
+// row (as the reference framework's op on a GPU).  A row with a NaN, a +inf or nothing but -inf has the loss and gradient NaN,
+// single -inf logits (masked classes) have probability zero.  Logits and dz in fp32, bf16 or fp16 (one rounding at the store),
+// everything in between in fp32.
+//
+// Bound by memory: one read of the logits and one write of the gradient.  A group of threads owns a row and keeps it in
+// REGISTERS between the sums and the gradient (64 bytes to 256 KB a row: up to 16 packs of 16 bytes for each of up to 1024 threads),
+// so the second use of a row costs no traffic.  Every thread finds the maximum of its own elements first and sums
+// exponentials relative to it; the pairs (maximum, sum) meet in one exchange: one barrier per row and not two.  Rows that do
+// not fit are streamed twice.  Rows may start at any element: packs are aligned to 16 bytes of memory, and the first and last
+// pack of a row are taken element by element.
+#include "dtf_api.h"
+#include "dtf_types.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+struct XentArgs {
+  int64_t tokens, classes;
+  int64_t ld, ldz;
+  const void* labels;
+  int wide;
+  float grad_scale;
+  const float* g;          // backward pass: upstream gradient of the rows
+  int64_t g_stride;
+  float* row_loss;         // may be null
+  float* stats;            // [tokens][2]: maximum and sum of exponentials relative to it (may be null)
+};
+
+// (maximum, sum of exponentials relative to it) of two disjoint sets.  A set of nothing but -inf (a thread past the end of
+// the row, masked classes) has the sum 0; so has a whole row of them, whose loss is NaN through m - z.
+__device__ __forceinline__ void merge(float& m, float& s, float om, float os) {
+  const float top = fmaxf(m, om), at = top == -INFINITY ? 0.f : top;
+  s = s * exp_of(m - at) + os * exp_of(om - at);
+  m = top;
+}
+
+// Over the G threads of a row (G = 64: a wave; otherwise the whole block).  The order of additions is fixed.
+template <int G>
+__device__ __forceinline__ void merge_row(float& m, float& s) {
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const float om = __shfl_xor(m, x), os = __shfl_xor(s, x);
+    merge(m, s, om, os);
+  }
+  // (two lanes that merge each other's pair may differ in the last bit of the sum: all take the first lane's)
+  s = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s)));
+  if (G > 64) {
+    __shared__ float2 of_wave[G / 64];
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = make_float2(m, s);
+    __syncthreads();
+    m = of_wave[0].x;
+    s = of_wave[0].y;
+#pragma unroll
+    for (int w = 1; w < G / 64; ++w) merge(m, s, of_wave[w].x, of_wave[w].y);
+  }
+}
+
+// One row as packs of 16 bytes aligned in memory; element e of pack i is class i * N + e - lead.
+template <typename T>
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  typedef Pack<T, N> P;
+  T* first;
+  int lead;
+  int classes;      // (a row has fewer than 2^31 elements)
+  int packs;
+  __device__ __forceinline__ Row(T* row, int64_t c) {
+    first = row;
+    lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+    classes = (int)c;
+    packs = (lead + classes + N - 1) / N;
+  }
+  __device__ __forceinline__ bool whole(int i) const { return i * N >= lead && i * N - lead + N <= classes; }
+  __device__ __forceinline__ bool inside(int c) const { return c >= 0 && c < classes; }
+  // V packs, `step` apart from pack i; outside the row: -inf.  The whole packs are requested first and together; the at most
+  // two partial ones of the row cost their threads a second round.
+  template <int V>
+  __device__ __forceinline__ void load(int i, int step, P (&p)[V]) const {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) p[k].v[e] = (T)(-INFINITY);
+      if (whole(i + k * step)) p[k] = *reinterpret_cast<const P*>(first + ((i + k * step) * N - lead));
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (i + k * step < packs && !whole(i + k * step)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int c = (i + k * step) * N + e - lead;
+          if (inside(c)) p[k].v[e] = first[c];
+        }
+      }
+    }
+  }
+};
+
+// Stores pack i of the row's gradient; `dst` has the logits' alignment modulo 16 bytes if SAME.
+template <typename T, bool SAME>
+__device__ __forceinline__ void store_pack(const Row<T>& row, T* dst, int i, const typename Row<T>::P& p) {
+  constexpr int N = Row<T>::N;
+  if (SAME && row.whole(i)) {
+    *reinterpret_cast<typename Row<T>::P*>(dst + (i * N - row.lead)) = p;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int c = i * N + e - row.lead;
+      if (row.inside(c)) dst[c] = p.v[e];
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ typename Row<T>::P gradient_pack(const Row<T>& row, int i, const typename Row<T>::P& z, float m,
+                                                            float factor, float weight, int label) {
+  typename Row<T>::P p;
+#pragma unroll
+  for (int e = 0; e < Row<T>::N; ++e) {
+    float d = factor * exp_of((float)z.v[e] - m);
+    if (i * Row<T>::N + e - row.lead == label) d -= weight;
+    p.v[e] = (T)d;
+  }
+  return p;
+}
+
+__device__ __forceinline__ int64_t label_of(const XentArgs& a, int64_t t) {
+  return a.wide ? static_cast<const int64_t*>(a.labels)[t] : (int64_t) static_cast<const int32_t*>(a.labels)[t];
+}
+
+// G threads per row (64: several rows per block), V packs per thread: the row fits G * V packs.
+template <typename T, int G, int V, bool SAME>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void xent_kernel(XentArgs a, T* logits, T* dz) {
+  constexpr int kRows = G < 256 ? 256 / G : 1;
+  typedef typename Row<T>::P P;
+  const int tid = threadIdx.x % G;
+  const int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / G;
+  if (t >= a.tokens) return;          // (a whole wave, or the whole block)
+  const Row<T> row(logits + t * a.ld, a.classes);
+  const int64_t label = label_of(a, t);
+  T* dst = dz + t * a.ldz;
+  if (label < 0 || label >= a.classes) {
+    const float fill = label < 0 ? 0.f : NAN;
+    if (dz) {
+      P p;
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) p.v[e] = (T)fill;
+      for (int i = tid; i < row.packs; i += G) store_pack<T, SAME>(row, dst, i, p);
+    }
+    if (tid == 0) {
+      if (a.row_loss) a.row_loss[t] = fill;
+      if (a.stats) a.stats[2 * t] = 0.f, a.stats[2 * t + 1] = 1.f;
+    }
+    return;
+  }
+  P z[V];
+  row.load(tid, G, z);
+  const float z_label = tid == 0 ? (float)row.first[label] : 0.f;     // (read before any thread of the row may store dz)
+  float m = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+#pragma unroll
+    for (int e = 0; e < Row<T>::N; ++e) m = fmaxf(m, (float)z[k].v[e]);
+  const float own = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+#pragma unroll
+    for (int e = 0; e < Row<T>::N; ++e) s += exp_of((float)z[k].v[e] - own);
+  merge_row<G>(m, s);
+  if (tid == 0) {
+    if (a.row_loss) a.row_loss[t] = (m - z_label) + logf(s);
+    if (a.stats) a.stats[2 * t] = m, a.stats[2 * t + 1] = s;
+  }
+  if (!dz) return;
+  const float factor = a.grad_scale / s;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    if (k * G + tid < row.packs)
+      store_pack<T, SAME>(row, dst, k * G + tid, gradient_pack<T>(row, k * G + tid, z[k], m, factor, a.grad_scale, (int)label));
+}
+
+// Rows of any length: two passes over memory (the first alone without dz).
+constexpr int kStream = 1024;
+template <typename T, bool SAME>
+__global__ __launch_bounds__(kStream) void xent_stream_kernel(XentArgs a, T* logits, T* dz) {
+  typedef typename Row<T>::P P;
+  const int tid = threadIdx.x;
+  const int64_t t = blockIdx.x;
+  const Row<T> row(logits + t * a.ld, a.classes);
+  const int64_t label = label_of(a, t);
+  const bool use = label >= 0 && label < a.classes;
+  T* dst = dz + t * a.ldz;
+  if (!use) {
+    const float fill = label < 0 ? 0.f : NAN;
+    if (dz) {
+      P p;
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) p.v[e] = (T)fill;
+      for (int i = tid; i < row.packs; i += kStream) store_pack<T, SAME>(row, dst, i, p);
+    }
+    if (tid == 0) {
+      if (a.row_loss) a.row_loss[t] = fill;
+      if (a.stats) a.stats[2 * t] = 0.f, a.stats[2 * t + 1] = 1.f;
+    }
+    return;
+  }
+  const float z_label = tid == 0 ? (float)row.first[label] : 0.f;
+  float m = -INFINITY, s = 0.f;
+  constexpr int U = 4;
+  for (int i0 = tid; i0 < row.packs; i0 += U * kStream) {
+    P z[U];
+    row.load(i0, kStream, z);
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) top = fmaxf(top, (float)z[k].v[e]);
+    const float own = top == -INFINITY ? 0.f : top;
+    s *= exp_of(m - own);             // (m = -inf: s is 0 and stays 0)
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) s += exp_of((float)z[k].v[e] - own);
+    m = top;
+  }
+  merge_row<kStream>(m, s);
+  if (tid == 0) {
+    if (a.row_loss) a.row_loss[t] = (m - z_label) + logf(s);
+    if (a.stats) a.stats[2 * t] = m, a.stats[2 * t + 1] = s;
+  }
+  if (!dz) return;
+  const float factor = a.grad_scale / s;
+  for (int i0 = tid; i0 < row.packs; i0 += U * kStream) {
+    P z[U];
+    row.load(i0, kStream, z);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (i0 + k * kStream < row.packs)
+        store_pack<T, SAME>(row, dst, i0 + k * kStream,
+                            gradient_pack<T>(row, i0 + k * kStream, z[k], m, factor, a.grad_scale, (int)label));
+  }
+}
+
+// The backward pass alone, from the statistics of the forward pass: a block takes kSlice packs of a row.
+constexpr int kGradPacks = 4, kGradThreads = 256, kSlice = kGradPacks * kGradThreads;
+template <typename T, bool SAME>
+__global__ __launch_bounds__(kGradThreads) void xent_grad_kernel(XentArgs a, T* logits, T* dz) {
+  typedef typename Row<T>::P P;
+  const int64_t t = blockIdx.x;
+  const Row<T> row(logits + t * a.ld, a.classes);
+  const int64_t label = label_of(a, t);
+  T* dst = dz + t * a.ldz;
+  const int i0 = blockIdx.y * kSlice + threadIdx.x;
+  const bool use = label >= 0 && label < a.classes;
+  P z[kGradPacks];
+  if (use) row.load(i0, kGradThreads, z);
+  const float weight = a.g[t * a.g_stride];
+  const float m = a.stats[2 * t], factor = weight / a.stats[2 * t + 1];
+#pragma unroll
+  for (int k = 0; k < kGradPacks; ++k) {
+    const int i = i0 + k * kGradThreads;
+    if (i >= row.packs) break;
+    P p;
+    if (use) {
+      p = gradient_pack<T>(row, i, z[k], m, factor, weight, (int)label);
+    } else {
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) p.v[e] = (T)(label < 0 ? 0.f : NAN);
+    }
+    store_pack<T, SAME>(row, dst, i, p);
+  }
+}
+
+template <typename T, bool SAME>
+int launch_xent(const XentArgs& a, T* logits, T* dz, hipStream_t s) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t packs = (a.classes + 2 * N - 2) / N;       // of a row that starts at the worst element
+  const unsigned rows = (unsigned)a.tokens;
+#define DTF_XENT(G, V)                                                                                           \
+  if (packs <= G * V) {                                                                                          \
+    xent_kernel<T, G, V, SAME><<<(rows + (G < 256 ? 256 / G : 1) - 1) / (G < 256 ? 256 / G : 1), G < 256 ? 256 : G, 0, s>>>(a, logits, dz); \
+    return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;                                            \
+  }
+  DTF_XENT(64, 1)
+  DTF_XENT(64, 4)
+  DTF_XENT(256, 4)
+  DTF_XENT(256, 8)
+  DTF_XENT(256, 16)
+  DTF_XENT(512, 16)
+  DTF_XENT(1024, 16)
+#undef DTF_XENT
+  xent_stream_kernel<T, SAME><<<rows, kStream, 0, s>>>(a, logits, dz);
+  return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
+}
+
+template <typename T>
+int run_xent(const XentArgs& a, const void* logits, void* dz, bool backward, hipStream_t s) {
+  T* z = static_cast<T*>(const_cast<void*>(logits));
+  T* d = static_cast<T*>(dz);
+  const bool same = !d || ((((uintptr_t)z ^ (uintptr_t)d) & 15u) == 0 && ((a.ld - a.ldz) * (int64_t)sizeof(T)) % 16 == 0);
+  if (backward) {
+    constexpr int N = 16 / sizeof(T);
+    const dim3 grid((unsigned)a.tokens, (unsigned)(((a.classes + 2 * N - 2) / N + kSlice - 1) / kSlice));
+    if (same) xent_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a, z, d);
+    else xent_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a, z, d);
+    return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
+  }
+  return same ? launch_xent<T, true>(a, z, d, s) : launch_xent<T, false>(a, z, d, s);
+}
+
+int checked(const XentArgs& a, const void* logits, int dtype, void* dz, bool backward, void* stream) {
+  // (grids stay below 2^32 threads, the class index of a row below 2^31)
+  if (a.tokens < 0 || a.tokens > (1 << 21) || a.classes < 1 || a.classes > (1 << 26) || dtype < 0 || dtype > 2 ||
+      a.ld < a.classes || (dz && a.ldz < a.classes))
+    return DTF_ERR_SHAPE;
+  if (a.tokens == 0) return DTF_OK;
+  if (!logits || !a.labels || (backward && (!dz || !a.stats || !a.g))) return DTF_ERR_NULL;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DTF_F32) return run_xent<float>(a, logits, dz, backward, s);
+  if (dtype == DTF_BF16) return run_xent<bf16_t>(a, logits, dz, backward, s);
+  return run_xent<f16_t>(a, logits, dz, backward, s);
+}
+
+}  // namespace
+
+extern "C" int dtf_sparse_xent(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                               int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats,
+                               void* stream) {
+  XentArgs a{};
+  a.tokens = tokens, a.classes = classes, a.ld = ld, a.ldz = dz ? ldz : ld;
+  a.labels = labels, a.wide = labels_wide, a.grad_scale = grad_scale, a.row_loss = row_loss, a.stats = stats;
+  return checked(a, logits, dtype, dz, false, stream);
+}
+
+extern "C" int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                                    int labels_wide, const float* stats, const float* g, int64_t g_stride, void* dz, int64_t ldz,
+                                    void* stream) {
+  XentArgs a{};
+  a.tokens = tokens, a.classes = classes, a.ld = ld, a.ldz = ldz;
+  a.labels = labels, a.wide = labels_wide, a.g = g, a.g_stride = g_stride, a.stats = const_cast<float*>(stats);
+  return checked(a, logits, dtype, dz, true, stream);
+}

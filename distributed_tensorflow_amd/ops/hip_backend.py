@@ -161,6 +161,15 @@ def _declare(lib: C.CDLL) -> None:
     for name in ("dtf_gemm_f32", "dtf_colsum", "dtf_softmax_xent", "dtf_dense_step_begin", "dtf_softmax_xent_step",
                  "dtf_softmax_xent_head"):
         getattr(lib, name).restype = C.c_int
+    lib.dtf_embed_lookup.argtypes = [vp, i32, i64, i32, i64, vp, i32, i64, f32, vp, i64, vp]
+    lib.dtf_embed_workspace.argtypes = [i64, i32]
+    lib.dtf_embed_workspace.restype = i64
+    lib.dtf_embed_grad.argtypes = [vp, i32, i64, vp, i64, vp, i32, i64, i32, i64, f32, vp, i64, vp]
+    lib.dtf_embed_sgd.argtypes = [vp, i32, i64, vp, i64, vp, i32, i64, i32, i64, f32, vp, vp, i64, vp]
+    lib.dtf_sparse_xent.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, f32, vp, vp, vp]
+    lib.dtf_sparse_xent_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, vp, i64, vp, i64, vp]
+    for name in ("dtf_embed_lookup", "dtf_embed_grad", "dtf_embed_sgd", "dtf_sparse_xent", "dtf_sparse_xent_grad"):
+        getattr(lib, name).restype = C.c_int
     lib.dtf_debug_force_generic_path.argtypes = [i32]
     lib.dtf_debug_force_generic_path.restype = None
     lib.dtf_debug_set_fwd_tile8.argtypes = [i32]
@@ -266,6 +275,39 @@ def _f32c(t: torch.Tensor, name: str) -> torch.Tensor:
     if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous():
         raise HipKernelError(f"{name} must be a contiguous float32 CUDA tensor, got {t.dtype} {t.device}")
     return t
+
+
+# ---------------------------------------------------------------------------
+# operands of the token-model operators (ops/embedding.py, ops/xent.py, ops/muon.py)
+# ---------------------------------------------------------------------------
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DTF_F32, DTF_BF16, DTF_F16
+
+
+def typed_rows(t: torch.Tensor, name: str) -> int:
+    """Row stride in elements of a 2-D fp32 / bf16 / fp16 GPU matrix with contiguous rows; anything else is refused."""
+    if not t.is_cuda or t.dtype not in TYPE_CODES or t.dim() != 2:
+        raise HipKernelError(f"{name} must be a 2-D float32, bfloat16 or float16 CUDA tensor, got {t.dtype} {tuple(t.shape)} "
+                             f"on {t.device}")
+    cols = t.shape[1]
+    if cols > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols:
+        raise HipKernelError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()} for {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(cols, 1)
+
+
+def int_vector(t: torch.Tensor, name: str, device) -> torch.Tensor:
+    """``t`` (int32 or int64, any shape, on ``device``) as a contiguous vector."""
+    if t.dtype not in (torch.int32, torch.int64) or t.device != device:
+        raise HipKernelError(f"{name} must be an int32 or int64 tensor on {device}, got {t.dtype} on {t.device}")
+    return t.reshape(-1).contiguous()
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        n = 1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 # ---------------------------------------------------------------------------

@@ -1,0 +1,93 @@
+"""Softmax cross-entropy against integer labels (csrc/xent.hip): the output end of a model over tokens, where the one-hot
+labels of ``hip_backend.softmax_xent`` would be a matrix as large as the logits.
+
+``sparse_softmax_xent(logits, labels)`` is the differentiable operator: the loss of every row
+(``tf.nn.sparse_softmax_cross_entropy_with_logits`` of a graph evaluates to it).  ``sparse_softmax_xent_step`` is the training
+step's form: losses and gradient in ONE launch that reads the logits once and keeps each row in registers in between.
+
+A negative label is padding: loss 0, a gradient row of zeros, the row's logits are not looked at.  A label that is no class
+(``>= classes``) gives NaN.  Logits in float32, bfloat16 or float16 with contiguous rows; losses in float32.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import hip_backend as hb
+
+
+def _operands(logits: torch.Tensor, labels: torch.Tensor):
+    ld = hb.typed_rows(logits, "logits")
+    flat = hb.int_vector(labels, "labels", logits.device)
+    if labels.dim() != 1 or flat.numel() != logits.shape[0]:
+        raise hb.HipKernelError(f"sparse_softmax_xent: one label per row of the logits, got {tuple(labels.shape)} for "
+                                f"{tuple(logits.shape)}")
+    return ld, flat
+
+
+def _dz_rows(dz: torch.Tensor, logits: torch.Tensor) -> int:
+    if dz.shape != logits.shape or dz.dtype != logits.dtype or dz.device != logits.device:
+        raise hb.HipKernelError("sparse_softmax_xent: dz must be shaped and typed like the logits, on their device")
+    if hb.overlap(dz, logits) and (dz.data_ptr() != logits.data_ptr() or dz.stride() != logits.stride()):
+        raise hb.HipKernelError("sparse_softmax_xent: dz may be the logits themselves, but not overlap them otherwise")
+    return hb.typed_rows(dz, "dz")
+
+
+def _forward(logits, labels, dz, grad_scale, stats):
+    lib = hb.require()
+    ld, flat = _operands(logits, labels)
+    ldz = 0 if dz is None else _dz_rows(dz, logits)
+    loss = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
+    hb._check(lib.dtf_sparse_xent(logits.data_ptr(), hb.TYPE_CODES[logits.dtype], logits.shape[0], logits.shape[1], ld,
+                                  flat.data_ptr(), int(flat.dtype == torch.int64), hb._ptr(dz), ldz, float(grad_scale),
+                                  loss.data_ptr(), hb._ptr(stats), hb._stream(logits)), "dtf_sparse_xent")
+    return loss, flat
+
+
+def sparse_softmax_xent_step(logits: torch.Tensor, labels: torch.Tensor, *, dz: Optional[torch.Tensor] = None,
+                             grad_scale: float = 1.0) -> torch.Tensor:
+    """Row losses (float32 ``[rows]``); ``dz`` (shaped like the logits, or the logits themselves) receives
+    ``grad_scale * d(row loss)/d(logits)`` in the same launch."""
+    return _forward(logits, labels, dz, grad_scale, None)[0]
+
+
+class _SparseXent(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels):
+        z = logits.detach()
+        stats = torch.empty((z.shape[0], 2), device=z.device, dtype=torch.float32)
+        loss, flat = _forward(z, labels, None, 1.0, stats)
+        ctx.save_for_backward(logits, flat, stats)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, flat, stats = ctx.saved_tensors
+        z = logits.detach()
+        g = g.to(torch.float32)
+        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        hb._check(hb.require().dtf_sparse_xent_grad(z.data_ptr(), hb.TYPE_CODES[z.dtype], z.shape[0], z.shape[1],
+                                                    hb.typed_rows(z, "logits"), flat.data_ptr(), int(flat.dtype == torch.int64),
+                                                    stats.data_ptr(), g.data_ptr(), g.stride(0), dz.data_ptr(), z.shape[1],
+                                                    hb._stream(z)), "dtf_sparse_xent_grad")
+        return dz, None
+
+
+def sparse_softmax_xent(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+    """Loss of every row, differentiable in the logits (GPU: the kernels above; CPU tensors: torch, same rules)."""
+    if logits.is_cuda:
+        rows = logits if logits.dim() != 2 or logits.shape[1] == 1 or logits.stride(1) == 1 else logits.contiguous()
+        return _SparseXent.apply(rows, labels)
+    if logits.dim() != 2 or labels.dim() != 1 or labels.shape[0] != logits.shape[0]:
+        raise ValueError("sparse_softmax_xent: one label per row of 2-D logits")
+    classes = logits.shape[1]
+    known = (labels >= 0) & (labels < classes)
+    at = torch.where(known, labels, torch.zeros_like(labels)).long()
+    # (the rows without a class are left out before the softmax, so that their logits cannot reach anything)
+    z = torch.where(known[:, None], logits.float(), torch.zeros_like(logits, dtype=torch.float32))
+    loss = -torch.log_softmax(z, dim=1).gather(1, at[:, None])[:, 0]
+    loss = torch.where(known, loss, torch.zeros_like(loss))
+    wrong = labels >= classes
+    nan = (torch.where(wrong[:, None], logits.float(), torch.zeros_like(z)) * float("nan")).sum(1)
+    return torch.where(wrong, nan, loss)
