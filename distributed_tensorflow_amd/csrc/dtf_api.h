@@ -275,6 +275,18 @@ int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t 
                          int labels_wide, const float* stats, const float* g, int64_t g_stride, void* dz, int64_t ldz,
                          void* stream);
 
+// Orthogonalised (Muon) update of up to DTF_MUON_MAX fp32 matrices [rows][cols] in one sequence of launches (muon.hip):
+//   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  w -= lr[0] * sqrt(max(1, cols / rows)) * factor(u)
+// factor: five Newton-Schulz steps on u / (|u|_F + eps).  HOST arrays of shapes and device addresses; workspace of
+// dtf_muon_workspace bytes, 256-byte aligned, contents unimportant, not shared by calls that may run at the same time.
+#define DTF_MUON_MAX 8
+int64_t dtf_muon_workspace(int count, const int32_t* rows, const int32_t* cols);
+int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols, const uint64_t* w, const uint64_t* g, const uint64_t* buf,
+                  const float* lr, float momentum, int nesterov, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+// out = factor(x), dtype as above (workspace: dtf_muon_workspace of the one shape)
+int dtf_orthogonalize(const void* x, int dtype, int rows, int cols, int64_t ldx, void* out, int64_t ldo, float eps,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 int dtf_abi_sizeof(int which);   // sizeof of DtfMlpDesc (0), DtfPipeDesc (1), DtfXgDesc (2)
 const char* dtf_hip_build_info(void);
 

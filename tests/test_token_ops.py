@@ -90,3 +90,35 @@ def test_cross_entropy_on_the_cpu():
     loss = xent.sparse_softmax_xent(z, labels)
     (g,) = torch.autograd.grad(loss, z, torch.ones(6))
     assert loss[2] == 0 and bool((g[2] == 0).all()) and loss[0] == 0 and bool((g[0] == 0).all()) and torch.allclose(g[3], w[3])
+
+
+def test_native_refusals_of_the_orthogonalised_update():
+    import ctypes as C
+
+    from distributed_tensorflow_amd.ops import muon
+
+    lib = hb.require()
+    one = 4096
+    r, c = (C.c_int32 * 9)(*[8] * 9), (C.c_int32 * 9)(*[6] * 9)
+    need = lib.dtf_muon_workspace(1, r, c)
+    assert need > 0 and lib.dtf_muon_workspace(0, r, c) == lib.dtf_muon_workspace(9, r, c) == lib.dtf_muon_workspace(1, None, c) == -1
+    assert lib.dtf_muon_workspace(1, (C.c_int32 * 1)(0), c) == lib.dtf_muon_workspace(1, (C.c_int32 * 1)(1 << 17), c) == -1
+
+    def factor(dtype=0, rows=8, cols=6, ldx=6, ldo=6, eps=0.0, x=one, o=one, ws=one, size=need):
+        return lib.dtf_orthogonalize(x, dtype, rows, cols, ldx, o, ldo, eps, ws, size, None)
+
+    assert factor(dtype=3) == factor(rows=0) == factor(cols=0) == factor(ldx=5) == factor(ldo=5) == factor(eps=-1.0) == SHAPE
+    assert factor(eps=float("nan")) == factor(size=need - 1) == factor(ws=one + 16) == SHAPE
+    assert factor(x=None) == factor(o=None) == factor(ws=None) == NULL
+    p = (C.c_uint64 * 9)(*[one] * 9)
+    null = (C.c_uint64 * 9)()
+
+    def step(n=1, w=p, g=p, b=p, lr=one, eps=0.0, ws=one, size=need):
+        return lib.dtf_muon_step(n, r, c, w, g, b, lr, 0.9, 1, eps, ws, size, None)
+
+    assert step(n=0) == step(n=9) == step(eps=-1.0) == step(size=need - 1) == step(ws=one + 16) == SHAPE
+    assert step(w=None) == step(lr=None) == step(ws=None) == step(w=null) == step(g=null) == step(b=null) == NULL
+    with pytest.raises(hb.HipKernelError):
+        muon.orthogonalize(torch.zeros(3, 4))
+    with pytest.raises(hb.HipKernelError):
+        muon.MuonPlan([torch.zeros(3, 4)], [torch.zeros(3, 4)], [torch.zeros(3, 4)])
