@@ -280,6 +280,7 @@ int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t 
 // factor: five Newton-Schulz steps on u / (|u|_F + eps).  HOST arrays of shapes and device addresses; workspace of
 // dtf_muon_workspace bytes, 256-byte aligned, contents unimportant, not shared by calls that may run at the same time.
 #define DTF_MUON_MAX 8
+void dtf_debug_set_muon_cut(int edge, int splits);
 int64_t dtf_muon_workspace(int count, const int32_t* rows, const int32_t* cols);
 int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols, const uint64_t* w, const uint64_t* g, const uint64_t* buf,
                   const float* lr, float momentum, int nesterov, float eps, void* workspace, int64_t workspace_bytes, void* stream);

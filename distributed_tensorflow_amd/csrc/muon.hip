@@ -24,14 +24,19 @@
 // GEMM form (row times row) serves all.  A row of a plane pair is groups of 32 columns: 32 hi halves then 32 lo halves, 128
 // bytes, one cache line per row and k-step.  Dimensions are padded with zeros to whole tiles: the products need no bounds.
 //
-// GEMM.  A workgroup owns a tile and walks k in steps of 32 through two LDS images filled by direct global-to-LDS loads (the
-// load of step k + 1 is in flight while step k is multiplied; one barrier per step).  A load instruction moves eight 128-byte rows;
-// its LDS side is fixed (lane l at 16 l), so the 16-byte chunks of a row are permuted on the GLOBAL side: slot s of row r holds
-// chunk s ^ (r & 7), and the 32 rows a fragment read touches spread over all banks.  Few tiles and a long k: several
-// workgroups split the k range of a tile and the last to arrive adds the partial sums in their order.
+// GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 and walks k in steps of 32 through two LDS images
+// filled by direct buffer-to-LDS loads.  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so
+// the 16-byte chunks of a row are permuted on the GLOBAL side: slot s of row r holds chunk s ^ (r & 7), and the rows that a
+// fragment read touches spread over the banks.  A step's two halves of 16 k alternate between two sets of fragment
+// registers: while one half is multiplied the next half's LDS reads are under way, across the step's single barrier too, and
+// the loads of step k + 2 go into the image that the barrier has just freed.  Large tiles matter here: per k-step of a tile
+// of edge T the matrix cores are busy for 0.047 T^2 cycles and the LDS for 6 T cycles (reads by four waves of T/2 x T/2, and the
+// loads): 100 % of the matrix time at 128, 50 % at 256.  Tile edge and split of k are chosen per stage by a cost
+// estimate (see choose()).  Few tiles and a long k: several workgroups take a range of k each and store their sums; a second
+// launch adds them in order and does what the product's own end does otherwise.
 //
-// All matrices of a call go through each launch together: 2 + 15 launches per step of the optimiser, whatever the number of
-// layers (up to 8; more are taken in groups).
+// All matrices of a call go through each launch together: 2 + 15 launches per step of the optimiser (up to 15 more where k is
+// split), whatever the number of layers (up to 8; more are taken in groups).
 #include "dtf_api.h"
 #include "dtf_types.h"
 
@@ -45,8 +50,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kMax = DTF_MUON_MAX;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleX = 32768.f, kScaleA = 16384.f, kScaleB = 8192.f;    // powers of two: entries stay below 65504
-constexpr int kNormBlocks = 128;
-constexpr int kMaxTickets = 4096;
+constexpr int kNormBlocks = 1024;     // at most
+constexpr int kWaves = 4;              // of a product workgroup
 
 // One matrix of a call.  `rows` x `cols` as the caller has it; m <= n its shape (or its transpose's) padded to mp x np.
 struct Item {
@@ -57,7 +62,7 @@ struct Item {
   int rows, cols, m, n, mp, np, flip;
   float shape_factor;   // sqrt(max(1, cols / rows))
   char *X, *XT[2], *A, *B;
-  double* norm;         // [kNormBlocks] partial sums of squares
+  double* norm;         // partial sums of squares
 };
 
 struct Call {
@@ -65,8 +70,8 @@ struct Call {
   int count, dtype;
   float mu, eps;
   int nesterov;
+  int norm_blocks;
   const float* lr;
-  uint32_t* tickets;
   float* partial;       // split products: [tile][split][elements of a tile]
 };
 
@@ -82,11 +87,28 @@ __device__ __forceinline__ float direction(const Call& c, const Item& it, int64_
 template <typename T>
 __global__ __launch_bounds__(256) void norm_kernel(Call c) {
   const Item& it = c.item[blockIdx.y];
-  if (blockIdx.y == 0)
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < kMaxTickets; i += kNormBlocks * 256) c.tickets[i] = 0;
-  const int64_t total = (int64_t)it.rows * it.cols;
+  const int64_t total = (int64_t)it.rows * it.cols, stride = (int64_t)gridDim.x * 256;
+  const int64_t me = (int64_t)blockIdx.x * 256 + threadIdx.x;
   double sum = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += kNormBlocks * 256) {
+  // four elements at a time where the matrix has no gaps and is aligned; the rest, or all of a strided one, one by one
+  const bool flat = it.ldu == it.cols && (reinterpret_cast<uintptr_t>(it.u) % (4 * sizeof(T))) == 0 &&
+                    (reinterpret_cast<uintptr_t>(it.buf) & 15u) == 0;
+  const int64_t quads = flat ? total / 4 : 0;
+  for (int64_t q = me; q < quads; q += stride) {
+    const Pack<T, 4> g = reinterpret_cast<const Pack<T, 4>*>(it.u)[q];
+    f32x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = (float)g.v[e];
+    if (it.buf) {
+      f32x4* at = reinterpret_cast<f32x4*>(it.buf) + q;
+      const f32x4 b = c.mu * *at + u;
+      *at = b;
+      u = c.nesterov ? u + c.mu * b : b;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += (double)u[e] * (double)u[e];
+  }
+  for (int64_t i = 4 * quads + me; i < total; i += stride) {
     int64_t at = i;
     if (it.ldu != it.cols) {
       const int64_t r = i / it.cols;
@@ -131,20 +153,19 @@ __device__ __forceinline__ void store_group(char* group, const uint32_t* pairs, 
 template <typename T>
 __global__ __launch_bounds__(256) void split_kernel(Call c) {
   __shared__ uint32_t tile[64][65];
-  __shared__ double inv_s;
+  __shared__ double of_wave[4];
   const Item& it = c.item[blockIdx.y];
   const int pr = it.flip ? it.np : it.mp, pc = it.flip ? it.mp : it.np;       // padded rows and columns as the caller has them
   const int tiles_c = pc / 64, tiles = (pr / 64) * tiles_c;
   if ((int)blockIdx.x >= tiles) return;
   const int r0 = (blockIdx.x / tiles_c) * 64, c0 = (blockIdx.x % tiles_c) * 64;
-  if (threadIdx.x < 64) {
-    double s = it.norm[threadIdx.x] + it.norm[threadIdx.x + 64];
+  double total = 0;
+  for (int i = threadIdx.x; i < c.norm_blocks; i += 256) total += it.norm[i];
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) s += __shfl_xor(s, x);
-    if (threadIdx.x == 0) inv_s = (double)kScaleX / (sqrt(s) + (double)c.eps);
-  }
+  for (int x = 32; x > 0; x >>= 1) total += __shfl_xor(total, x);
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = total;
   __syncthreads();
-  const double inv = inv_s;
+  const double inv = (double)kScaleX / (sqrt((of_wave[0] + of_wave[1]) + (of_wave[2] + of_wave[3])) + (double)c.eps);
 #pragma unroll 4
   for (int k = 0; k < 16; ++k) {
     const int r = (threadIdx.x >> 6) + 4 * k, col = threadIdx.x & 63;
@@ -165,9 +186,9 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
 enum Stage { kGram = 0, kPoly = 1, kStep = 2, kLast = 3 };     // A = X X^T;  B = bA + cAA;  X = aX + BX;  the same, to the output
 
 struct Tiles {
-  int first[kMax + 1];     // first workgroup of every matrix
-  int splits[kMax];
-  int ticket0[kMax];       // first ticket, and first tile of the partial sums
+  int first[kMax + 1];     // first workgroup (finish: first wave) of every matrix
+  int64_t tile0[kMax];     // first tile of the partial sums
+  int splits;              // workgroups per tile
 };
 
 // This wave's loads have landed and its LDS reads are done, then the workgroup's.  (0x0070: vmcnt 0, lgkmcnt 0.  A barrier alone
@@ -177,23 +198,37 @@ __device__ __forceinline__ void wait_and_barrier() {
   __syncthreads();
 }
 
-// ROWS rows of a plane pair, the 128-byte group `k` of each, to an LDS image; W waves.
-template <int ROWS, int W>
-__device__ __forceinline__ void fetch(const char* src, int64_t row_bytes, char* __restrict lds, int wave, int lane, int k) {
-  const char* at = src + (int64_t)(wave * 8 + (lane >> 3)) * row_bytes + (int64_t)k * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+// ROWS rows of a plane pair from a tile's first row on; rows past the last one are read as the last one (their products are not
+// stored).
+template <int ROWS>
+struct Fetcher {
+  static constexpr int kLoads = ROWS / (8 * kWaves);
+  const char* base;
+  unsigned at[kLoads];
+  __device__ __forceinline__ void init(const char* plane, int row0, int rows, int64_t row_bytes, int wave, int lane) {
+    base = plane + row0 * row_bytes;
 #pragma unroll
-  for (int i = 0; i < ROWS / (8 * W); ++i)
-    __builtin_amdgcn_global_load_lds((global_void*)(at + (int64_t)i * 8 * W * row_bytes), (lds_void*)(lds + (i * W + wave) * 1024), 16, 0, 0);
-}
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+      at[i] = (unsigned)(min(r, rows - 1 - row0) * row_bytes) + (unsigned)(((lane & 7) ^ (lane >> 3)) << 4);
+    }
+  }
+  // The 128-byte group `k` of every row to an LDS image.
+  __device__ __forceinline__ void go(char* __restrict lds, int wave, int k) const {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)0xffffffffu, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + (i * kWaves + wave) * 1024), 16, at[i], k * 128, 0, 0);
+  }
+};
 
-// One k-step of 32: a wave's MI x NI tiles of 32 x 32.  `p` and `q`: LDS images of the workgroup's rows of the two operands.
+// Operands of one half of a k-step (16 k): MI and NI tiles of 32 rows, hi and lo.
 template <int MI, int NI>
-__device__ __forceinline__ void multiply(const char* __restrict p, const char* __restrict q, f32x16 (&acc)[MI][NI], int row_p,
-                                         int row_q, int lane) {
-  const int r = lane & 31;
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    half8 a[MI][2], b[NI][2];
+struct Half {
+  half8 a[MI][2], b[NI][2];
+  // `p`, `q`: LDS images of the workgroup's rows of the two operands
+  __device__ __forceinline__ void read(const char* __restrict p, const char* __restrict q, int row_p, int row_q, int lane, int ks) {
+    const int r = lane & 31;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int slot = ((h * 4 + ks * 2 + (lane >> 5)) ^ (r & 7)) << 4;      // (every base row is a multiple of 32)
@@ -202,7 +237,9 @@ __device__ __forceinline__ void multiply(const char* __restrict p, const char* _
 #pragma unroll
       for (int j = 0; j < NI; ++j) b[j][h] = *reinterpret_cast<const half8*>(q + (row_q + 32 * j + r) * 128 + slot);
     }
-    // the small products first; a tile's three MFMAs are MI * NI apart
+  }
+  // hi lo, lo hi, hi hi; the three MFMAs of a tile are MI * NI apart
+  __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
 #pragma unroll
     for (int t = 0; t < 3; ++t)
 #pragma unroll
@@ -211,42 +248,100 @@ __device__ __forceinline__ void multiply(const char* __restrict p, const char* _
         for (int j = 0; j < NI; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][t == 1], b[j][t == 0], acc[i][j], 0, 0, 0);
   }
+};
+
+// What becomes of a 32 x 32 tile of a stage's product at (i0, j0).  Element e of `sum`: row 8 (e / 4) + 4 (lane / 32) + e % 4
+// and column lane % 32.  `turn`: 32 x 33 words of LDS that this wave alone uses.  `mirror`: also store the transposed tile of a
+// symmetric result.
+__device__ __forceinline__ void store_tile(const Call& c, const Item& it, int stage, int parity, int i0, int j0, bool mirror,
+                                           const f32x16& sum, uint32_t* turn, int lane) {
+  const int half = lane >> 5, jc = lane & 31;
+  float v[16];
+  if (stage == kGram) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = sum[e] * (kScaleA / (kScaleX * kScaleX));
+  } else {
+    // the matrix in the linear term, through its transpose: 4 consecutive rows of one column are 8 + 8 bytes
+    const char* s = (stage == kPoly ? it.A : it.XT[parity]) + plane_at(j0 + jc, i0, it.mp) + 8 * half;
+    const float lin = stage == kPoly ? kB * (kScaleB / kScaleA) : stage == kStep ? kA : kA / kScaleX;
+    const float quad = stage == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
+                       : stage == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const half4 hi = *reinterpret_cast<const half4*>(s + 16 * g), lo = *reinterpret_cast<const half4*>(s + 64 + 16 * g);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[4 * g + x] = lin * ((float)hi[x] + (float)lo[x]) + quad * sum[4 * g + x];
+    }
+  }
+  if (stage == kLast) {
+    const float step_size = it.buf ? c.lr[0] * it.shape_factor : 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = i0 + 8 * (e / 4) + 4 * half + e % 4, col = j0 + jc;
+      if (row < it.m && col < it.n) {
+        const int64_t at = it.flip ? (int64_t)col * it.ldo + row : (int64_t)row * it.ldo + col;
+        if (it.buf) {
+          float* w = static_cast<float*>(it.out) + at;
+          *w -= step_size * v[e];
+        } else if (c.dtype == DTF_F32) {
+          static_cast<float*>(it.out)[at] = v[e];
+        } else if (c.dtype == DTF_BF16) {
+          static_cast<bf16_t*>(it.out)[at] = (bf16_t)v[e];
+        } else {
+          static_cast<f16_t*>(it.out)[at] = (f16_t)v[e];
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) turn[(8 * (e / 4) + 4 * half + e % 4) * 33 + jc] = split_pair(v[e]);
+  // (a wave's own tile: no barrier, only the order of its own LDS accesses)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  const int line = lane >> 1, part = lane & 1;
+  char* straight = stage == kGram ? it.A : stage == kPoly ? it.B : it.X;
+  char* turned = stage == kGram ? it.A : stage == kPoly ? it.B : it.XT[parity ^ 1];
+  store_group(straight + plane_at(i0 + line, j0, stage <= kPoly ? it.mp : it.np), turn + line * 33, 1, part);
+  if (mirror) store_group(turned + plane_at(j0 + line, i0, it.mp), turn + line, 33, part);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-template <int TILE, int WM, int WN, typename T>
-__global__ __launch_bounds__(WM * WN * 64) void product_kernel(Call c, Tiles tl, int stage, int parity) {
-  constexpr int W = WM * WN, MI = TILE / WM / 32, NI = TILE / WN / 32;
+// Tile `t` of a stage: rows and columns in tiles.  Symmetric results: t = tj (tj + 1) / 2 + ti, ti <= tj.
+__device__ __forceinline__ void tile_place(const Item& it, int stage, int edge, int t, int& ti, int& tj) {
+  if (stage <= kPoly) {
+    tj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (tj * (tj + 1) / 2 > t) --tj;
+    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
+    ti = t - tj * (tj + 1) / 2;
+  } else {
+    const int tiles_m = (it.mp + edge - 1) / edge;
+    tj = t / tiles_m;
+    ti = t - tj * tiles_m;
+  }
+}
+
+template <int TILE>
+__global__ __launch_bounds__(kWaves * 64, TILE <= 64 ? 4 : TILE <= 128 ? 2 : 1) void product_kernel(Call c, Tiles tl, int stage, int parity) {
+  constexpr int MI = TILE / 64, NI = TILE / 64;
   constexpr int kImage = TILE * 128;
-  constexpr int kStage = W * 32 * 33 * 4;                        // a 32 x 33 word tile per wave
-  __shared__ __attribute__((aligned(1024))) char image0[2 * kImage > kStage ? 2 * kImage : kStage];
+  constexpr int kTurn = kWaves * 32 * 33 * 4;                        // a 32 x 33 word tile per wave
+  __shared__ __attribute__((aligned(1024))) char image0[2 * kImage > kTurn ? 2 * kImage : kTurn];
   __shared__ __attribute__((aligned(1024))) char image1[2 * kImage];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int which = 0;
   while ((int)blockIdx.x >= tl.first[which + 1]) ++which;
   const Item& it = c.item[which];
-  const int splits = tl.splits[which], local = blockIdx.x - tl.first[which];
-  const int tile = local / splits, part = local - tile * splits;
-  const bool symmetric = stage <= kPoly;
+  const int local = blockIdx.x - tl.first[which], tile = local / tl.splits, part = local - tile * tl.splits;
   int ti, tj;
-  if (symmetric) {                      // tile t = tj (tj + 1) / 2 + ti, ti <= tj
-    tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while (tj * (tj + 1) / 2 > tile) --tj;
-    while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
-    ti = tile - tj * (tj + 1) / 2;
-  } else {
-    const int tiles_m = it.mp / TILE;
-    tj = tile / tiles_m;
-    ti = tile - tj * tiles_m;
-  }
-  const char* P = stage == kGram ? it.X : stage == kPoly ? it.A : it.B;
-  const char* Q = stage == kGram ? it.X : stage == kPoly ? it.A : it.XT[parity];
+  tile_place(it, stage, TILE, tile, ti, tj);
   const int depth = stage == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
   const int64_t row_bytes = (int64_t)depth * 4;
-  const char* p = P + (int64_t)ti * TILE * row_bytes;
-  const char* q = Q + (int64_t)tj * TILE * row_bytes;
+  Fetcher<TILE> p, q;
+  p.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
+  q.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.XT[parity], tj * TILE, stage <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
   const int pairs = depth / 64;
-  const int k_first = 2 * (int)((int64_t)pairs * part / splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / splits);
-  const int row_p = (wave / WN) * (TILE / WM), row_q = (wave % WN) * (TILE / WN);
+  const int k_first = 2 * (int)((int64_t)pairs * part / tl.splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / tl.splits);
+  const int row_p = (wave >> 1) * (TILE / 2), row_q = (wave & 1) * (TILE / 2);
 
   f32x16 acc[MI][NI];
 #pragma unroll
@@ -255,137 +350,119 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Call c, Tiles tl,
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  fetch<TILE, W>(p, row_bytes, image0, wave, lane, k_first);
-  fetch<TILE, W>(q, row_bytes, image0 + kImage, wave, lane, k_first);
-  for (int k = k_first; k < k_last; k += 2) {
-    // every load of image 0 has landed, and every wave is done with image 1
-    wait_and_barrier();
-    fetch<TILE, W>(p, row_bytes, image1, wave, lane, k + 1);
-    fetch<TILE, W>(q, row_bytes, image1 + kImage, wave, lane, k + 1);
-    __builtin_amdgcn_sched_barrier(0);       // (the loads go out before the step's LDS reads, not after them)
-    multiply<MI, NI>(image0, image0 + kImage, acc, row_p, row_q, lane);
-    wait_and_barrier();
-    if (k + 2 < k_last) {
-      fetch<TILE, W>(p, row_bytes, image0, wave, lane, k + 2);
-      fetch<TILE, W>(q, row_bytes, image0 + kImage, wave, lane, k + 2);
+  Half<MI, NI> first, second;
+  if (k_first < k_last) {                      // (a matrix with fewer steps than parts: this part's sums are zeros)
+    p.go(image0, wave, k_first);
+    q.go(image0 + kImage, wave, k_first);
+    // Two steps a turn.  The scheduling barriers keep the LDS reads and the loads in front of the products that cover them.  (The
+    // turn begins at a full wait because the compiler adds one where the loop is entered: elsewhere it would cut into the loads.)
+#pragma clang loop unroll(disable)
+    for (int k = k_first; k < k_last; k += 2) {
+      wait_and_barrier();                      // image 0 has landed, every wave is done with image 1
+      p.go(image1, wave, k + 1);
+      q.go(image1 + kImage, wave, k + 1);
+      first.read(image0, image0 + kImage, row_p, row_q, lane, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (k > k_first) second.multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
+      second.read(image0, image0 + kImage, row_p, row_q, lane, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      first.multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_and_barrier();                      // image 1 has landed, every wave is done with image 0
+      if (k + 2 < k_last) {
+        p.go(image0, wave, k + 2);
+        q.go(image0 + kImage, wave, k + 2);
+      }
+      first.read(image1, image1 + kImage, row_p, row_q, lane, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      second.multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
+      second.read(image1, image1 + kImage, row_p, row_q, lane, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      first.multiply(acc);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    multiply<MI, NI>(image1, image1 + kImage, acc, row_p, row_q, lane);
+    second.multiply(acc);
+    wait_and_barrier();                        // every wave is done with the images
   }
 
-  if (splits > 1) {
-    constexpr int kElems = TILE * TILE;
-    float* mine = c.partial + ((int64_t)tl.ticket0[which] + (int64_t)tile * splits) * kElems;
+  if (tl.splits > 1) {
+    float* to = c.partial + ((tl.tile0[which] + tile) * tl.splits + part) * (TILE * TILE) + wave * (TILE * TILE / 4) + lane * 4;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<f32x4*>(mine + (int64_t)part * kElems + (((i * NI + j) * 4 + e / 4) * W * 64 + tid) * 4) =
+          *reinterpret_cast<f32x4*>(to + ((i * NI + j) * 4 + e / 4) * 256) =
               f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-    __threadfence();
-    __syncthreads();
-    __shared__ uint32_t arrived;
-    uint32_t* ticket = c.tickets + tl.ticket0[which] + tile;
-    if (tid == 0) arrived = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if ((int)arrived != splits - 1) return;
-    __threadfence();
-    if (tid == 0) *ticket = 0;           // for the next launch
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-          for (int s = 0; s < splits; ++s)
-            sum += *reinterpret_cast<const f32x4*>(mine + (int64_t)s * kElems + (((i * NI + j) * 4 + e / 4) * W * 64 + tid) * 4);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[i][j][e + x] = sum[x];
-        }
+    return;
   }
-  wait_and_barrier();                    // image 0 becomes the waves' turning tiles
-
-  // Element e of acc[i][j]: row 8 (e / 4) + 4 (lane / 32) + e % 4 and column lane % 32 of the 32 x 32 tile.
+  // Nobody reads the images any more: image 0 becomes the waves' turning tiles, and a row of a
+  // wave's tiles at a time goes through image 1, so that the code of store_tile() is there MI times and not MI * NI times (with
+  // all of it unrolled the accumulators of the largest tile ended up in scratch memory).
   uint32_t* turn = reinterpret_cast<uint32_t*>(image0) + wave * 32 * 33;
-  const int half = lane >> 5, jc = lane & 31;
-  const float step_size = stage == kLast && it.buf ? c.lr[0] * it.shape_factor : 0.f;
+  f32x4* line = reinterpret_cast<f32x4*>(image1 + wave * (2 * kImage / kWaves)) + lane;
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < MI; ++i) {
 #pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) line[(j * 4 + e / 4) * 64] = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma clang loop unroll(disable)
     for (int j = 0; j < NI; ++j) {
       const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q + 32 * j;
-      float v[16];
-      if (stage == kGram) {
+      if (i0 >= it.mp || j0 >= (stage <= kPoly ? it.mp : it.np)) break;
+      f32x16 sum;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * (kScaleA / (kScaleX * kScaleX));
-      } else {
-        // the matrix in the linear term, through its transpose: 4 consecutive rows of one column are 8 + 8 bytes
-        const char* s = (stage == kPoly ? it.A : it.XT[parity]) + plane_at(j0 + jc, i0, it.mp) + 8 * half;
-        const float lin = stage == kPoly ? kB * (kScaleB / kScaleA) : stage == kStep ? kA : kA / kScaleX;
-        const float quad = stage == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
-                           : stage == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = line[(j * 4 + g) * 64];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const half4 hi = *reinterpret_cast<const half4*>(s + 16 * g), lo = *reinterpret_cast<const half4*>(s + 64 + 16 * g);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[4 * g + x] = lin * ((float)hi[x] + (float)lo[x]) + quad * acc[i][j][4 * g + x];
-        }
+        for (int x = 0; x < 4; ++x) sum[4 * g + x] = v[x];
       }
-      if (stage == kLast) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = i0 + 8 * (e / 4) + 4 * half + e % 4, col = j0 + jc;
-          if (row < it.m && col < it.n) {
-            const int64_t at = it.flip ? (int64_t)col * it.ldo + row : (int64_t)row * it.ldo + col;
-            if (it.buf) {
-              float* w = static_cast<float*>(it.out) + at;
-              *w -= step_size * v[e];
-            } else {
-              static_cast<T*>(it.out)[at] = (T)v[e];
-            }
-          }
-        }
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) turn[(8 * (e / 4) + 4 * half + e % 4) * 33 + jc] = split_pair(v[e]);
-      // (a wave's own tile: no barrier, only the order of its own LDS accesses)
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const int line = lane >> 1, part_of = lane & 1;
-      char* straight = stage == kGram ? it.A : stage == kPoly ? it.B : it.X;
-      char* turned = stage == kGram ? it.A : stage == kPoly ? it.B : it.XT[parity ^ 1];
-      const int straight_cols = stage <= kPoly ? it.mp : it.np;
-      store_group(straight + plane_at(i0 + line, j0, straight_cols), turn + line * 33, 1, part_of);
-      if (!symmetric || ti != tj) store_group(turned + plane_at(j0 + line, i0, it.mp), turn + line, 33, part_of);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, turn, lane);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// Split products: the sums of a 32 x 32 tile's parts in order, one wave each.  `edge`: of the product's tiles.
+__global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge, int stage, int parity) {
+  __shared__ uint32_t turns[4][32 * 33];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.x * 4 + wave;
+  if (id >= tl.first[kMax]) return;
+  int which = 0;
+  while (id >= tl.first[which + 1]) ++which;
+  const Item& it = c.item[which];
+  const int side = edge / 64, per_wave = side * side, per_tile = 4 * per_wave;      // (of a product wave: side x side tiles)
+  const int local = id - tl.first[which], tile = local / per_tile, sub = local - tile * per_tile;
+  const int of_wave = sub / per_wave, ij = sub - of_wave * per_wave;
+  int ti, tj;
+  tile_place(it, stage, edge, tile, ti, tj);
+  const int i0 = ti * edge + (of_wave >> 1) * (edge / 2) + 32 * (ij / side), j0 = tj * edge + (of_wave & 1) * (edge / 2) + 32 * (ij % side);
+  if (i0 >= it.mp || j0 >= (stage <= kPoly ? it.mp : it.np)) return;
+  const int64_t elems = (int64_t)edge * edge;
+  const float* from = c.partial + (tl.tile0[which] + tile) * tl.splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
+  f32x16 sum;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < tl.splits; ++s) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(from + s * elems + g * 256);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum[4 * g + x] += v[x];
+    }
+  }
+  store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, turns[wave], lane);
 }
 
 // --- host ---------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-struct Shape {
-  int m, n, mp, np, flip;
-};
-Shape shape_of(int rows, int cols, int tile) {
-  Shape s;
-  s.flip = rows > cols;
-  s.m = s.flip ? cols : rows;
-  s.n = s.flip ? rows : cols;
-  s.mp = (int)up(s.m, tile);
-  s.np = (int)up(s.n, tile);
-  return s;
-}
-
-// 64 x 64 tiles while the largest product of the call has fewer than 128 tiles of 128 x 128.
-int tile_of(int count, const int32_t* rows, const int32_t* cols) {
-  int64_t tiles = 0;
-  for (int i = 0; i < count; ++i) tiles += up(rows[i], 128) / 128 * (up(cols[i], 128) / 128);
-  return tiles < 128 ? 64 : 128;
-}
 
 constexpr int kMaxDim = 1 << 16;
 
@@ -396,102 +473,147 @@ bool bad_shapes(int count, const int32_t* rows, const int32_t* cols) {
   return false;
 }
 
-// Workgroups that split the k range of a tile: enough for two per CU, each with at least 8 steps of 32.
-int splits_for(int64_t tiles, int depth) {
-  int64_t s = 512 / (tiles > 0 ? tiles : 1);
-  const int64_t most = depth / 64 / 4;
-  if (s > most) s = most;
-  if (s > 16) s = 16;
-  return s < 1 ? 1 : (int)s;
+// How a stage's product is cut: tile edge and workgroups per tile (a range of k each).
+struct Cut {
+  int edge, splits;
+};
+struct StagePlan {
+  Cut cut;
+  Tiles product, finish;
+  int blocks, finish_waves;
+  int64_t partial_floats;
+};
+
+int64_t tiles_of(const Call& c, int i, int stage, int edge) {
+  const int64_t tm = (c.item[i].mp + edge - 1) / edge, tn = (c.item[i].np + edge - 1) / edge;
+  return stage <= kPoly ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-struct StageTiles {
-  Tiles t;
-  int64_t partial_tiles;
-  int blocks;
-};
-StageTiles stage_tiles(const Call& c, int stage, int tile) {
-  StageTiles r{};
-  int64_t total = 0;
-  int tiles[kMax];
+int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut)
+
+// The cheapest cut by an estimate of its time in cycles.  A k-step of a tile costs its MFMAs at the rate they were measured to
+// reach, shared by the workgroups on its CU (four of 64, two of 128, one of 192 and 256), but at least the latency of a
+// load-barrier-read round; whole rounds of workgroups are paid for.  Splitting adds a launch and two passes over the sums.
+Cut choose(const Call& c, int stage) {
+  static const struct { int edge, resident; double mfma; } kinds[] = {{256, 1, 3650}, {192, 1, 2150}, {128, 2, 1080}, {64, 4, 330}};
+  Cut best{128, 1};
+  double least = 1e300;
+  int depth = 0;
   for (int i = 0; i < c.count; ++i) {
-    const int tm = c.item[i].mp / tile, tn = c.item[i].np / tile;
-    tiles[i] = stage <= kPoly ? tm * (tm + 1) / 2 : tm * tn;
-    total += tiles[i];
+    const int d = stage == kGram ? c.item[i].np : c.item[i].mp;
+    depth = d > depth ? d : depth;
   }
-  int64_t at = 0, tickets = 0;
+  for (const auto& kind : kinds) {
+    if (g_force_edge && kind.edge != g_force_edge) continue;
+    int64_t tiles = 0;
+    for (int i = 0; i < c.count; ++i) tiles += tiles_of(c, i, stage, kind.edge);
+    for (int s = 1; s <= 16; ++s) {
+      if (g_force_splits && s != g_force_splits && s != 1) continue;
+      if (s > 1 && depth / 64 < 2 * s) break;
+      const double groups = (double)tiles * s, steps = 2.0 * ((depth / 64 + s - 1) / s);
+      double cycles = 0, left = groups;
+      const double per_round = 256.0 * kind.resident;
+      const int64_t full = (int64_t)(left / per_round);
+      const double latency = 750;
+      auto step = [&](double n) { return n * kind.mfma > latency ? n * kind.mfma : latency; };
+      cycles += full * steps * step(kind.resident);
+      left -= full * per_round;
+      if (left > 0) cycles += steps * step((double)((int64_t)((left + 255) / 256)));
+      cycles += 6000;                                        // launch, first loads, end
+      if (s > 1) cycles += 7000 + groups * kind.edge * kind.edge * 8.0 / 1800;     // (4.3 TB/s)
+      if (g_force_splits && s == g_force_splits) cycles = 0;
+      if (cycles < least) {
+        least = cycles;
+        best = Cut{kind.edge, s};
+      }
+    }
+  }
+  return best;
+}
+
+StagePlan plan_stage(const Call& c, int stage) {
+  StagePlan r{};
+  r.cut = choose(c, stage);
+  const int edge = r.cut.edge, subs = (edge / 32) * (edge / 32);
+  int64_t at = 0;
   for (int i = 0; i < c.count; ++i) {
-    const int depth = stage == kGram ? c.item[i].np : c.item[i].mp;
-    int s = splits_for(total, depth);
-    if (tickets + (int64_t)tiles[i] * s > kMaxTickets) s = 1;
-    r.t.first[i] = (int)at;
-    r.t.splits[i] = s;
-    r.t.ticket0[i] = (int)tickets;
-    at += (int64_t)tiles[i] * s;
-    if (s > 1) tickets += (int64_t)tiles[i] * s;
+    const int64_t tiles = tiles_of(c, i, stage, edge);
+    r.product.first[i] = (int)(at * r.cut.splits);
+    r.finish.first[i] = (int)(at * subs);
+    r.product.tile0[i] = r.finish.tile0[i] = at;
+    at += tiles;
   }
-  for (int i = c.count; i <= kMax; ++i) r.t.first[i] = (int)at;
-  r.blocks = (int)at;
-  r.partial_tiles = tickets;
+  for (int i = c.count; i <= kMax; ++i) {
+    r.product.first[i] = (int)(at * r.cut.splits);
+    r.finish.first[i] = (int)(at * subs);
+  }
+  r.product.splits = r.finish.splits = r.cut.splits;
+  r.blocks = (int)(at * r.cut.splits);
+  r.finish_waves = (int)(at * subs);
+  r.partial_floats = r.cut.splits > 1 ? at * r.cut.splits * edge * edge : 0;
   return r;
 }
 
 struct Layout {
   int64_t total;
-  int tile;
+  StagePlan stage[3];
 };
-// Fills the workspace part of `c.item` (offsets from `base`, which may be null when only the size is asked for).
+// Fills the workspace part of `c` (from `base`, which may be null when only the size is asked for) and cuts the products.
 Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, char* base) {
   Layout l;
-  l.tile = tile_of(count, rows, cols);
   c.count = count;
-  int64_t at = 0;
+  int64_t at = 0, most = 0;
   auto take = [&](int64_t bytes) {
     char* p = base + at;
     at += up(bytes, 1024);
     return p;
   };
-  c.tickets = reinterpret_cast<uint32_t*>(take(kMaxTickets * 4));
   for (int i = 0; i < count; ++i) {
     Item& it = c.item[i];
-    const Shape s = shape_of(rows[i], cols[i], l.tile);
     it.rows = rows[i], it.cols = cols[i];
-    it.m = s.m, it.n = s.n, it.mp = s.mp, it.np = s.np, it.flip = s.flip;
+    it.flip = rows[i] > cols[i];
+    it.m = it.flip ? cols[i] : rows[i];
+    it.n = it.flip ? rows[i] : cols[i];
+    it.mp = (int)up(it.m, 64), it.np = (int)up(it.n, 64);
     it.norm = reinterpret_cast<double*>(take(kNormBlocks * 8));
-    it.X = take((int64_t)s.mp * s.np * 4);
-    it.XT[0] = take((int64_t)s.mp * s.np * 4);
-    it.XT[1] = take((int64_t)s.mp * s.np * 4);
-    it.A = take((int64_t)s.mp * s.mp * 4);
-    it.B = take((int64_t)s.mp * s.mp * 4);
+    const int64_t wide = (int64_t)it.mp * it.np * 4, square = (int64_t)it.mp * it.mp * 4;
+    it.X = take(wide), it.XT[0] = take(wide), it.XT[1] = take(wide);
+    it.A = take(square), it.B = take(square);
+    const int64_t elements = (int64_t)rows[i] * cols[i];
+    most = elements > most ? elements : most;
   }
+  const int64_t blocks = (most + 2047) / 2048;           // eight elements a thread
+  c.norm_blocks = (int)(blocks > kNormBlocks ? kNormBlocks : blocks);
   int64_t partial = 0;
   for (int stage = kGram; stage <= kStep; ++stage) {
-    const int64_t p = stage_tiles(c, stage, l.tile).partial_tiles;
-    partial = p > partial ? p : partial;
+    l.stage[stage] = plan_stage(c, stage);
+    partial = l.stage[stage].partial_floats > partial ? l.stage[stage].partial_floats : partial;
   }
-  c.partial = reinterpret_cast<float*>(take(partial * l.tile * l.tile * 4));
+  c.partial = reinterpret_cast<float*>(take(partial * 4));
   l.total = at;
   return l;
 }
 
 template <typename T>
-int run(Call& c, int tile, hipStream_t s) {
-  norm_kernel<T><<<dim3(kNormBlocks, c.count), 256, 0, s>>>(c);
+int run(Call& c, const Layout& l, hipStream_t s) {
+  norm_kernel<T><<<dim3(c.norm_blocks, c.count), 256, 0, s>>>(c);
   int64_t most = 0;
   for (int i = 0; i < c.count; ++i) {
     const int64_t t = (int64_t)(c.item[i].mp / 64) * (c.item[i].np / 64);
     most = t > most ? t : most;
   }
   split_kernel<T><<<dim3((unsigned)most, c.count), 256, 0, s>>>(c);
-  StageTiles st[3];
-  for (int stage = kGram; stage <= kStep; ++stage) st[stage] = stage_tiles(c, stage, tile);
   for (int k = 0; k < 5; ++k)
     for (int stage = kGram; stage <= kStep; ++stage) {
       const int what = stage == kStep && k == 4 ? kLast : stage;
-      if (tile == 64)
-        product_kernel<64, 2, 2, T><<<st[stage].blocks, 256, 0, s>>>(c, st[stage].t, what, k & 1);
-      else
-        product_kernel<128, 2, 2, T><<<st[stage].blocks, 256, 0, s>>>(c, st[stage].t, what, k & 1);
+      const StagePlan& p = l.stage[stage];
+      switch (p.cut.edge) {
+        case 64: product_kernel<64><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
+        case 128: product_kernel<128><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
+        case 192: product_kernel<192><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
+        default: product_kernel<256><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1);
+      }
+      if (p.cut.splits > 1) finish_kernel<<<(p.finish_waves + 3) / 4, 256, 0, s>>>(c, p.finish, p.cut.edge, what, k & 1);
     }
   return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
 }
@@ -515,9 +637,9 @@ extern "C" int dtf_orthogonalize(const void* x, int dtype, int rows, int cols, i
   c.item[0].u = x, c.item[0].ldu = ldx, c.item[0].out = out, c.item[0].ldo = ldo;
   c.dtype = dtype, c.eps = eps;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DTF_F32) return run<float>(c, l.tile, s);
-  if (dtype == DTF_BF16) return run<bf16_t>(c, l.tile, s);
-  return run<f16_t>(c, l.tile, s);
+  if (dtype == DTF_F32) return run<float>(c, l, s);
+  if (dtype == DTF_BF16) return run<bf16_t>(c, l, s);
+  return run<f16_t>(c, l, s);
 }
 
 extern "C" int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols, const uint64_t* w, const uint64_t* g,
@@ -537,5 +659,12 @@ extern "C" int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols
     it.shape_factor = cols[i] > rows[i] ? sqrtf((float)cols[i] / (float)rows[i]) : 1.f;
   }
   c.mu = momentum, c.nesterov = nesterov, c.eps = eps, c.lr = lr;
-  return run<float>(c, l.tile, (hipStream_t)stream);
+  return run<float>(c, l, (hipStream_t)stream);
+}
+
+// Tuning and tests: products of the next calls in tiles of this edge (64, 128, 192, 256) with this many parts of k where k is long
+// enough; 0: chosen from the shapes.  (The workspace of a plan has to be made under the same setting.)
+extern "C" void dtf_debug_set_muon_cut(int edge, int splits) {
+  g_force_edge = edge == 64 || edge == 128 || edge == 192 || edge == 256 ? edge : 0;
+  g_force_splits = splits > 0 && splits <= 16 ? splits : 0;
 }

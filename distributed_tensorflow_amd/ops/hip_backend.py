@@ -170,6 +170,8 @@ def _declare(lib: C.CDLL) -> None:
     lib.dtf_sparse_xent_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, vp, i64, vp, i64, vp]
     lib.dtf_muon_workspace.argtypes = [i32, vp, vp]
     lib.dtf_muon_workspace.restype = i64
+    lib.dtf_debug_set_muon_cut.argtypes = [i32, i32]
+    lib.dtf_debug_set_muon_cut.restype = None
     lib.dtf_muon_step.argtypes = [i32, vp, vp, vp, vp, vp, vp, f32, i32, f32, vp, i64, vp]
     lib.dtf_orthogonalize.argtypes = [vp, i32, i32, i32, i64, vp, i64, f32, vp, i64, vp]
     for name in ("dtf_muon_step", "dtf_orthogonalize", "dtf_embed_lookup", "dtf_embed_grad", "dtf_embed_sgd", "dtf_sparse_xent", "dtf_sparse_xent_grad"):

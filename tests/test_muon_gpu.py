@@ -62,6 +62,30 @@ def test_factor_against_64_bits(shape, dtype):
         assert torch.equal(got, muon.orthogonalize(x))
 
 
+@pytest.mark.parametrize("edge", [64, 128, 192, 256])
+@pytest.mark.parametrize("splits", [1, 2, 5])
+def test_every_cut_of_the_products(edge, splits):
+    """Tile edges and parts of k that the shapes alone would not choose: tiles that stick out on either side, parts without a
+    step (a short matrix next to a long one), symmetric results with one and several tiles."""
+    lib = hb.require()
+    lib.dtf_debug_set_muon_cut(edge, splits)
+    try:
+        for shape in ((70, 130), (130, 900), (700, 520), (64, 64), (260, 2000)):
+            x = gradient(*shape, seed=sum(shape))
+            want = factor(x)
+            assert float((muon.orthogonalize(x).double() - want).norm()) <= float(allowed(x, want)), shape
+        shapes = [(30, 40), (500, 300), (64, 2000)]
+        ws = [torch.zeros(s, device="cuda") for s in shapes]
+        gs = [gradient(*s, seed=i) for i, s in enumerate(shapes)]
+        muon.muon_step(muon.MuonPlan(ws, gs, [torch.zeros(s, device="cuda") for s in shapes]), torch.ones(1, device="cuda"),
+                       momentum=0.0, nesterov=False)
+        for w, g in zip(ws, gs):
+            want = -math.sqrt(max(1.0, w.shape[1] / w.shape[0])) * factor(g)
+            assert float((w.double() - want).norm()) <= math.sqrt(max(1.0, w.shape[1] / w.shape[0])) * float(allowed(g, factor(g)))
+    finally:
+        lib.dtf_debug_set_muon_cut(0, 0)
+
+
 def test_layouts_and_in_place():
     room = torch.randn(300, 500, device="cuda", generator=gen(1))
     x = room[5:205, 3:133]
