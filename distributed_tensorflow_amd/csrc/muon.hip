@@ -24,16 +24,18 @@
 // GEMM form (row times row) serves all.  A row of a plane pair is groups of 32 columns: 32 hi halves then 32 lo halves, 128
 // bytes, one cache line per row and k-step.  Dimensions are padded with zeros to whole tiles: the products need no bounds.
 //
-// GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 and walks k in steps of 32 through two LDS images
-// filled by direct buffer-to-LDS loads.  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so
-// the 16-byte chunks of a row are permuted on the GLOBAL side: slot s of row r holds chunk s ^ (r & 7), and the rows that a
-// fragment read touches spread over the banks.  A step's two halves of 16 k alternate between two sets of fragment
-// registers: while one half is multiplied the next half's LDS reads are under way, across the step's single barrier too, and
-// the loads of step k + 2 go into the image that the barrier has just freed.  Large tiles matter here: per k-step of a tile
-// of edge T the matrix cores are busy for 0.047 T^2 cycles and the LDS for 6 T cycles (reads by four waves of T/2 x T/2, and the
-// loads): 100 % of the matrix time at 128, 50 % at 256.  Tile edge and split of k are chosen per stage by a cost
-// estimate (see choose()).  Few tiles and a long k: several workgroups take a range of k each and store their sums; a second
-// launch adds them in order and does what the product's own end does otherwise.
+// GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 and walks k in steps of 32 through a ring of 8, 4, 3
+// or 2 LDS images filled by direct buffer-to-LDS loads: 130 to 140 KB, one workgroup per CU, the loads of a step requested one
+// to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away, against 0.1 to 1.8 us of products per
+// step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so the 16-byte chunks of a row are
+// permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the sixteen rows that a quarter of a fragment
+// read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
+// A step's two halves of 16 k alternate between two sets of fragment registers: the LDS reads of one half and the loads are
+// spread between the MFMAs of the half before, across the step's single barrier too.  Large tiles matter: per k-step of a
+// tile of edge T the matrix cores are busy for 0.047 T^2 cycles and the LDS for 6 T (reads by four waves of T/2 x T/2, and the
+// loads).  Tile edge and split of k are chosen per stage by a cost estimate (see choose()).  Few tiles and a long k: several
+// workgroups take a range of k each and store their sums; a second launch adds them in order and does what the product's
+// own end does otherwise.
 //
 // All matrices of a call go through each launch together: 2 + 15 launches per step of the optimiser (up to 15 more where k is
 // split), whatever the number of layers (up to 8; more are taken in groups).
@@ -44,13 +46,16 @@ namespace {
 
 typedef f16_t half8 __attribute__((ext_vector_type(8)));
 typedef f16_t half4 __attribute__((ext_vector_type(4)));
+typedef f16_t half2 __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kMax = DTF_MUON_MAX;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleX = 32768.f, kScaleA = 16384.f, kScaleB = 8192.f;    // powers of two: entries stay below 65504
-constexpr int kNormBlocks = 1024;     // at most
+constexpr int kNormBlocks = 1024;     // at most: four partial sums a thread of split_kernel
 constexpr int kWaves = 4;              // of a product workgroup
 
 // One matrix of a call.  `rows` x `cols` as the caller has it; m <= n its shape (or its transpose's) padded to mp x np.
@@ -159,20 +164,35 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
   const int tiles_c = pc / 64, tiles = (pr / 64) * tiles_c;
   if ((int)blockIdx.x >= tiles) return;
   const int r0 = (blockIdx.x / tiles_c) * 64, c0 = (blockIdx.x % tiles_c) * 64;
+  const int col = threadIdx.x & 63;
+  // All requests at once and before the norm is added up, from clamped places: one by one they took 15 us.
+  const T* gp = static_cast<const T*>(it.u) + min(c0 + col, it.cols - 1);
+  const float* bp = it.buf + min(c0 + col, it.cols - 1);
+  float u[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) u[k] = (float)gp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.ldu];
   double total = 0;
-  for (int i = threadIdx.x; i < c.norm_blocks; i += 256) total += it.norm[i];
+#pragma unroll
+  for (int i = 0; i < kNormBlocks; i += 256) {
+    const double part = it.norm[min(i + (int)threadIdx.x, c.norm_blocks - 1)];
+    total += i + (int)threadIdx.x < c.norm_blocks ? part : 0.0;
+  }
+  if (it.buf) {
+    float b[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) b[k] = bp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.cols];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) u[k] = c.nesterov ? u[k] + c.mu * b[k] : b[k];
+  }
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) total += __shfl_xor(total, x);
   if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = total;
   __syncthreads();
   const double inv = (double)kScaleX / (sqrt((of_wave[0] + of_wave[1]) + (of_wave[2] + of_wave[3])) + (double)c.eps);
-#pragma unroll 4
+#pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const int r = (threadIdx.x >> 6) + 4 * k, col = threadIdx.x & 63;
-    float x = 0.f;
-    if (r0 + r < it.rows && c0 + col < it.cols)
-      x = (float)((double)direction<T>(c, it, (int64_t)(r0 + r) * it.ldu + c0 + col, (int64_t)(r0 + r) * it.cols + c0 + col) * inv);
-    tile[r][col] = split_pair(x);
+    const int r = (threadIdx.x >> 6) + 4 * k;
+    tile[r][col] = r0 + r < it.rows && c0 + col < it.cols ? split_pair((float)((double)u[k] * inv)) : 0u;
   }
   __syncthreads();
   char* straight = it.flip ? it.XT[0] : it.X;          // [pr][pc]
@@ -191,11 +211,15 @@ struct Tiles {
   int splits;              // workgroups per tile
 };
 
-// This wave's loads have landed and its LDS reads are done, then the workgroup's.  (0x0070: vmcnt 0, lgkmcnt 0.  A barrier alone
-// does not wait for loads that go to LDS.)
+// At most `LEFT` of this wave's loads are still under way and its LDS reads are done, then the workgroup's.  (A barrier alone does
+// not wait for loads that go to LDS, and __syncthreads() would wait for all of them.  The empty statements keep the compiler's
+// own memory accesses on their side.)
+template <int LEFT>
 __device__ __forceinline__ void wait_and_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  __syncthreads();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4) << 14 | 7 << 4);     // vmcnt LEFT, lgkmcnt 0, expcnt untouched
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // ROWS rows of a plane pair from a tile's first row on; rows past the last one are read as the last one (their products are not
@@ -210,15 +234,17 @@ struct Fetcher {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = (i * kWaves + wave) * 8 + (lane >> 3);
-      at[i] = (unsigned)(min(r, rows - 1 - row0) * row_bytes) + (unsigned)(((lane & 7) ^ (lane >> 3)) << 4);
+      at[i] = (unsigned)(min(r, rows - 1 - row0) * row_bytes) + (unsigned)(((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
   }
   // The 128-byte group `k` of every row to an LDS image.
   __device__ __forceinline__ void go(char* __restrict lds, int wave, int k) const {
+#ifdef __HIP_DEVICE_COMPILE__          // (the host pass of the compiler does not know the descriptor's type)
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)0xffffffffu, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + (i * kWaves + wave) * 1024), 16, at[i], k * 128, 0, 0);
+#endif
   }
 };
 
@@ -231,59 +257,113 @@ struct Half {
     const int r = lane & 31;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int slot = ((h * 4 + ks * 2 + (lane >> 5)) ^ (r & 7)) << 4;      // (every base row is a multiple of 32)
+      const int slot = ((h * 4 + ks * 2 + (lane >> 5)) ^ ((r >> 1) & 7)) << 4;      // (every base row is a multiple of 32)
 #pragma unroll
       for (int i = 0; i < MI; ++i) a[i][h] = *reinterpret_cast<const half8*>(p + (row_p + 32 * i + r) * 128 + slot);
 #pragma unroll
       for (int j = 0; j < NI; ++j) b[j][h] = *reinterpret_cast<const half8*>(q + (row_q + 32 * j + r) * 128 + slot);
     }
   }
-  // hi lo, lo hi, hi hi; the three MFMAs of a tile are MI * NI apart
-  __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
+  // hi lo, lo hi, hi hi; the three MFMAs of a tile are MI * NI apart, or, with SUMS = 3, have a sum each (a chain of MFMAs on
+  // one sum runs at half their rate)
+  template <int SUMS>
+  __device__ __forceinline__ void multiply(f32x16 (&acc)[SUMS][MI][NI]) const {
 #pragma unroll
     for (int t = 0; t < 3; ++t)
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][t == 1], b[j][t == 0], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NI; ++j) {
+          f32x16& sum = acc[SUMS == 3 ? t : 0][i][j];
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][t == 1], b[j][t == 0], sum, 0, 0, 0);
+        }
   }
 };
 
-// What becomes of a 32 x 32 tile of a stage's product at (i0, j0).  Element e of `sum`: row 8 (e / 4) + 4 (lane / 32) + e % 4
-// and column lane % 32.  `turn`: 32 x 33 words of LDS that this wave alone uses.  `mirror`: also store the transposed tile of a
-// symmetric result.
+// Instruction order of a half step: the LDS reads of the next half (and, with LOADS, the loads) spread over the first three
+// quarters of its MFMAs.  A wave issues in order: reads in one block left the matrix pipe idle while they queued for the LDS
+// (52 % busy against 69 % at 4096 x 4096).
+template <int R, int READS, int MFMAS, int LOADS>
+__device__ __forceinline__ void interleave() {
+  constexpr int kOver = MFMAS - MFMAS / 4;
+  if constexpr (R < READS) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                // an LDS read
+    if constexpr ((R + 1) * LOADS / READS > R * LOADS / READS)
+      __builtin_amdgcn_sched_group_barrier(0x010, (R + 1) * LOADS / READS - R * LOADS / READS, 0);    // a load
+    if constexpr ((R + 1) * kOver / READS > R * kOver / READS)
+      __builtin_amdgcn_sched_group_barrier(0x008, (R + 1) * kOver / READS - R * kOver / READS, 0);    // MFMAs
+    interleave<R + 1, READS, MFMAS, LOADS>();
+  } else {
+    __builtin_amdgcn_sched_group_barrier(0x008, MFMAS - kOver, 0);
+  }
+}
+
+// A wave's 32 x 32 tile of a stage's product, rows from i0 and columns from j0 on.  Element e of a lane: row 8 (e / 4) +
+// 4 (lane / 32) + e % 4 and column lane % 32.  In memory it is 32 lines of 128 bytes, and every access below moves whole lines (lane
+// l has the 16-byte chunk l % 8 of line l / 8 + 8 n): accesses of 8 or 16 bytes to 32 lines at a time cost 5000 cycles a tile.
+// The way between the two layouts is through LDS.
+constexpr int kTurnRow = 36;                      // words of a line: its 16-byte chunks spread over the banks
+constexpr int kTurnWords = 2 * 32 * kTurnRow;     // two turning areas of a wave
+// Order of a wave's own LDS accesses (nobody else touches its areas).
+__device__ __forceinline__ void own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The linear term's lines (of A, or of X through its transpose).
+struct Linear {
+  u32x4 chunk[4];
+  __device__ __forceinline__ void read(const Item& it, int stage, int parity, int i0, int j0, int lane) {
+    const char* s = (stage == kPoly ? it.A : it.XT[parity]) + plane_at(j0 + (lane >> 3), i0, it.mp) + 16 * (lane & 7);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * it.mp * 4);
+  }
+};
+
+// What becomes of the tile.  `area`: the wave's turning areas.  `mirror`: also store the transposed tile of a symmetric result.
 __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int stage, int parity, int i0, int j0, bool mirror,
-                                           const f32x16& sum, uint32_t* turn, int lane) {
+                                           const f32x16& sum, const Linear& linear, uint32_t* area, int lane) {
   const int half = lane >> 5, jc = lane & 31;
+  uint32_t* turn = area;
+  uint32_t* lines = area + 32 * kTurnRow;
   float v[16];
   if (stage == kGram) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = sum[e] * (kScaleA / (kScaleX * kScaleX));
   } else {
-    // the matrix in the linear term, through its transpose: 4 consecutive rows of one column are 8 + 8 bytes
-    const char* s = (stage == kPoly ? it.A : it.XT[parity]) + plane_at(j0 + jc, i0, it.mp) + 8 * half;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      *reinterpret_cast<u32x4*>(lines + ((lane >> 3) + 8 * n) * kTurnRow + 4 * (lane & 7)) = linear.chunk[n];
+    own_lds();
     const float lin = stage == kPoly ? kB * (kScaleB / kScaleA) : stage == kStep ? kA : kA / kScaleX;
     const float quad = stage == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
                        : stage == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
+    const char* line = reinterpret_cast<const char*>(lines + jc * kTurnRow) + 8 * half;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const half4 hi = *reinterpret_cast<const half4*>(s + 16 * g), lo = *reinterpret_cast<const half4*>(s + 64 + 16 * g);
+      const half4 hi = *reinterpret_cast<const half4*>(line + 16 * g), lo = *reinterpret_cast<const half4*>(line + 64 + 16 * g);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[4 * g + x] = lin * ((float)hi[x] + (float)lo[x]) + quad * sum[4 * g + x];
+      for (int x = 0; x < 4; ++x)      // (two mixed-precision multiply-adds: the planes are not converted)
+        v[4 * g + x] = fmaf((float)hi[x], lin, fmaf((float)lo[x], lin, quad * sum[4 * g + x]));
     }
   }
   if (stage == kLast) {
-    const float step_size = it.buf ? c.lr[0] * it.shape_factor : 0.f;
+    const int64_t step_row = it.flip ? 1 : it.ldo, step_col = it.flip ? it.ldo : 1;
+    const int64_t at0 = (i0 + 4 * half) * step_row + (j0 + jc) * step_col;
+    auto inside = [&](int e) { return i0 + 8 * (e / 4) + 4 * half + e % 4 < it.m && j0 + jc < it.n; };
+    if (it.buf) {
+      const float step_size = c.lr[0] * it.shape_factor;
+      float* w = static_cast<float*>(it.out) + at0;
+      float old[16];                      // (all of them requested before the first store)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) old[e] = inside(e) ? w[(8 * (e / 4) + e % 4) * step_row] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (inside(e)) w[(8 * (e / 4) + e % 4) * step_row] = old[e] - step_size * v[e];
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int row = i0 + 8 * (e / 4) + 4 * half + e % 4, col = j0 + jc;
-      if (row < it.m && col < it.n) {
-        const int64_t at = it.flip ? (int64_t)col * it.ldo + row : (int64_t)row * it.ldo + col;
-        if (it.buf) {
-          float* w = static_cast<float*>(it.out) + at;
-          *w -= step_size * v[e];
-        } else if (c.dtype == DTF_F32) {
+      if (inside(e)) {
+        const int64_t at = at0 + (8 * (e / 4) + e % 4) * step_row;
+        if (c.dtype == DTF_F32) {
           static_cast<float*>(it.out)[at] = v[e];
         } else if (c.dtype == DTF_BF16) {
           static_cast<bf16_t*>(it.out)[at] = (bf16_t)v[e];
@@ -294,16 +374,49 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int st
     }
     return;
   }
+  // hi and lo of two rows at a time
+  half2 hi[8], lo[8];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) turn[(8 * (e / 4) + 4 * half + e % 4) * 33 + jc] = split_pair(v[e]);
-  // (a wave's own tile: no barrier, only the order of its own LDS accesses)
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  const int line = lane >> 1, part = lane & 1;
-  char* straight = stage == kGram ? it.A : stage == kPoly ? it.B : it.X;
-  char* turned = stage == kGram ? it.A : stage == kPoly ? it.B : it.XT[parity ^ 1];
-  store_group(straight + plane_at(i0 + line, j0, stage <= kPoly ? it.mp : it.np), turn + line * 33, 1, part);
-  if (mirror) store_group(turned + plane_at(j0 + line, i0, it.mp), turn + line, 33, part);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int p = 0; p < 8; ++p) {
+    const float2v x = {v[2 * p], v[2 * p + 1]};
+    hi[p] = __builtin_convertvector(x, half2);
+    lo[p] = __builtin_convertvector(x - __builtin_convertvector(hi[p], float2v), half2);
+  }
+  f16_t* at = reinterpret_cast<f16_t*>(turn + 4 * half * kTurnRow) + jc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    at[(8 * (e / 4) + e % 4) * 2 * kTurnRow] = hi[e / 2][e % 2];
+    at[(8 * (e / 4) + e % 4) * 2 * kTurnRow + 32] = lo[e / 2][e % 2];
+  }
+  if (mirror) {
+    // Line j of the transposed tile: this lane has rows 4 half .. 4 half + 3 of every eight, the lane 32 away the other four.
+    // Exchanged between two groups of eight, each lane holds whole chunks.
+    own_lds();                            // (the linear term has been read)
+    uint32_t* line = lines + jc * kTurnRow + 4 * half;
+#pragma unroll
+    for (int g = 0; g < 4; g += 2)
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const half2* of = part ? lo : hi;
+        const auto s0 = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, of[2 * g]), __builtin_bit_cast(uint32_t, of[2 * g + 2]), false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, of[2 * g + 1]), __builtin_bit_cast(uint32_t, of[2 * g + 3]), false, false);
+        *reinterpret_cast<u32x4*>(line + 4 * g + 16 * part) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+      }
+  }
+  own_lds();
+  const int l8 = lane >> 3, chunk = lane & 7;
+  if (mirror) {
+    char* to = (stage == kGram ? it.A : stage == kPoly ? it.B : it.XT[parity ^ 1]) + plane_at(j0 + l8, i0, it.mp) + 16 * chunk;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * it.mp * 4) = *reinterpret_cast<const u32x4*>(lines + (l8 + 8 * n) * kTurnRow + 4 * chunk);
+  }
+  const int cols = stage <= kPoly ? it.mp : it.np;
+  char* to = (stage == kGram ? it.A : stage == kPoly ? it.B : it.X) + plane_at(i0 + l8, j0, cols) + 16 * chunk;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+    *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * cols * 4) = *reinterpret_cast<const u32x4*>(turn + (l8 + 8 * n) * kTurnRow + 4 * chunk);
+  own_lds();
 }
 
 // Tile `t` of a stage: rows and columns in tiles.  Symmetric results: t = tj (tj + 1) / 2 + ti, ti <= tj.
@@ -314,77 +427,151 @@ __device__ __forceinline__ void tile_place(const Item& it, int stage, int edge, 
     while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
     ti = t - tj * (tj + 1) / 2;
   } else {
-    const int tiles_m = (it.mp + edge - 1) / edge;
-    tj = t / tiles_m;
-    ti = t - tj * tiles_m;
+    // groups of eight tile rows, column by column inside: neighbours share rows of both operands
+    const int tiles_m = (it.mp + edge - 1) / edge, tiles_n = (it.np + edge - 1) / edge;
+    const int group = t / (8 * tiles_n), high = min(8, tiles_m - 8 * group), in = t - group * 8 * tiles_n;
+    tj = in / high;
+    ti = 8 * group + in - tj * high;
   }
 }
 
-template <int TILE>
-__global__ __launch_bounds__(kWaves * 64, TILE <= 64 ? 4 : TILE <= 128 ? 2 : 1) void product_kernel(Call c, Tiles tl, int stage, int parity) {
-  constexpr int MI = TILE / 64, NI = TILE / 64;
-  constexpr int kImage = TILE * 128;
-  constexpr int kTurn = kWaves * 32 * 33 * 4;                        // a 32 x 33 word tile per wave
-  __shared__ __attribute__((aligned(1024))) char image0[2 * kImage > kTurn ? 2 * kImage : kTurn];
-  __shared__ __attribute__((aligned(1024))) char image1[2 * kImage];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The matrix that workgroup (wave) `id` works for.  (Compared with all bounds at once: one by one each would be a trip to memory.)
+__device__ __forceinline__ int owner(const Tiles& tl, int id) {
   int which = 0;
-  while ((int)blockIdx.x >= tl.first[which + 1]) ++which;
+#pragma unroll
+  for (int i = 1; i < kMax; ++i) which += id >= tl.first[i] ? 1 : 0;
+  return which;
+}
+
+constexpr int ring_of(int tile) { return tile == 256 ? 2 : tile == 192 ? 3 : tile == 128 ? 4 : 8; }
+constexpr int kTurn = kWaves * kTurnWords * 4;      // all waves' turning areas, in bytes
+
+// LDS image I of the ring: the rows of one operand, then the other's.  (One variable each: the compiler must see that a load to
+// one image does not concern the reads of another.)
+template <int TILE, int I>
+__device__ __forceinline__ char* image() {
+  __shared__ __attribute__((aligned(1024))) char bytes[I == 0 && 2 * TILE * 128 < kTurn ? kTurn : 2 * TILE * 128];
+  return bytes;
+}
+
+template <int TILE>
+struct Product {
+  static constexpr int kRing = ring_of(TILE), MI = TILE / 64, NI = TILE / 64;
+  static constexpr int kLoads = 2 * Fetcher<TILE>::kLoads;       // of a wave and step
+  static constexpr int kReads = 2 * (MI + NI), kMfmas = 3 * MI * NI, kSums = MI * NI == 1 ? 3 : 1;
+  typedef f32x16 Sums[kSums][MI][NI];
+  Fetcher<TILE> p, q;
+  Half<MI, NI> first, second;
+  int wave, lane, row_p, row_q;
+
+  template <int I>
+  __device__ __forceinline__ void load(int k) const {
+    p.go(image<TILE, I>(), wave, k);
+    q.go(image<TILE, I>() + TILE * 128, wave, k);
+  }
+  template <int I>
+  __device__ __forceinline__ void preload(int k, int last) const {
+    if constexpr (I < kRing - 1) {
+      load<I>(min(k + I, last));
+      preload<I + 1>(k, last);
+    }
+  }
+  // Step k, in image I; `last`: the last step of the range (loaded again by the steps at the end, which nobody reads).
+  template <int I>
+  __device__ __forceinline__ void step(Sums& acc, int k, int last) {
+    wait_and_barrier<(kRing - 2) * kLoads>();          // step k has landed, every wave is done with step k - 1
+    load<(I + kRing - 1) % kRing>(min(k + kRing - 1, last));
+    first.read(image<TILE, I>(), image<TILE, I>() + TILE * 128, row_p, row_q, lane, 0);
+    second.template multiply<kSums>(acc);                              // the second half of step k - 1
+    interleave<0, kReads, kMfmas, kLoads>();
+    __builtin_amdgcn_sched_barrier(0);
+    second.read(image<TILE, I>(), image<TILE, I>() + TILE * 128, row_p, row_q, lane, 1);
+    first.template multiply<kSums>(acc);
+    interleave<0, kReads, kMfmas, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Steps k, k + 1, ... of two rounds of the ring; whether the range goes on behind them.
+  static constexpr int kSteps = 2 * kRing;
+  template <int I>
+  __device__ __forceinline__ bool turn(Sums& acc, int k, int last) {
+    step<I % kRing>(acc, k + I, last);
+    if (k + I == last) return false;
+    if constexpr (I + 1 < kSteps) return turn<I + 1>(acc, k, last);
+    return true;
+  }
+  __device__ __forceinline__ void run(Sums& acc, int first_step, int last) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                      // (the first step multiplies these)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) second.a[i][h] = half8{};
+#pragma unroll
+      for (int j = 0; j < NI; ++j) second.b[j][h] = half8{};
+    }
+    preload<0>(first_step, last);
+    int k = first_step;
+    if constexpr (kRing == 2) {                        // (ranges are whole pairs of steps: one way out, which the accumulators
+#pragma clang loop unroll(disable)
+      for (; k < last; k += 2) {                       //  of the largest tile need to stay where they are)
+        step<0>(acc, k, last);
+        step<1>(acc, k + 1, last);
+      }
+    } else {
+      // (the first turn stands by itself: at the head of a loop the compiler waits for every load once)
+      if (turn<0>(acc, k, last)) {
+        k += kSteps;
+#pragma clang loop unroll(disable)
+        while (turn<0>(acc, k, last)) k += kSteps;
+      }
+    }
+    second.template multiply<kSums>(acc);
+    wait_and_barrier<0>();                             // nothing is on its way to the images any more, and nobody reads them
+  }
+};
+
+template <int TILE>
+__global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles tl, int stage, int parity) {
+  constexpr int MI = Product<TILE>::MI, NI = Product<TILE>::NI;
+  Product<TILE> g;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go round the eight XCDs; numbered so that those of one XCD follow each other, and with the tiles of one range of k
+  // next to each other, the workgroups that share an L2 read the same rows.
+  const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
+  const int id = xcd * per + min(xcd, extra) + (int)(blockIdx.x >> 3);
+  const int which = owner(tl, id);
   const Item& it = c.item[which];
-  const int local = blockIdx.x - tl.first[which], tile = local / tl.splits, part = local - tile * tl.splits;
+  const int tiles = (tl.first[which + 1] - tl.first[which]) / tl.splits;
+  const int local = id - tl.first[which], part = local / tiles, tile = local - part * tiles;
   int ti, tj;
   tile_place(it, stage, TILE, tile, ti, tj);
   const int depth = stage == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
   const int64_t row_bytes = (int64_t)depth * 4;
-  Fetcher<TILE> p, q;
-  p.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
-  q.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.XT[parity], tj * TILE, stage <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
+  g.p.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
+  g.q.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.XT[parity], tj * TILE, stage <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
+  g.wave = wave, g.lane = lane;
+  const int row_p = g.row_p = (wave >> 1) * (TILE / 2), row_q = g.row_q = (wave & 1) * (TILE / 2);
   const int pairs = depth / 64;
   const int k_first = 2 * (int)((int64_t)pairs * part / tl.splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / tl.splits);
-  const int row_p = (wave >> 1) * (TILE / 2), row_q = (wave & 1) * (TILE / 2);
 
-  f32x16 acc[MI][NI];
+  const int columns = stage <= kPoly ? it.mp : it.np;
+  Linear early{};                         // (of the smallest tile: under way during the product)
+  if (MI * NI == 1 && stage != kGram && tl.splits == 1 && ti * TILE + row_p < it.mp && tj * TILE + row_q < columns)
+    early.read(it, stage, parity, ti * TILE + row_p, tj * TILE + row_q, lane);
+  constexpr int kSums = Product<TILE>::kSums;
+  typename Product<TILE>::Sums sums;
+  f32x16 (&acc)[MI][NI] = sums[0];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int t = 0; t < kSums; ++t)
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  Half<MI, NI> first, second;
-  if (k_first < k_last) {                      // (a matrix with fewer steps than parts: this part's sums are zeros)
-    p.go(image0, wave, k_first);
-    q.go(image0 + kImage, wave, k_first);
-    // Two steps a turn.  The scheduling barriers keep the LDS reads and the loads in front of the products that cover them.  (The
-    // turn begins at a full wait because the compiler adds one where the loop is entered: elsewhere it would cut into the loads.)
-#pragma clang loop unroll(disable)
-    for (int k = k_first; k < k_last; k += 2) {
-      wait_and_barrier();                      // image 0 has landed, every wave is done with image 1
-      p.go(image1, wave, k + 1);
-      q.go(image1 + kImage, wave, k + 1);
-      first.read(image0, image0 + kImage, row_p, row_q, lane, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      if (k > k_first) second.multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
-      second.read(image0, image0 + kImage, row_p, row_q, lane, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      first.multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
-      wait_and_barrier();                      // image 1 has landed, every wave is done with image 0
-      if (k + 2 < k_last) {
-        p.go(image0, wave, k + 2);
-        q.go(image0 + kImage, wave, k + 2);
-      }
-      first.read(image1, image1 + kImage, row_p, row_q, lane, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      second.multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
-      second.read(image1, image1 + kImage, row_p, row_q, lane, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      first.multiply(acc);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    second.multiply(acc);
-    wait_and_barrier();                        // every wave is done with the images
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[t][i][j][e] = 0.f;
+  if (k_first < k_last) g.run(sums, k_first, k_last - 1);         // (a matrix with fewer steps than parts: this part's sums are zeros)
+
+  if constexpr (kSums == 3) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][0][e] += sums[1][0][0][e] + sums[2][0][0][e];
   }
 
   if (tl.splits > 1) {
@@ -399,22 +586,26 @@ __global__ __launch_bounds__(kWaves * 64, TILE <= 64 ? 4 : TILE <= 128 ? 2 : 1) 
               f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
     return;
   }
-  // Nobody reads the images any more: image 0 becomes the waves' turning tiles, and a row of a
-  // wave's tiles at a time goes through image 1, so that the code of store_tile() is there MI times and not MI * NI times (with
-  // all of it unrolled the accumulators of the largest tile ended up in scratch memory).
-  uint32_t* turn = reinterpret_cast<uint32_t*>(image0) + wave * 32 * 33;
-  f32x4* line = reinterpret_cast<f32x4*>(image1 + wave * (2 * kImage / kWaves)) + lane;
+  // Nobody reads the images any more: image 0 becomes the waves' turning tiles, and a row of a wave's tiles at a time goes through
+  // image 1, so that the code of store_tile() is there MI times and not MI * NI times (with all of it unrolled the accumulators
+  // of the largest tile ended up in scratch memory).
+  uint32_t* turn = reinterpret_cast<uint32_t*>(image<TILE, 0>()) + wave * kTurnWords;
+  f32x4* line = reinterpret_cast<f32x4*>(image<TILE, 1>() + wave * (2 * TILE * 128 / kWaves)) + lane;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
+    const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q;
+    if (i0 >= it.mp || j0 >= columns) break;
+    Linear next = early;
+    if (MI * NI > 1 && stage != kGram) next.read(it, stage, parity, i0, j0, lane);
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) line[(j * 4 + e / 4) * 64] = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    own_lds();
 #pragma clang loop unroll(disable)
-    for (int j = 0; j < NI; ++j) {
-      const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q + 32 * j;
-      if (i0 >= it.mp || j0 >= (stage <= kPoly ? it.mp : it.np)) break;
+    for (int j = 0; j < NI && j0 + 32 * j < columns; ++j) {
+      const Linear linear = next;
+      if (stage != kGram && j + 1 < NI && j0 + 32 * (j + 1) < columns) next.read(it, stage, parity, i0, j0 + 32 * (j + 1), lane);
       f32x16 sum;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -422,20 +613,19 @@ __global__ __launch_bounds__(kWaves * 64, TILE <= 64 ? 4 : TILE <= 128 ? 2 : 1) 
 #pragma unroll
         for (int x = 0; x < 4; ++x) sum[4 * g + x] = v[x];
       }
-      store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, turn, lane);
+      store_tile(c, it, stage, parity, i0, j0 + 32 * j, stage > kPoly || ti != tj, sum, linear, turn, lane);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    own_lds();
   }
 }
 
 // Split products: the sums of a 32 x 32 tile's parts in order, one wave each.  `edge`: of the product's tiles.
 __global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge, int stage, int parity) {
-  __shared__ uint32_t turns[4][32 * 33];
+  __shared__ __attribute__((aligned(16))) uint32_t turns[4][kTurnWords];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x * 4 + wave;
   if (id >= tl.first[kMax]) return;
-  int which = 0;
-  while (id >= tl.first[which + 1]) ++which;
+  const int which = owner(tl, id);
   const Item& it = c.item[which];
   const int side = edge / 64, per_wave = side * side, per_tile = 4 * per_wave;      // (of a product wave: side x side tiles)
   const int local = id - tl.first[which], tile = local / per_tile, sub = local - tile * per_tile;
@@ -446,19 +636,23 @@ __global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge,
   if (i0 >= it.mp || j0 >= (stage <= kPoly ? it.mp : it.np)) return;
   const int64_t elems = (int64_t)edge * edge;
   const float* from = c.partial + (tl.tile0[which] + tile) * tl.splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
+  Linear linear{};
+  if (stage != kGram) linear.read(it, stage, parity, i0, j0, lane);
   f32x16 sum;
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < tl.splits; ++s) {
+  for (int s0 = 0; s0 < tl.splits; s0 += 4) {
+    f32x4 v[4][4];                         // (four parts requested together; past the end the last one again)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(from + s * elems + g * 256);
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) sum[4 * g + x] += v[x];
-    }
+      for (int g = 0; g < 4; ++g) v[k][g] = *reinterpret_cast<const f32x4*>(from + min(s0 + k, tl.splits - 1) * elems + g * 256);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[e] += s0 + k < tl.splits ? v[k][e / 4][e % 4] : 0.f;
   }
-  store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, turns[wave], lane);
+  store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, linear, turns[wave], lane);
 }
 
 // --- host ---------------------------------------------------------------------------------------------------------------
@@ -491,12 +685,16 @@ int64_t tiles_of(const Call& c, int i, int stage, int edge) {
 
 int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut)
 
-// The cheapest cut by an estimate of its time in cycles.  A k-step of a tile costs its MFMAs at the rate they were measured to
-// reach, shared by the workgroups on its CU (four of 64, two of 128, one of 192 and 256), but at least the latency of a
-// load-barrier-read round; whole rounds of workgroups are paid for.  Splitting adds a launch and two passes over the sums.
+// The cheapest cut by an estimate in microseconds.  By tile edge: a k-step with few and with all CUs at work (a full chip runs
+// into its power limit: 1.3 PFLOP/s of fp16 products at 1.4 to 1.6 GHz, where a lone workgroup does a step at 96 % of the matrix
+// rate at 2.4 GHz) and what a workgroup spends outside its steps, both measured.  One workgroup per CU at a time.  Long launches
+// stay near the power limit even when some CUs have no work.  A split product pays a second launch and its sums' traffic.
+// Against the choice, in us: 4096^2 x 4096 symmetric 192/1 178 (256/1 242, 128/1 233, 128/2 224); 4096^3 256/1 313 (192/1 345,
+// 128/1 359, 64/1 472); 1024 x 4096 x 1024 128/1 33 (256/1 72, 64/1 44); 1024^2 x 1024 symmetric 64/1 12 (128/4 19, 256/1 70).
 Cut choose(const Call& c, int stage) {
-  static const struct { int edge, resident; double mfma; } kinds[] = {{256, 1, 3650}, {192, 1, 2150}, {128, 2, 1080}, {64, 4, 330}};
-  Cut best{128, 1};
+  static const struct { int edge; double step, loaded, rest; } kinds[] = {
+      {256, 1.34, 2.3, 18.0}, {192, 0.755, 1.3, 11.5}, {128, 0.39, 0.65, 6.0}, {64, 0.175, 0.24, 2.0}};
+  Cut best{64, 1};
   double least = 1e300;
   int depth = 0;
   for (int i = 0; i < c.count; ++i) {
@@ -510,20 +708,18 @@ Cut choose(const Call& c, int stage) {
     for (int s = 1; s <= 16; ++s) {
       if (g_force_splits && s != g_force_splits && s != 1) continue;
       if (s > 1 && depth / 64 < 2 * s) break;
-      const double groups = (double)tiles * s, steps = 2.0 * ((depth / 64 + s - 1) / s);
-      double cycles = 0, left = groups;
-      const double per_round = 256.0 * kind.resident;
-      const int64_t full = (int64_t)(left / per_round);
-      const double latency = 750;
-      auto step = [&](double n) { return n * kind.mfma > latency ? n * kind.mfma : latency; };
-      cycles += full * steps * step(kind.resident);
-      left -= full * per_round;
-      if (left > 0) cycles += steps * step((double)((int64_t)((left + 255) / 256)));
-      cycles += 6000;                                        // launch, first loads, end
-      if (s > 1) cycles += 7000 + groups * kind.edge * kind.edge * 8.0 / 1800;     // (4.3 TB/s)
-      if (g_force_splits && s == g_force_splits) cycles = 0;
-      if (cycles < least) {
-        least = cycles;
+      const int64_t groups = tiles * s, full = groups / 256;
+      const double steps = 2.0 * ((depth / 64 + s - 1) / s), share = (groups - full * 256) / 256.0;
+      double us = 3.5 + full * (steps * kind.loaded + kind.rest);
+      if (share > 0) {
+        const bool lasting = us + steps * kind.loaded > 100;
+        const double busy = kind.loaded * (lasting ? 0.45 + 0.55 * share : share);
+        us += steps * (busy > kind.step ? busy : kind.step) + kind.rest;
+      }
+      if (s > 1) us += 3 + (double)groups * kind.edge * kind.edge * 8 / 8e6;
+      if (g_force_splits && s == g_force_splits) us = 0;
+      if (us < least) {
+        least = us;
         best = Cut{kind.edge, s};
       }
     }
