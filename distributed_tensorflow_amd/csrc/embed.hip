@@ -10,32 +10,38 @@
 // must not serialise on its row, so the tokens are SORTED by id (stable, least significant digit first) and equal ids are
 // summed as runs of the sorted order, in ascending t:
 //
-//   sort      digits of up to 9 bits, two launches per digit: counts of every block, then the scatter, each block of which
-//             adds up the counts in front of it by itself (at most 128 blocks, so that is at most 128 coalesced rows).
-//             Ranks inside a wave come from ballots over the digit's bits.  Up to 4096 tokens: one workgroup, all digits
-//             in LDS, one launch.
+//   sort      digits of up to 10 bits (a vocabulary of 2^20 - 1 takes two), two launches per digit: counts of every block, then
+//             the scatter, each block of which adds up the counts in front of it by itself (at most 64 blocks, so that is at
+//             most 64 coalesced rows).  Ranks inside a wave come from ballots over the digit's bits.  Up to 4096 tokens:
+//             one workgroup, all digits in LDS, one launch.
 //   sums      a group of lanes owns a chunk of consecutive sorted positions and a slice of columns, walks the chunk with
 //             the loads of four positions in flight, and stores each run that lies inside the chunk.  The pieces of a run
 //             that crosses chunks go to an fp32 workspace row of their chunk.  Further blocks of the same launch look up
 //             (binary search in the sorted ids) which rows of the table do not occur and store their zeros, so no row of
 //             the gradient is written twice.
-//   joins     one group of waves per run that crosses chunks adds its pieces in order.  The chunk borders depend on the
-//             sizes alone: the result is the same bits every time.
+//   joins     a wave per run that crosses chunks and slice of columns adds its pieces in order; all sixteen waves of a block
+//             share a run of more than 32 pieces (a frequent token).  The chunk borders depend on the sizes alone: the result
+//             is the same bits every time.
 #include "dtf_api.h"
 #include "dtf_types.h"
 
 #include <type_traits>
 
+#ifndef AHEAD
+#define AHEAD 4
+#endif
 namespace {
 
 constexpr int kSmall = 4096;        // tokens sorted by one workgroup
 constexpr int kSortThreads = 1024;
 constexpr int kWaves = kSortThreads / 64;
-constexpr int kMaxDigit = 9;        // bits
-constexpr int kMaxSortBlocks = 128;
+constexpr int kMaxDigit = 10;       // bits
+constexpr int kMaxSortBlocks = 64;
 constexpr int kThreads = 256;
+constexpr int64_t kCaches = (int64_t)256 << 20;     // bytes: a result of more does not stay in the last cache anyway
 constexpr int kFillRows = 32;       // rows of the table per zero-filling block
-constexpr int kJoinChunks = 4;      // chunks whose crossing runs one block joins
+constexpr int kJoinWaves = 16;
+constexpr int kLongRun = 32;        // pieces
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t t) {
   return wide ? static_cast<const int64_t*>(ids)[t] : (int64_t) static_cast<const int32_t*>(ids)[t];
@@ -46,30 +52,46 @@ __device__ __forceinline__ uint32_t load_key(const void* ids, int wide, int64_t 
   return (id >= 0 && id < (int64_t)rows) ? (uint32_t)id : rows;
 }
 
-// --- lookup ------------------------------------------------------------------------------------------------------------
-// 1 << lanes_log2 lanes per row, as many rows per block as fit; the grid strides over the tokens.
+// A pack to memory, past the caches if `past`: results larger than they are.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T, int N>
+__device__ __forceinline__ void put(T* at, const Pack<T, N>& p, bool past) {
+  if constexpr (sizeof(T) * N == 16) {
+    if (past) {
+      __builtin_nontemporal_store(__builtin_bit_cast(u32x4, p), reinterpret_cast<u32x4*>(at));
+      return;
+    }
+  }
+  *reinterpret_cast<Pack<T, N>*>(at) = p;
+}
+
+// --- lookup ------------------------------------------------------------------------------------------------------------
+// 1 << lanes_log2 lanes per row, as many rows per block as fit, U tokens at a time (their rows requested together); the grid
+// strides over the tokens.
+template <typename T, int N, int U>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(const T* __restrict__ table, int64_t ld, int64_t rows,
                                                           const void* __restrict__ ids, int wide, int64_t tokens, int packs,
-                                                          int lanes_log2, float scale, T* __restrict__ out, int64_t ldo) {
+                                                          int lanes_log2, float scale, T* __restrict__ out, int64_t ldo, bool past) {
   const int group = threadIdx.x >> lanes_log2, groups = kThreads >> lanes_log2;
   const int lane = threadIdx.x & ((1 << lanes_log2) - 1);
-  for (int64_t t = (int64_t)blockIdx.x * groups + group; t < tokens; t += (int64_t)gridDim.x * groups) {
-    const int64_t id = load_id(ids, wide, t);
-    const bool inside = id >= 0 && id < rows;
-    const T* src = table + (inside ? id : 0) * ld;
-    T* dst = out + t * ldo;
+  for (int64_t t0 = ((int64_t)blockIdx.x * groups + group) * U; t0 < tokens; t0 += (int64_t)gridDim.x * groups * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = load_id(ids, wide, min(t0 + u, tokens - 1));
     for (int c = lane; c < packs; c += 1 << lanes_log2) {
-      Pack<T, N> p;
-      if (inside) {
-        p = *reinterpret_cast<const Pack<T, N>*>(src + (int64_t)c * N);
+      Pack<T, N> p[U];
 #pragma unroll
-        for (int e = 0; e < N; ++e) p.v[e] = (T)(scale * (float)p.v[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) p.v[e] = (T)0.0f;
+      for (int u = 0; u < U; ++u) {       // (padding reads row 0 and forgets it)
+        const bool inside = id[u] >= 0 && id[u] < rows;
+        p[u] = *reinterpret_cast<const Pack<T, N>*>(table + (inside ? id[u] : 0) * ld + (int64_t)c * N);
       }
-      *reinterpret_cast<Pack<T, N>*>(dst + (int64_t)c * N) = p;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool inside = id[u] >= 0 && id[u] < rows;
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[u].v[e] = inside ? (T)(scale * (float)p[u].v[e]) : (T)0.0f;
+        if (t0 + u < tokens) put(out + (t0 + u) * ldo + (int64_t)c * N, p[u], past);
+      }
     }
   }
 }
@@ -86,33 +108,34 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool va
 }
 
 // Stable places of one batch of kSortThreads items.  `base[d]` is where the next item with digit d goes; it is advanced.
-// `wave_at[w][d]` is zero on entry and on exit.  Every thread of the block calls it.
+// `wave_at[w][d]` is zero on entry and on exit: only the entries of digits that wave w has are set, and its leaders clear them
+// again after its lanes have read them (LDS accesses of a wave stay in order).  Every thread of the block calls it.
 __device__ __forceinline__ uint32_t place(uint32_t digit, int bits, bool valid, uint32_t* base, uint32_t* wave_at) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << bits;
   const uint64_t mask = same_digit(digit, bits, valid);
   const uint32_t rank = __popcll(mask & ((1ull << lane) - 1));
   const bool leader = valid && rank == 0;
-  if (leader) wave_at[wave * digits + digit] = __popcll(mask);
+  volatile uint32_t* mine = wave_at + wave * digits + digit;
+  if (leader) *mine = __popcll(mask);
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kSortThreads) {
-    uint32_t at = base[d];
+    uint32_t n[kWaves], at = base[d];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n[w] = wave_at[w * digits + d];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const uint32_t n = wave_at[w * digits + d];
-      wave_at[w * digits + d] = at;
-      at += n;
+      if (n[w]) wave_at[w * digits + d] = at;
+      at += n[w];
     }
     base[d] = at;
   }
   __syncthreads();
-  const uint32_t to = valid ? wave_at[wave * digits + digit] + rank : 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
-  __syncthreads();
+  const uint32_t to = valid ? *mine + rank : 0;
+  if (leader) *mine = 0;
   return to;
 }
 
-// Exclusive prefix sum over `digits` (<= 512) totals, one per thread; every thread of the block calls it.
+// Exclusive prefix sum over `digits` (<= 1024) totals, one per thread; every thread of the block calls it.
 __device__ __forceinline__ uint32_t digit_prefix(uint32_t v, uint32_t* wave_sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t inc = v;
@@ -134,11 +157,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void* __
                                                                   uint32_t rows, int key_bits, uint32_t* __restrict__ keys,
                                                                   uint32_t* __restrict__ order) {
   __shared__ uint2 item[2][kSmall];
-  __shared__ uint32_t wave_at[kWaves * 256];
-  __shared__ uint32_t base[256], wave_sum[kWaves];
+  __shared__ uint32_t wave_at[kWaves << kMaxDigit];
+  __shared__ uint32_t base[1 << kMaxDigit], wave_sum[kWaves];
   for (int i = threadIdx.x; i < tokens; i += kSortThreads) item[0][i] = make_uint2(load_key(ids, wide, i, rows), (uint32_t)i);
-  for (int i = threadIdx.x; i < kWaves * 256; i += kSortThreads) wave_at[i] = 0;
-  const int passes = (key_bits + 7) / 8, bits = (key_bits + passes - 1) / passes, digits = 1 << bits;
+  const int passes = (key_bits + kMaxDigit - 1) / kMaxDigit, bits = (key_bits + passes - 1) / passes, digits = 1 << bits;
+  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
   int cur = 0;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
@@ -208,11 +231,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass a, 
   for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
   uint32_t total = 0, before = 0;
   if (threadIdx.x < digits) {
-#pragma unroll 8
-    for (int b = 0; b < blocks; ++b) {
-      const uint32_t n = counts[(int64_t)b * digits + threadIdx.x];
-      total += n;
-      before += b < (int)blockIdx.x ? n : 0;
+    for (int b0 = 0; b0 < blocks; b0 += 32) {
+      uint32_t n[32];                     // (requested together; past the end the last block's again)
+#pragma unroll
+      for (int k = 0; k < 32; ++k) n[k] = counts[(int64_t)min(b0 + k, blocks - 1) * digits + threadIdx.x];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        total += b0 + k < blocks ? n[k] : 0;
+        before += b0 + k < (int)blockIdx.x ? n[k] : 0;
+      }
     }
   }
   const uint32_t at = digit_prefix(total, wave_sum);
@@ -250,6 +277,8 @@ struct SumArgs {
   float* pieces;             // [chunks][2][piece_ld]: the run that began before the chunk, the run that goes on behind it
   int64_t piece_ld;
   int64_t sum_blocks;        // blocks past these write the zeros of rows that do not occur
+  bool past;                 // the gradient is larger than the caches
+  int join_chunks;           // chunks whose crossing runs one block joins (at most 64: one lane looks at each)
 };
 
 template <typename T, int N, bool UPDATE>
@@ -264,7 +293,7 @@ __device__ __forceinline__ void store_row(const SumArgs& a, T* table, uint32_t r
 #pragma unroll
     for (int e = 0; e < N; ++e) p.v[e] = (T)(f * acc[e]);
   }
-  *at = p;
+  put(reinterpret_cast<T*>(at), p, !UPDATE && a.past);
 }
 
 template <typename T, int N, bool UPDATE>
@@ -291,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
 #pragma unroll
     for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
     for (int r = group; r < kFillRows; r += groups)
-      if (missing[r] && in_row) *reinterpret_cast<Pack<T, N>*>(table + (row0 + r) * a.ldt + (int64_t)pack * N) = zero;
+      if (missing[r] && in_row) put(table + (row0 + r) * a.ldt + (int64_t)pack * N, zero, a.past);
     return;
   }
   const int64_t chunk = (int64_t)blockIdx.x * groups + group;
@@ -304,8 +333,9 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  float* piece = a.pieces + chunk * 2 * a.piece_ld + (int64_t)pack * N;
-  constexpr int kAhead = 4;
+  Pack<float, N>* piece = reinterpret_cast<Pack<float, N>*>(a.pieces + chunk * 2 * a.piece_ld + (int64_t)pack * N);
+  Pack<float, N> sum;
+  constexpr int kAhead = AHEAD;
   for (int64_t i0 = first; i0 < last && run < a.rows; i0 += kAhead) {
     uint32_t key[kAhead];
     Pack<T, N> v[kAhead];
@@ -320,7 +350,8 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
       if (key[j] != run) {
         if (from_before) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) piece[e] = acc[e];
+          for (int e = 0; e < N; ++e) sum.v[e] = acc[e];
+          *piece = sum;
         } else {
           store_row<T, N, UPDATE>(a, table, run, pack, acc, f);
         }
@@ -338,55 +369,90 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
   if (run >= a.rows) return;                               // padding sits behind every row
   const bool goes_on = last < a.tokens && a.keys[last] == run;
   if (from_before || goes_on) {
-    float* to = from_before ? piece : piece + a.piece_ld;
 #pragma unroll
-    for (int e = 0; e < N; ++e) to[e] = acc[e];
+    for (int e = 0; e < N; ++e) sum.v[e] = acc[e];
+    *(from_before ? piece : reinterpret_cast<Pack<float, N>*>(reinterpret_cast<float*>(piece) + a.piece_ld)) = sum;
   } else {
     store_row<T, N, UPDATE>(a, table, run, pack, acc, f);
   }
 }
 
+// How many chunks from `c0` on begin with `run`.  They are the first ones or none (the ids are sorted): 64 places at a time, then
+// 64 places between the last that does and the first that does not.
+__device__ __forceinline__ int64_t run_of_chunks(const SumArgs& a, int64_t c0, uint32_t run, int lane) {
+  int64_t low = c0, n = a.chunks - c0;         // chunks c0 .. low - 1 do, chunks from low + n on do not
+  while (n > 0) {
+    const int64_t step = (n + 63) / 64, c = low + lane * step;
+    const int hits = __popcll(__ballot(c < low + n && a.keys[min(c, a.chunks - 1) * a.chunk] == run));
+    if (hits == 0) break;
+    const int64_t end = low + n;
+    low += (hits - 1) * step + 1;
+    n = min(step - 1, end - low);
+  }
+  return low - c0;
+}
+
 // Runs that cross chunks: the chunk a run begins in names it; its pieces are that chunk's second workspace row and the
-// first rows of the chunks behind it.  Four waves take every fourth piece each; their sums meet in order.
+// first rows of the chunks behind it.
 template <typename T, bool UPDATE>
-__global__ __launch_bounds__(kThreads) void join_kernel(SumArgs a, T* __restrict__ table) {
-  __shared__ f32x4 part[4][64];
+__global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(SumArgs a, T* __restrict__ table) {
+  __shared__ f32x4 part[kJoinWaves][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = (blockIdx.y * 64 + lane) * 4;
   const float f = UPDATE ? a.lr[0] * a.scale : a.scale;
-  for (int k = 0; k < kJoinChunks; ++k) {
-    const int64_t chunk = (int64_t)blockIdx.x * kJoinChunks + k;
-    if (chunk >= a.chunks) break;
-    const int64_t first = chunk * a.chunk, last = first + a.chunk;
-    if (last >= a.tokens) break;
-    const uint32_t run = a.keys[last - 1];
-    if (run >= a.rows || a.keys[last] != run) continue;
-    if (a.keys[first] == run && first > 0 && a.keys[first - 1] == run) continue;    // it began before this chunk
-    // how many chunks behind this one begin with the run: the ids are sorted, so the first that does not ends the count
-    int64_t pieces = 0;
-    for (int64_t c0 = chunk + 1;; c0 += 64) {
-      const int64_t c = c0 + lane;
-      const uint64_t same = __ballot(c < a.chunks && a.keys[min(c, a.chunks - 1) * a.chunk] == run);
-      pieces += __popcll(same);
-      if (same != ~0ull) break;
-    }
+  // lane l looks at chunk chunk0 + l: its first key, and whether its last run is one that begins in it and goes on behind it
+  const int64_t chunk0 = (int64_t)blockIdx.x * a.join_chunks, mine = min(chunk0 + lane, a.chunks - 1);
+  const int64_t first = mine * a.chunk, last = min(first + a.chunk, a.tokens);
+  const uint32_t first_key = a.keys[first], last_key = a.keys[last - 1];
+  const uint32_t before = a.keys[max(first - 1, (int64_t)0)], behind = a.keys[min(last, a.tokens - 1)];
+  const bool begins = lane < a.join_chunks && chunk0 + lane < a.chunks && last < a.tokens && last_key < a.rows && behind == last_key &&
+                      !(first_key == last_key && first > 0 && before == last_key);
+  uint64_t todo = __ballot(begins);
+  auto add = [&](int64_t chunk, int64_t pieces, int64_t p, int step) {       // pieces p, p + step, ...; piece 0 in the run's own chunk
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    if (col < a.dim) {
-      const float* src = a.pieces + chunk * 2 * a.piece_ld + col;
-      if (wave == 0) sum = *reinterpret_cast<const f32x4*>(src + a.piece_ld);
-#pragma unroll 8
-      for (int64_t p = wave + 1; p <= pieces; p += 4) sum += *reinterpret_cast<const f32x4*>(src + p * 2 * a.piece_ld);
-    }
-    __syncthreads();
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave == 0 && col < a.dim) {
-      sum = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
-      T* row = table + (int64_t)run * a.ldt + col;
+    if (col >= a.dim) return sum;
+    const float* src = a.pieces + chunk * 2 * a.piece_ld + col;
+    for (; p <= pieces; p += 8 * step) {
+      f32x4 v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < a.dim) row[e] = UPDATE ? (T)((float)row[e] - f * sum[e]) : (T)(f * sum[e]);
+      for (int k = 0; k < 8; ++k) {
+        const int64_t q = min(p + k * step, pieces);
+        v[k] = *reinterpret_cast<const f32x4*>(src + (q ? q * 2 : 1) * a.piece_ld);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (p + k * step <= pieces) sum += v[k];
     }
+    return sum;
+  };
+  auto store = [&](uint32_t run, f32x4 sum) {
+    T* row = table + (int64_t)run * a.ldt + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < a.dim) row[e] = UPDATE ? (T)((float)row[e] - f * sum[e]) : (T)(f * sum[e]);
+  };
+  for (int turn = 0; todo; ++turn, todo &= todo - 1) {
+    const int l = __builtin_ctzll(todo);
+    const uint32_t run = __shfl(last_key, l);
+    const int64_t chunk = chunk0 + l;
+    // the chunks behind this one that begin with the run; the ids are sorted, so the first that does not ends the count
+    uint64_t same = __ballot(chunk0 + lane < a.chunks && first_key == run) >> (l + 1 < 64 ? l + 1 : 63);
+    if (l == 63) same = 0;
+    int64_t pieces = same == ~0ull ? 64 : __builtin_ctzll(~same);
+    if (chunk + pieces + 1 == chunk0 + 64) pieces += run_of_chunks(a, chunk0 + 64, run, lane);       // past the chunks the lanes look at
+    if (pieces <= kLongRun) {
+      if (turn % kJoinWaves == wave) store(run, add(chunk, pieces, 0, 1));
+      continue;
+    }
+    part[wave][lane] = add(chunk, pieces, wave, kJoinWaves);
+    __syncthreads();
+    if (wave == 0) {
+      f32x4 sum = part[0][lane];
+#pragma unroll
+      for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
+      store(run, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -396,10 +462,10 @@ inline int log2_lanes(int packs) {
   return l;
 }
 
-// Sorted positions per chunk: enough chunks for 256 CUs x 1024 threads, at least 4 and at most 32 positions.
+// Sorted positions per chunk: enough chunks for 256 CUs x 1024 threads, at least 4 and at most 64 positions.
 inline int chunk_of(int64_t tokens, int64_t lanes) {
   const int64_t c = tokens * lanes / (256 * 1024);
-  return c < 4 ? 4 : c > 32 ? 32 : (int)c;
+  return c < 4 ? 4 : c > 64 ? 64 : (int)c;
 }
 
 struct Workspace {
@@ -459,8 +525,13 @@ void launch_sums(SumArgs a, const T* g, T* table, int64_t fill_rows, hipStream_t
   const int64_t fill = (fill_rows + kFillRows - 1) / kFillRows;
   const dim3 grid((unsigned)(a.sum_blocks + fill), (a.packs + lanes - 1) / lanes);
   if (grid.x) sum_kernel<T, N, UPDATE><<<grid, kThreads, 0, s>>>(a, g, table);
-  if (a.chunks > 1)
-    join_kernel<T, UPDATE><<<dim3((unsigned)((a.chunks + kJoinChunks - 1) / kJoinChunks), (a.dim + 255) / 256), kThreads, 0, s>>>(a, table);
+  if (a.chunks > 1) {
+    // few enough chunks per block that a thousand blocks share the runs: they are a chain of trips to memory each, and the
+    // frequent tokens' runs lie side by side (32768 tokens x 256: 64 chunks a block 23 us, 4 chunks 8 us)
+    const int64_t slices = (a.dim + 255) / 256, per = a.chunks * slices / 1024;
+    a.join_chunks = per < 4 ? 4 : per > 64 ? 64 : (int)per;
+    join_kernel<T, UPDATE><<<dim3((unsigned)((a.chunks + a.join_chunks - 1) / a.join_chunks), (unsigned)slices), kJoinWaves * 64, 0, s>>>(a, table);
+  }
 }
 
 template <typename T>
@@ -483,6 +554,7 @@ int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const v
   a.lr = lr;
   a.pieces = reinterpret_cast<float*>(ws + w.pieces);
   a.piece_ld = w.piece_ld;
+  a.past = rows * dim * (int64_t)sizeof(T) > kCaches;
   const T* gp = static_cast<const T*>(g);
   T* tp = static_cast<T*>(table);
   const int bytes = dtf_access_bytes((uint64_t)g | (uint64_t)table | (uint64_t)(ldg * sizeof(T)) | (uint64_t)(ldt * sizeof(T)) |
@@ -509,9 +581,13 @@ int launch_lookup(const void* table, int64_t ld, int64_t rows, const void* ids, 
   auto go = [&](auto n) {
     constexpr int N = decltype(n)::value;
     const int packs = dim / N, l = log2_lanes(packs), groups = kThreads >> l;
-    int64_t grid = (tokens + groups - 1) / groups;
+    // four tokens at a time once that still leaves eight blocks for every CU
+    const bool many = tokens / (4 * groups) >= 8 * 256;
+    int64_t grid = (tokens + groups * (many ? 4 : 1) - 1) / (groups * (many ? 4 : 1));
     if (grid > (1 << 20)) grid = 1 << 20;       // (blocks x threads stays below 2^32)
-    lookup_kernel<T, N><<<(unsigned)grid, kThreads, 0, s>>>(tp, ld, rows, ids, wide, tokens, packs, l, scale, op, ldo);
+    const bool past = tokens * dim * (int64_t)sizeof(T) > kCaches;
+    if (many) lookup_kernel<T, N, 4><<<(unsigned)grid, kThreads, 0, s>>>(tp, ld, rows, ids, wide, tokens, packs, l, scale, op, ldo, past);
+    else lookup_kernel<T, N, 1><<<(unsigned)grid, kThreads, 0, s>>>(tp, ld, rows, ids, wide, tokens, packs, l, scale, op, ldo, past);
   };
   if (bytes == 16) go(std::integral_constant<int, 16 / sizeof(T)>());
   else if (bytes == 8) go(std::integral_constant<int, 8 / sizeof(T)>());
