@@ -43,19 +43,17 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Opti
     ld = hb.typed_rows(table, "table")
     flat = hb.int_vector(ids, "ids", table.device)
     rows, dim = table.shape
-    shape = tuple(ids.shape) + (dim,)
     if out is None:
-        dst = torch.empty((flat.numel(), dim), device=table.device, dtype=table.dtype)
-        result, ldo = dst.view(shape), dim
+        dst, ldo = table.new_empty((*ids.shape, dim)), dim
     else:
         ldo = _out_matrix(out, (flat.numel(), dim), table, "out")
         if hb.overlap(out, table) or hb.overlap(out, flat):
             raise hb.HipKernelError("lookup: out must not overlap the table or the ids")
-        dst = result = out
+        dst = out
     hb._check(lib.dtf_embed_lookup(table.data_ptr(), hb.TYPE_CODES[table.dtype], rows, dim, ld, flat.data_ptr(),
                                    int(flat.dtype == torch.int64), flat.numel(), float(scale), dst.data_ptr(), ldo,
                                    hb._stream(table)), "dtf_embed_lookup")
-    return result
+    return dst
 
 
 def _workspace(lib, tokens: int, dim: int, device) -> torch.Tensor:
@@ -74,7 +72,7 @@ def lookup_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: float =
     g, ldg = _gradient_rows(ids, grad)
     dim = g.shape[1]
     if out is None:
-        out = torch.empty((rows, dim), device=g.device, dtype=g.dtype)
+        out = g.new_empty((rows, dim))
     ldt = _out_matrix(out, (rows, dim), g, "out")
     if hb.overlap(out, g) or hb.overlap(out, flat):
         raise hb.HipKernelError("lookup_grad: out must not overlap the upstream gradient or the ids")

@@ -291,28 +291,36 @@ TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DTF_
 
 def typed_rows(t: torch.Tensor, name: str) -> int:
     """Row stride in elements of a 2-D fp32 / bf16 / fp16 GPU matrix with contiguous rows; anything else is refused."""
-    if not t.is_cuda or t.dtype not in TYPE_CODES or t.dim() != 2:
-        raise HipKernelError(f"{name} must be a 2-D float32, bfloat16 or float16 CUDA tensor, got {t.dtype} {tuple(t.shape)} "
+    shape = t.shape
+    if len(shape) != 2 or t.dtype not in TYPE_CODES or not t.is_cuda:
+        raise HipKernelError(f"{name} must be a 2-D float32, bfloat16 or float16 CUDA tensor, got {t.dtype} {tuple(shape)} "
                              f"on {t.device}")
-    cols = t.shape[1]
-    if cols > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < cols:
-        raise HipKernelError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()} for {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(cols, 1)
+    rows, cols = shape
+    if t.is_contiguous():        # (the usual case, on the way to a launch of a few microseconds)
+        return cols or 1
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        raise HipKernelError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()} for {tuple(shape)}")
+    return t.stride(0) if rows > 1 else max(cols, 1)
 
 
 def int_vector(t: torch.Tensor, name: str, device) -> torch.Tensor:
     """``t`` (int32 or int64, any shape, on ``device``) as a contiguous vector."""
     if t.dtype not in (torch.int32, torch.int64) or t.device != device:
         raise HipKernelError(f"{name} must be an int32 or int64 tensor on {device}, got {t.dtype} on {t.device}")
-    return t.reshape(-1).contiguous()
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
+
+
+def _span(t: torch.Tensor):
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.numel() * t.element_size()
+    n = 1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else 0
+    return at, at + n * t.element_size()
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the address ranges of two tensors meet."""
-    def span(t):
-        n = 1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
 
 

@@ -29,7 +29,7 @@ def _operands(logits: torch.Tensor, labels: torch.Tensor):
 def _dz_rows(dz: torch.Tensor, logits: torch.Tensor) -> int:
     if dz.shape != logits.shape or dz.dtype != logits.dtype or dz.device != logits.device:
         raise hb.HipKernelError("sparse_softmax_xent: dz must be shaped and typed like the logits, on their device")
-    if hb.overlap(dz, logits) and (dz.data_ptr() != logits.data_ptr() or dz.stride() != logits.stride()):
+    if (dz.data_ptr() != logits.data_ptr() or dz.stride() != logits.stride()) and hb.overlap(dz, logits):
         raise hb.HipKernelError("sparse_softmax_xent: dz may be the logits themselves, but not overlap them otherwise")
     return hb.typed_rows(dz, "dz")
 
@@ -38,7 +38,7 @@ def _forward(logits, labels, dz, grad_scale, stats):
     lib = hb.require()
     ld, flat = _operands(logits, labels)
     ldz = 0 if dz is None else _dz_rows(dz, logits)
-    loss = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
+    loss = torch.empty((logits.shape[0],), device=logits.device, dtype=torch.float32)
     hb._check(lib.dtf_sparse_xent(logits.data_ptr(), hb.TYPE_CODES[logits.dtype], logits.shape[0], logits.shape[1], ld,
                                   flat.data_ptr(), int(flat.dtype == torch.int64), hb._ptr(dz), ldz, float(grad_scale),
                                   loss.data_ptr(), hb._ptr(stats), hb._stream(logits)), "dtf_sparse_xent")
