@@ -261,11 +261,11 @@ __global__ __launch_bounds__(kStream) void xent_stream_kernel(XentArgs a, T* log
   }
   if (!dz) return;
   const float factor = a.grad_scale / s;
-  for (int i0 = tid; i0 < row.packs; i0 += U * kStream) {
-    P z[U];
+  for (int i0 = tid; i0 < row.packs; i0 += 2 * kStream) {
+    P z[2];
     row.load(i0, kStream, z);
 #pragma unroll
-    for (int k = 0; k < U; ++k)
+    for (int k = 0; k < 2; ++k)
       if (i0 + k * kStream < row.packs)
         store_pack<T, SAME>(row, dst, i0 + k * kStream,
                             gradient_pack<T>(row, i0 + k * kStream, z[k], m, factor, a.grad_scale, (int)label));

@@ -179,7 +179,8 @@ _OP_NAMES = {"const": "Const", "placeholder": "Placeholder", "random_normal": "r
              "init_vars": "init", "group": "group_deps", "no_op": "NoOp", "train": "GradientDescent",
              "scalar_summary": "ScalarSummary", "merge_summary": "Merge/MergeSummary", "assign": "Assign",
              "assign_add": "AssignAdd", "stop_gradient": "StopGradient", "maximum": "Maximum", "minimum": "Minimum",
-             "abs": "Abs", "greater": "Greater", "less": "Less"}
+             "abs": "Abs", "greater": "Greater", "less": "Less", "embedding_lookup": "embedding_lookup",
+             "sparse_softmax_xent": "SparseSoftmaxCrossEntropyWithLogits"}
 
 
 def _default_op_name(op: str) -> str:
@@ -466,6 +467,32 @@ def softmax_cross_entropy_with_logits(_sentinel=None, labels=None, logits=None, 
     return Tensor("softmax_xent", (labels, logits), {}, name=name, dtype=logits.dtype, shape=shape)
 
 
+def embedding_lookup(params, ids, name=None, scale: float = 1.0) -> Tensor:
+    """``scale * params[ids]``: rows of a 2-D table for ids of any shape.  An id outside the table gives a row of zeros and has no
+    gradient (padding).  ``params``: one table, or a list of one."""
+    if isinstance(params, (list, tuple)):
+        if len(params) != 1:
+            raise ValueError("embedding_lookup: one table (a table dealt over several variables is not supported)")
+        params = params[0]
+    table, ids = _t(params), _t(ids)
+    if table.shape is not None and len(table.shape) != 2:
+        raise ValueError(f"embedding_lookup: the table must be a matrix, got shape {table.shape}")
+    if ids.dtype not in (int32, int64):
+        raise ValueError(f"embedding_lookup: ids must be int32 or int64, got {ids.dtype}")
+    shape = None if table.shape is None or ids.shape is None else tuple(ids.shape) + (table.shape[1],)
+    return Tensor("embedding_lookup", (table, ids), {"scale": float(scale)}, name=name, dtype=table.dtype, shape=shape)
+
+
+def sparse_softmax_cross_entropy_with_logits(_sentinel=None, labels=None, logits=None, name=None) -> Tensor:
+    """Loss of every row of ``logits [..., classes]`` against integer ``labels [...]``.  A negative label is padding: loss and gradient
+    0; a label that is no class gives NaN."""
+    labels, logits = _t(labels), _t(logits)
+    if labels.dtype not in (int32, int64):
+        raise ValueError(f"sparse_softmax_cross_entropy_with_logits: labels must be int32 or int64, got {labels.dtype}")
+    shape = None if logits.shape is None else tuple(logits.shape[:-1])
+    return Tensor("sparse_softmax_xent", (labels, logits), {}, name=name, dtype=logits.dtype, shape=shape)
+
+
 def _axes(axis, reduction_indices):
     ax = axis if axis is not None else reduction_indices
     if ax is None:
@@ -537,6 +564,8 @@ class _NN:
     softmax = staticmethod(softmax)
     log_softmax = staticmethod(log_softmax)
     softmax_cross_entropy_with_logits = staticmethod(softmax_cross_entropy_with_logits)
+    sparse_softmax_cross_entropy_with_logits = staticmethod(sparse_softmax_cross_entropy_with_logits)
+    embedding_lookup = staticmethod(embedding_lookup)
 
 
 nn = _NN()

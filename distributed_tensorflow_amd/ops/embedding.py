@@ -104,6 +104,15 @@ def lookup_sgd(table: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, lr: t
     return table
 
 
+def update_rows(table: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, lr: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``lookup_sgd`` for tables on either kind of device (CPU tensors: torch, same rules)."""
+    if table.is_cuda:
+        return lookup_sgd(table, ids, grad, lr, scale)
+    flat = ids.reshape(-1).long()
+    inside = (flat >= 0) & (flat < table.shape[0])
+    return table.index_add_(0, flat[inside], grad.reshape(-1, table.shape[1])[inside], alpha=-float(lr) * float(scale))
+
+
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale):

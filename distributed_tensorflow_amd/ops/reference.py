@@ -147,3 +147,20 @@ def random_normal(shape, seed: int, offset: int = 0, mean: float = 0.0, stddev: 
     t = torch.empty(tuple(shape), dtype=torch.float32)
     t.normal_(mean, stddev, generator=gen)
     return t.to(device)
+
+
+def orthogonalize(x: torch.Tensor, eps: float = 1e-7) -> torch.Tensor:
+    """Oracle (and CPU path) of ops/muon.py: five Newton-Schulz steps on ``x / (|x|_F + eps)`` in the type of ``x``."""
+    flip = x.shape[0] > x.shape[1]
+    y = x.t() if flip else x
+    y = (y.double() / (y.double().square().sum().sqrt() + eps)).to(x.dtype)
+    for _ in range(5):
+        p = y @ y.t()
+        y = 3.4445 * y + (-4.7750 * p + 2.0315 * (p @ p)) @ y
+    return y.t() if flip else y
+
+
+def muon_step(w: torch.Tensor, g: torch.Tensor, buf: torch.Tensor, lr: float, momentum: float, nesterov: bool) -> None:
+    """Oracle (and CPU path) of one matrix of ops/muon.py's ``muon_step``, in place."""
+    buf.mul_(momentum).add_(g)
+    w.sub_(lr * max(1.0, w.shape[1] / w.shape[0]) ** 0.5 * orthogonalize(g + momentum * buf if nesterov else buf))

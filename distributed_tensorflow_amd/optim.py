@@ -72,6 +72,60 @@ class GradientDescentOptimizer(Optimizer):
         return self.learning_rate
 
 
+def lookup_tables(loss: Optional[G.Tensor]) -> set:
+    """Variables that ``loss`` reads through embedding lookups alone (not also as a factor of a product, say)."""
+    tables, others, seen, stack = set(), set(), set(), [loss] if loss is not None else []
+    while stack:
+        node = stack.pop()
+        if node in seen:
+            continue
+        seen.add(node)
+        for k, i in enumerate(node.inputs):
+            if isinstance(i, G.Variable):
+                (tables if node.op == "embedding_lookup" and k == 0 else others).add(i)
+            else:
+                stack.append(i)
+    return tables - others
+
+
+class MuonOptimizer(Optimizer):
+    """Muon: every matrix of the model takes the orthogonalised direction of its momentum,
+
+        buf = momentum * buf + g;   W -= learning_rate * sqrt(max(1, cols / rows)) * factor(g + momentum * buf)
+
+    (``buf`` itself without ``use_nesterov``; ``factor``: ops/muon.py), all matrices in one sequence of launches; the other
+    variables - biases, and the tables of embedding lookups, whose rows are not directions of one map - take plain gradient
+    descent with ``sgd_learning_rate`` (default: ``learning_rate``).  The momentum of ``W`` is the variable ``<name of W>/Muon``:
+    saved and restored with the model.  Local sessions only: a parameter server applies plain gradient descent."""
+
+    def __init__(self, learning_rate: float, momentum: float = 0.95, use_nesterov: bool = True,
+                 sgd_learning_rate: Optional[float] = None, use_locking: bool = False, name: str = "Muon"):
+        super().__init__(use_locking, name)
+        self.learning_rate = float(learning_rate)
+        self.momentum = float(momentum)
+        self.use_nesterov = bool(use_nesterov)
+        self.sgd_learning_rate = self.learning_rate if sgd_learning_rate is None else float(sgd_learning_rate)
+        if not 0.0 <= self.momentum < 1.0:
+            raise ValueError(f"MuonOptimizer: momentum must be in [0, 1), got {momentum}")
+
+    def lr_value(self) -> float:
+        """Learning rate of the variables that take plain gradient descent."""
+        return self.sgd_learning_rate
+
+    def apply_gradients(self, grads_and_vars, global_step=None, name=None) -> G.Tensor:
+        op = super().apply_gradients(grads_and_vars, global_step, name)
+        tables = lookup_tables(op.attrs["loss"])
+        slots = {}
+        for v in op.attrs["var_list"]:
+            if len(v.shape) == 2 and v not in tables:
+                # (one momentum per variable, also where two train ops update it)
+                slot = next((s for s in v.graph.variables if s.op_name == f"{v.op_name}/Muon"), None)
+                slots[v] = slot if slot is not None else G.Variable(trainable=False, name=f"{v.op_name}/Muon", _init_spec=("zeros",),
+                                                                    _shape=v.shape, _scoped=False)
+        op.attrs["slots"] = slots
+        return op
+
+
 class QueueRunner:
     """The chief's aggregation loop, runnable on a thread (``Supervisor.start_queue_runners``)."""
 
@@ -155,6 +209,8 @@ class SyncReplicasOptimizer(Optimizer):
                  variable_averages=None, variables_to_average=None, use_locking: bool = False,
                  name: str = "sync_replicas"):
         super().__init__(use_locking, name)
+        if isinstance(opt, MuonOptimizer):
+            raise ValueError("SyncReplicasOptimizer aggregates gradients for plain gradient descent; MuonOptimizer is for local sessions")
         self._opt = opt
         self.replicas_to_aggregate = int(replicas_to_aggregate)
         self.total_num_replicas = int(total_num_replicas if total_num_replicas is not None else replicas_to_aggregate)

@@ -16,7 +16,7 @@ split by the round-robin placement (2 PS: 4,044 B to ps0, 314,000 B to ps1).
 from __future__ import annotations
 
 import struct
-from typing import List, Optional
+from typing import Dict, List, Optional
 
 import numpy as np
 import torch
@@ -89,14 +89,30 @@ class LocalVariableStore:
         if bump_step and self._gs_off is not None:
             gs = self.slab[self._gs_off:self._gs_off + 1]
         if self.slab.is_cuda:
-            if self._lr_t is None or float(self._lr_cached) != float(lr):
-                self._lr_t = torch.full((1,), float(lr), dtype=torch.float32, device=self.device)
-                self._lr_cached = float(lr)
-            hb.sgd_apply_(self.slab, grads, self._lr_t, 1.0, False, gs)
+            hb.sgd_apply_(self.slab, grads, self.lr_tensor(lr), 1.0, False, gs)
         else:
             self.slab.sub_(grads, alpha=float(lr))
             if gs is not None:
                 gs.add_(1.0)
+
+    def lr_tensor(self, lr: float) -> torch.Tensor:
+        """``lr`` as one float32 on the slab's device (made again only when it changes)."""
+        if self._lr_t is None or float(self._lr_cached) != float(lr):
+            self._lr_t = torch.full((1,), float(lr), dtype=torch.float32, device=self.device)
+            self._lr_cached = float(lr)
+        return self._lr_t
+
+    def apply_vars(self, grads: Dict[str, torch.Tensor], lr: float, bump_step: bool = True):
+        """Plain gradient descent of the named variables alone: the rest of the slab (large tables, whose rows are updated where
+        they lie) is neither read nor written."""
+        for name, g in grads.items():
+            p = self.layout.view(self.slab, name).view(-1)
+            if p.is_cuda:
+                hb.sgd_apply_(p, g.contiguous().view(-1), self.lr_tensor(lr))
+            else:
+                p.sub_(g.reshape(-1), alpha=float(lr))
+        if bump_step and self._gs_off is not None:
+            self.slab[self._gs_off:self._gs_off + 1].add_(1.0)
 
     def global_step(self) -> int:
         if self._gs_off is None:

@@ -36,8 +36,8 @@ from . import graph as G
 from .cluster import ConfigProto, lookup_server
 from .utils.trace import Collector, span
 from .models.mlp import MLPEngine
-from .ops import gemm as gemm_op
-from .optim import Optimizer, SyncReplicasOptimizer
+from .ops import embedding as embedding_op, gemm as gemm_op, muon as muon_op, reference as reference_op, xent as xent_op
+from .optim import MuonOptimizer, Optimizer, SyncReplicasOptimizer, lookup_tables
 from .parallel.store import LocalVariableStore, RemoteVariableStore
 from .placement import DeviceSpec
 from .summary import Summary
@@ -214,6 +214,7 @@ class Session:
         self._engines: Dict[Any, MLPEngine] = {}
         self._plans: Dict[int, Any] = {}          # train op -> what runs it (fused model, dense stack, accuracy nodes)
         self._reads_vars: Dict[Any, bool] = {}    # node -> whether evaluating it reads variables
+        self._lookups = None                      # during a step with sparse updates: (tables, what was looked up of them)
         self._replica_owner = None
         self._closed = False
         self.fused_steps = 0
@@ -488,6 +489,19 @@ class Session:
             # the hand-written fp32 MFMA GEMM (forward and, through autograd, both gradient products) on a GPU;
             # torch.matmul for what it does not cover
             r = gemm_op.matmul(ev(ins[0]), ev(ins[1]), node.attrs["transpose_a"], node.attrs["transpose_b"])
+        elif op == "embedding_lookup":
+            if self._lookups is not None and ins[0] in self._lookups[0]:
+                # a table whose rows are updated where they lie: the rows that were looked up are the leaf, not the table
+                ids = ev(ins[1])
+                r = embedding_op.embedding_lookup(self._var_view(ins[0]).detach(), ids, node.attrs["scale"]).requires_grad_(True)
+                self._lookups[1].append((ins[0], ids, node.attrs["scale"], r))
+            else:
+                r = embedding_op.embedding_lookup(ev(ins[0]), ev(ins[1]), node.attrs["scale"])
+        elif op == "sparse_softmax_xent":
+            labels, logits = ev(ins[0]), ev(ins[1])
+            if labels.shape != logits.shape[:-1]:
+                raise ValueError(f"{node.name}: labels of shape {tuple(labels.shape)} for logits of shape {tuple(logits.shape)}")
+            r = xent_op.sparse_softmax_xent(logits.reshape(-1, logits.shape[-1]), labels.reshape(-1)).view(labels.shape)
         elif op == "add":
             r = ev(ins[0]) + ev(ins[1])
         elif op == "sub":
@@ -668,7 +682,12 @@ class Session:
                     dense = None
             head = m if m is not None else dense
             acc_nodes = [n for n in self.graph.nodes if head is not None and match_accuracy(n, head)]
-            plan = {"mlp": m, "dense": dense, "acc_nodes": acc_nodes}
+            # Tables whose rows can be updated where they lie: read by lookups alone, next to the step that looks them up
+            tables = set()
+            if m is None and dense is None and not self.store.is_remote \
+                    and not isinstance(train_op.attrs["optimizer"], SyncReplicasOptimizer):
+                tables = lookup_tables(loss) & set(train_op.attrs["var_list"])
+            plan = {"mlp": m, "dense": dense, "acc_nodes": acc_nodes, "tables": tables}
             self._plans[id(train_op)] = plan
         return plan
 
@@ -727,6 +746,8 @@ class Session:
             elif not self._served_by_step(f, m, plan):
                 return None
         opt = train_op.attrs["optimizer"]
+        if isinstance(opt, MuonOptimizer):       # (_run_train refuses it, before anything is pushed)
+            return None
         if not self._local_step_ready:           # (the shards are allocated and mapped before the first view of them)
             self.store.sync_local_step()
             self._local_step_ready = True
@@ -778,6 +799,10 @@ class Session:
         m = plan["mlp"]
         lr = opt.lr_value()
         sync = isinstance(opt, SyncReplicasOptimizer) and self.store.is_remote
+        plain = not isinstance(opt, MuonOptimizer)       # the update is p -= lr * g for every variable
+        if not plain and self.store.is_remote:
+            raise NotImplementedError("MuonOptimizer: variables on parameter servers take plain gradient descent; use a local session")
+        sparse_grads = None
         applied = False
         if m is not None and m["x"] in feed:
             xv = feed[m["x"]]
@@ -786,7 +811,7 @@ class Session:
             with span("stage"):
                 self._stage(eng, m, feed)
             with span("step"):
-                if not self.store.is_remote:
+                if not self.store.is_remote and plain:
                     # no parameter server: the SGD update happens inside the step's two launches
                     self._bind_local_update(eng, train_op, lr)
                     eng.step_fused(0)
@@ -823,7 +848,7 @@ class Session:
                 eng._x_stage.copy_(self._as_f32(feed[d["x"]]), non_blocking=True)
                 eng._y_stage.copy_(self._as_f32(feed[d["y_"]]), non_blocking=True)
             with span("step"):
-                if not self.store.is_remote:
+                if not self.store.is_remote and plain:
                     gs_var = train_op.attrs["global_step"]
                     eng.set_lr(lr) if getattr(eng, "_lr_val", None) != lr else None
                     eng._lr_val = lr
@@ -840,6 +865,27 @@ class Session:
                 cache[n] = host[1]
             self.fused_steps += 1
             self.dense_steps += 1
+        elif plan["tables"]:
+            var_list = [v for v in train_op.attrs["var_list"] if v not in plan["tables"]]
+            leaves = {v: self._var_view(v).detach().clone().requires_grad_(True) for v in var_list}
+            fcache = {}
+            self._lookups = (plan["tables"], [])
+            try:
+                with span("step_generic"):
+                    loss_val = self._eval(train_op.attrs["loss"], feed, fcache, leaves)
+                    looked_up = self._lookups[1]
+                    grads = torch.autograd.grad(loss_val, [leaves[v] for v in var_list] + [r for _, _, _, r in looked_up],
+                                                allow_unused=True)
+            finally:
+                self._lookups = None
+            with span("row_updates"):
+                for (table, ids, scale, _), g in zip(looked_up, grads[len(var_list):]):
+                    if g is not None:
+                        embedding_op.update_rows(self._var_view(table), ids, g, self.store.lr_tensor(lr), scale)
+            sparse_grads = {v.op_name: g for v, g in zip(var_list, grads) if g is not None}
+            for k, val in fcache.items():   # forward values seen by the other fetches
+                cache[k] = val.detach() if isinstance(val, torch.Tensor) else val
+            self.generic_steps += 1
         else:
             self.grad.zero_()
             var_list = train_op.attrs["var_list"]
@@ -864,6 +910,13 @@ class Session:
             return
         if applied:
             return
+        if not plain:
+            with span("muon"):
+                self._muon_update(train_op, opt, sparse_grads)
+        if sparse_grads is not None:
+            with span("push_apply"):
+                self.store.apply_vars(sparse_grads, lr, bump_step=train_op.attrs["global_step"] is not None)
+            return
         if sync:
             if not self._local_step_ready:
                 self.store.sync_local_step()
@@ -884,6 +937,35 @@ class Session:
             with span("push_apply"):
                 self.store.push_apply(self.grad, lr, opt.use_locking,
                                       bump_step=train_op.attrs["global_step"] is not None)
+
+    def _muon_update(self, train_op, opt: MuonOptimizer, grads: Optional[Dict[str, torch.Tensor]]):
+        """The matrices of a train op: momentum, orthogonalised direction, weights, all in place; their gradients then are
+        out of what plain gradient descent applies (``grads`` by name, or the gradient slab if None)."""
+        slots = train_op.attrs["slots"]
+        if grads is not None:
+            for v in slots:                       # (a plan's tensors stay: the gradients go to the slab)
+                if v.op_name in grads:
+                    self.layout.view(self.grad, v.op_name).copy_(grads.pop(v.op_name))
+                else:
+                    self.layout.view(self.grad, v.op_name).zero_()
+        triples = [(self._var_view(v), self.layout.view(self.grad, v.op_name), self._var_view(s)) for v, s in slots.items()]
+        if not triples:
+            return
+        if self.device.type == "cuda":
+            key = ("muon", id(train_op))
+            plan = self._engines.get(key)
+            if plan is None:
+                plan = self._engines[key] = muon_op.MuonPlan(*zip(*triples))
+                plan.lr, plan.lr_value = torch.zeros(1, dtype=torch.float32, device=self.device), 0.0
+            if plan.lr_value != opt.learning_rate:
+                plan.lr.fill_(opt.learning_rate)
+                plan.lr_value = opt.learning_rate
+            muon_op.muon_step(plan, plan.lr, momentum=opt.momentum, nesterov=opt.use_nesterov)
+        else:
+            for w, g, buf in triples:
+                reference_op.muon_step(w, g, buf, opt.learning_rate, opt.momentum, opt.use_nesterov)
+        for _, g, _ in triples:
+            g.zero_()
 
     def _stats_to_host(self, stats: torch.Tensor) -> torch.Tensor:
         """The two statistics of a fused step on the host; waits for the step."""

@@ -1,6 +1,7 @@
 """``train`` namespace: the ``tf.train.*`` names the reference uses, plus the device-resident loop."""
 from ..cluster import ClusterSpec, Server  # noqa: F401
-from ..optim import GradientDescentOptimizer, Optimizer, QueueRunner, SyncReplicasOptimizer  # noqa: F401
+from ..optim import (GradientDescentOptimizer, MuonOptimizer, Optimizer, QueueRunner,  # noqa: F401
+                     SyncReplicasOptimizer)
 from ..placement import (GreedyLoadBalancingStrategy, RoundRobinStrategy,  # noqa: F401
                          replica_device_setter)
 from .saver import Saver, latest_checkpoint, read_bundle  # noqa: F401

@@ -1,0 +1,258 @@
+"""A model over tokens in a graph: embedding lookup, dense layers, cross-entropy against integer labels, trained with plain gradient
+descent and with MuonOptimizer, against the same steps written out in 64 bits.  (CPU sessions here, the same on a GPU with
+``-m gpu``.)
+
+Tolerance of a trained variable: the forward and backward pass in fp32 and the orthogonalisation are each good to 1e-4 of their
+result's norm (sums of up to 256 fp32 terms, 256 * 2^-24 = 1.5e-5, through three layers; the quintic's largest derivative to the
+fifth, 485 * 2^-24 = 2.9e-5, on rounded directions); three steps move a variable by no more than the sum of its updates, so it is
+compared within 3e-4 of how far it has moved, and 2^-22 of itself for the rounding of the stored values."""
+import numpy as np
+import pytest
+import torch
+
+import distributed_tensorflow_amd as tf
+
+V, D, CONTEXT, HIDDEN, BATCH = 211, 16, 4, 48, 37
+
+
+def build(optimizer):
+    ids = tf.placeholder(tf.int64, [None, CONTEXT], name="ids")
+    labels = tf.placeholder(tf.int64, [None], name="labels")
+    tf.set_random_seed(3)
+    init = {"table": ([V, D], 0.3), "W1": ([CONTEXT * D, HIDDEN], 1 / 8), "b1": ([HIDDEN], 0.1), "W2": ([HIDDEN, V], 1 / 7),
+            "b2": ([V], 0.1)}
+    var = {k: tf.Variable(tf.random_normal(shape, stddev=std), name=k) for k, (shape, std) in init.items()}
+    step = tf.get_variable("global_step", [], initializer=tf.constant_initializer(0), trainable=False)
+    x = tf.reshape(tf.nn.embedding_lookup(var["table"], ids, scale=2.0), [-1, CONTEXT * D])
+    h = tf.tanh(tf.add(tf.matmul(x, var["W1"]), var["b1"]))
+    logits = tf.add(tf.matmul(h, var["W2"]), var["b2"])
+    loss = tf.reduce_mean(tf.nn.sparse_softmax_cross_entropy_with_logits(labels=labels, logits=logits))
+    train = optimizer.minimize(loss, global_step=step)
+    return ids, labels, var, step, loss, train
+
+
+def batch(seed):
+    rng = np.random.RandomState(seed)
+    ids = (V ** rng.rand(BATCH, CONTEXT)).astype(np.int64) - 1
+    ids[0, 1], ids[5, 3] = -1, V                      # padding on either side
+    labels = rng.randint(0, V, BATCH)
+    labels[3] = -1
+    return ids, labels
+
+
+def written_out(p, ids, labels):
+    """Loss and gradients in 64 bits."""
+    leaf = {k: v.clone().requires_grad_(True) for k, v in p.items()}
+    inside = torch.tensor((ids >= 0) & (ids < V))
+    rows = 2.0 * leaf["table"][torch.tensor(ids).clamp(0, V - 1)] * inside[..., None]
+    h = torch.tanh(rows.reshape(BATCH, -1) @ leaf["W1"] + leaf["b1"])
+    logp = torch.log_softmax(h @ leaf["W2"] + leaf["b2"], 1)
+    lab = torch.tensor(labels)
+    loss = (-logp[torch.arange(BATCH), lab.clamp(min=0)] * (lab >= 0)).sum() / BATCH
+    return loss.detach(), dict(zip(leaf, torch.autograd.grad(loss, list(leaf.values()))))
+
+
+def factor(x):
+    flip = x.shape[0] > x.shape[1]
+    y = x.t() if flip else x
+    y = y / (y.norm() + 1e-7)
+    for _ in range(5):
+        p = y @ y.t()
+        y = 3.4445 * y + (-4.7750 * p + 2.0315 * p @ p) @ y
+    return y.t() if flip else y
+
+
+def run(kind, steps=3):
+    with tf.Graph().as_default():
+        opt = tf.train.MuonOptimizer(0.05, momentum=0.9, sgd_learning_rate=0.2) if kind == "muon" \
+            else tf.train.GradientDescentOptimizer(0.2)
+        ids, labels, var, step, loss, train = build(opt)
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            read = lambda: {k: sess.var_tensor(v).detach().cpu().double().clone() for k, v in var.items()}  # noqa: E731
+            p = read()
+            start = {k: v.clone() for k, v in p.items()}
+            buf = {k: torch.zeros_like(p[k]) for k in ("W1", "W2")}
+            moved = {k: 0.0 for k in p}
+            for s in range(steps):
+                i, lab = batch(s)
+                _, got_loss = sess.run([train, loss], feed_dict={ids: i, labels: lab})
+                want_loss, g = written_out(p, i, lab)
+                assert abs(got_loss - float(want_loss)) <= 1e-4 * abs(float(want_loss))
+                for k in p:
+                    if kind == "muon" and k in buf:
+                        buf[k] = 0.9 * buf[k] + g[k]
+                        d = 0.05 * max(1.0, p[k].shape[1] / p[k].shape[0]) ** 0.5 * factor(g[k] + 0.9 * buf[k])
+                    else:
+                        d = 0.2 * g[k]
+                    p[k] = p[k] - d
+                    moved[k] += float(d.norm())
+            got = read()
+            for k in p:
+                assert float((got[k] - p[k]).norm()) <= 3e-4 * moved[k] + 2.0 ** -22 * float(p[k].norm()), k
+            untouched = np.setdiff1d(np.arange(V), np.concatenate([batch(s)[0].ravel() for s in range(steps)]))
+            assert len(untouched) and torch.equal(got["table"][untouched], start["table"][untouched])
+            assert sess.run(step) == steps and sess.generic_steps == steps
+            if kind == "muon":
+                for k in buf:
+                    slot = next(v for v in tf.global_variables() if v.op_name == f"{k}/Muon")
+                    assert float((sess.var_tensor(slot).cpu().double() - buf[k]).norm()) <= 1e-4 * float(buf[k].norm())
+                assert not [v for v in tf.global_variables() if v.op_name in ("table/Muon", "b1/Muon")]
+
+
+@pytest.mark.parametrize("kind", ["sgd", "muon"])
+def test_token_model_on_the_cpu(kind):
+    with tf.device("/cpu:0"):
+        run(kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["sgd", "muon"])
+def test_token_model_on_the_gpu(kind):
+    run(kind)
+
+
+def _stack_with_muon(widths):
+    """MuonOptimizer on graphs that the engines recognise (two layers: models/mlp.py, more: models/dense.py): the engine's gradient
+    pass, then the matrices' own update."""
+    rng = np.random.RandomState(5)
+    n = len(widths) - 1
+    with tf.Graph().as_default():
+        x = tf.placeholder(tf.float32, [None, widths[0]])
+        y = tf.placeholder(tf.float32, [None, widths[-1]])
+        w = [tf.Variable(tf.random_normal([a, b], stddev=a ** -0.5), name=f"w{k}") for k, (a, b) in enumerate(zip(widths, widths[1:]))]
+        b = [tf.Variable(tf.zeros([m]), name=f"b{k}") for k, m in enumerate(widths[1:])]
+        h = x
+        for k in range(n):
+            h = tf.add(tf.matmul(h, w[k]), b[k])
+            h = tf.nn.relu(h) if k + 1 < n else h
+        loss = tf.reduce_mean(tf.nn.softmax_cross_entropy_with_logits(labels=y, logits=h))
+        step = tf.train.get_or_create_global_step()
+        train = tf.train.MuonOptimizer(0.1, use_nesterov=False, sgd_learning_rate=0.3).minimize(loss, global_step=step)
+        xs = rng.rand(16, widths[0]).astype(np.float32)
+        ys = np.eye(widths[-1], dtype=np.float32)[rng.randint(0, widths[-1], 16)]
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            vs = w + b
+            p = [sess.var_tensor(v).cpu().double().requires_grad_(True) for v in vs]
+            sess.run([train, loss], feed_dict={x: xs, y: ys})
+            out = torch.tensor(xs).double()
+            for k in range(n):
+                out = out @ p[k] + p[n + k]
+                out = torch.relu(out) if k + 1 < n else out
+            want = -(torch.tensor(ys).double() * torch.log_softmax(out, 1)).sum(1).mean()
+            g = torch.autograd.grad(want, p)
+            for k, v in enumerate(vs):
+                d = 0.1 * max(1.0, p[k].shape[1] / p[k].shape[0]) ** 0.5 * factor(g[k]) if k < n else 0.3 * g[k]
+                got = sess.var_tensor(v).cpu().double()
+                assert float((got - (p[k].detach() - d)).norm()) <= 1e-4 * float(d.norm()) + 2.0 ** -22 * float(got.norm()), v.op_name
+            assert sess.run(step) == 1.0 and sess.fused_steps == 1
+            return sess.dense_steps
+
+
+@pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
+def test_muon_on_a_dense_stack_on_the_cpu(widths):
+    with tf.device("/cpu:0"):
+        _stack_with_muon(widths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
+def test_muon_on_a_dense_stack_on_the_gpu(widths):
+    assert _stack_with_muon(widths) == len(widths) - 3
+
+
+def test_a_table_that_is_also_multiplied_takes_the_dense_gradient():
+    """Shared input and output embedding: the lookups' rows alone would miss the product's gradient."""
+    with tf.Graph().as_default(), tf.device("/cpu:0"):
+        ids = tf.placeholder(tf.int32, [None])
+        labels = tf.placeholder(tf.int32, [None])
+        table = tf.Variable(tf.random_normal([9, 4]), name="table")
+        logits = tf.matmul(tf.nn.embedding_lookup([table], ids), table, transpose_b=True)
+        loss = tf.reduce_mean(tf.nn.sparse_softmax_cross_entropy_with_logits(labels=labels, logits=logits))
+        train = tf.train.GradientDescentOptimizer(0.5).minimize(loss)
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            p = sess.var_tensor(table).double().requires_grad_(True)
+            i, lab = np.array([1, 1, 8, 0]), np.array([2, 3, 3, 0])
+            sess.run(train, feed_dict={ids: i, labels: lab})
+            want = torch.nn.functional.cross_entropy(p[torch.tensor(i)] @ p.t(), torch.tensor(lab))
+            (g,) = torch.autograd.grad(want, p)
+            assert float((sess.var_tensor(table).double() - (p.detach() - 0.5 * g)).abs().max()) < 1e-5
+
+
+def test_lookups_of_higher_rank_and_two_of_one_table():
+    with tf.Graph().as_default(), tf.device("/cpu:0"):
+        a, b = tf.placeholder(tf.int64, [2, 3]), tf.placeholder(tf.int64, [2, 3])
+        table = tf.Variable(tf.random_normal([7, 5]), name="table")
+        both = tf.multiply(tf.nn.embedding_lookup(table, a), tf.nn.embedding_lookup(table, b, scale=0.5))
+        labels = tf.placeholder(tf.int64, [2, 3])
+        loss = tf.reduce_sum(tf.nn.sparse_softmax_cross_entropy_with_logits(labels=labels, logits=both))
+        train = tf.train.GradientDescentOptimizer(0.1).minimize(loss)
+        assert both.shape == (2, 3, 5)
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            p = sess.var_tensor(table).double().requires_grad_(True)
+            i, j = np.array([[0, 1, 6], [2, 2, 0]]), np.array([[1, 1, 0], [3, 4, 5]])
+            lab = np.array([[0, 1, 2], [3, 4, -1]])
+            sess.run(train, feed_dict={a: i, b: j, labels: lab})
+            z = p[torch.tensor(i)] * 0.5 * p[torch.tensor(j)]
+            want = torch.nn.functional.cross_entropy(z.reshape(6, 5), torch.tensor(lab).reshape(6), ignore_index=-1, reduction="sum")
+            (g,) = torch.autograd.grad(want, p)
+            assert float((sess.var_tensor(table).double() - (p.detach() - 0.1 * g)).abs().max()) < 1e-5
+
+
+def test_refusals_of_the_graph():
+    with tf.Graph().as_default():
+        table = tf.Variable(tf.zeros([4, 3]))
+        ids = tf.placeholder(tf.int64, [None])
+        with pytest.raises(ValueError):
+            tf.nn.embedding_lookup([table, table], ids)
+        with pytest.raises(ValueError):
+            tf.nn.embedding_lookup(tf.Variable(tf.zeros([4])), ids)
+        with pytest.raises(ValueError):
+            tf.nn.embedding_lookup(table, tf.placeholder(tf.float32, [None]))
+        with pytest.raises(ValueError):
+            tf.nn.sparse_softmax_cross_entropy_with_logits(labels=tf.placeholder(tf.float32, [None]), logits=tf.matmul(table, table))
+        with pytest.raises(ValueError):
+            tf.train.MuonOptimizer(0.1, momentum=1.0)
+        with pytest.raises(ValueError):
+            tf.train.SyncReplicasOptimizer(tf.train.MuonOptimizer(0.1), replicas_to_aggregate=2)
+
+
+@pytest.mark.parametrize("kind", ["sgd", "muon"])
+def test_token_model_on_a_parameter_server(kind):
+    """One shard and one worker over TCP: the table's gradient travels like any other; MuonOptimizer is refused before a push."""
+    from cluster_utils import cluster_dict
+
+    cluster = tf.train.ClusterSpec(cluster_dict(1, 1))
+    cfg = tf.ConfigProto(allow_soft_placement=True, operation_timeout_in_ms=20000)
+    ps, worker = tf.train.Server(cluster, "ps", 0, config=cfg), tf.train.Server(cluster, "worker", 0, config=cfg)
+    try:
+        g = tf.Graph()
+        with g.as_default(), tf.device(tf.train.replica_device_setter(worker_device="/job:worker/task:0/cpu:0", cluster=cluster)):
+            opt = tf.train.MuonOptimizer(0.1) if kind == "muon" else tf.train.GradientDescentOptimizer(0.2)
+            ids, labels, var, step, loss, train = build(opt)
+            init = tf.global_variables_initializer()
+        sv = tf.train.Supervisor(graph=g, is_chief=True, global_step=step, init_op=init)
+        sess = sv.prepare_or_wait_for_session(worker.target)
+        p = {k: sess.var_tensor(v).detach().cpu().double().clone() for k, v in var.items()}
+        i, lab = batch(0)
+        if kind == "muon":
+            with pytest.raises(NotImplementedError):
+                sess.run(train, feed_dict={ids: i, labels: lab})
+            assert sess.run(step) == 0
+        else:
+            sess.run(train, feed_dict={ids: i, labels: lab})
+            _, grads = written_out(p, i, lab)
+            sess.run(loss, feed_dict={ids: i, labels: lab})              # (pulls)
+            for k, v in var.items():
+                d = 0.2 * grads[k]
+                got = sess.var_tensor(v).detach().cpu().double()
+                assert float((got - (p[k] - d)).norm()) <= 1e-4 * float(d.norm()) + 2.0 ** -22 * float(got.norm()), k
+            assert sess.run(step) == 1
+        sv.stop()
+        sess.close()
+    finally:
+        worker.stop()
+        ps.stop()
