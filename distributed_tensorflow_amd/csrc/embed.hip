@@ -7,13 +7,20 @@
 // An id outside [0, rows) is padding: a row of zeros, no gradient.  Storage fp32, bf16 or fp16; sums in fp32, rounded once.
 //
 // All three are bound by memory.  The gradient must not depend on the order in which atomics land, and a frequent token
-// must not serialise on its row, so the tokens are SORTED by id (stable, least significant digit first) and equal ids are
-// summed as runs of the sorted order, in ascending t:
+// must not serialise on its row.
+//
+// Up to 4096 tokens, where launches and trips to memory count: one launch, a block per token.  The block of an id's FIRST
+// occurrence finds the others by comparing (T^2 / 64 wave steps in all), each wave in a range of tokens of its own, and the
+// waves' sums meet in order; the other blocks end at once.  (Sorting these few tokens by one workgroup, summing and joining
+// took 22 us at 3001 tokens; this takes 10.)
+//
+// More tokens are SORTED by id (stable, least significant digit first) and equal ids are summed as runs of the sorted order, in
+// ascending t:
 //
 //   sort      digits of up to 10 bits (a vocabulary of 2^20 - 1 takes two), two launches per digit: counts of every block, then
-//             the scatter, each block of which adds up the counts in front of it by itself (at most 64 blocks, so that is at
-//             most 64 coalesced rows).  Ranks inside a wave come from ballots over the digit's bits.  Up to 4096 tokens:
-//             one workgroup, all digits in LDS, one launch.
+//             the scatter, each block of which adds up the counts in front of it by itself (at most 64 blocks).  Ranks inside a
+//             wave come from ballots over the digit's bits.  (One launch whose blocks each count all the items: 24 us a digit
+//             instead of 12 at 32768 tokens.)
 //   sums      a group of lanes owns a chunk of consecutive sorted positions and a slice of columns, walks the chunk with
 //             the loads of four positions in flight, and stores each run that lies inside the chunk.  The pieces of a run
 //             that crosses chunks go to an fp32 workspace row of their chunk.  Further blocks of the same launch look up
@@ -27,12 +34,10 @@
 
 #include <type_traits>
 
-#ifndef AHEAD
-#define AHEAD 4
-#endif
 namespace {
 
-constexpr int kSmall = 4096;        // tokens sorted by one workgroup
+constexpr int kSmall = 4096;        // tokens compared with each other instead of sorted
+constexpr int kSmallWaves = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kWaves = kSortThreads / 64;
 constexpr int kMaxDigit = 10;       // bits
@@ -63,6 +68,15 @@ __device__ __forceinline__ void put(T* at, const Pack<T, N>& p, bool past) {
     }
   }
   *reinterpret_cast<Pack<T, N>*>(at) = p;
+}
+
+// The other way: a pack that is read once.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> get(const T* at, bool past) {
+  if constexpr (sizeof(T) * N == 16) {
+    if (past) return __builtin_bit_cast(Pack<T, N>, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at)));
+  }
+  return *reinterpret_cast<const Pack<T, N>*>(at);
 }
 
 // --- lookup ------------------------------------------------------------------------------------------------------------
@@ -152,43 +166,6 @@ __device__ __forceinline__ uint32_t digit_prefix(uint32_t v, uint32_t* wave_sum)
   return before + inc - v;
 }
 
-// The whole sort in one workgroup, items and counters in LDS.
-__global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const void* __restrict__ ids, int wide, int tokens,
-                                                                  uint32_t rows, int key_bits, uint32_t* __restrict__ keys,
-                                                                  uint32_t* __restrict__ order) {
-  __shared__ uint2 item[2][kSmall];
-  __shared__ uint32_t wave_at[kWaves << kMaxDigit];
-  __shared__ uint32_t base[1 << kMaxDigit], wave_sum[kWaves];
-  for (int i = threadIdx.x; i < tokens; i += kSortThreads) item[0][i] = make_uint2(load_key(ids, wide, i, rows), (uint32_t)i);
-  const int passes = (key_bits + kMaxDigit - 1) / kMaxDigit, bits = (key_bits + passes - 1) / passes, digits = 1 << bits;
-  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
-  int cur = 0;
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * bits;
-    if (threadIdx.x < digits) base[threadIdx.x] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < tokens; i += kSortThreads) atomicAdd(&base[(item[cur][i].x >> shift) & (digits - 1)], 1u);
-    __syncthreads();
-    const uint32_t total = threadIdx.x < digits ? base[threadIdx.x] : 0;
-    const uint32_t at = digit_prefix(total, wave_sum);
-    if (threadIdx.x < digits) base[threadIdx.x] = at;
-    __syncthreads();
-    for (int i0 = 0; i0 < tokens; i0 += kSortThreads) {
-      const int i = i0 + threadIdx.x;
-      const bool valid = i < tokens;
-      const uint2 it = valid ? item[cur][i] : make_uint2(0, 0);
-      const uint32_t to = place((it.x >> shift) & (digits - 1), bits, valid, base, wave_at);
-      if (valid) item[cur ^ 1][to] = it;
-    }
-    __syncthreads();
-    cur ^= 1;
-  }
-  for (int i = threadIdx.x; i < tokens; i += kSortThreads) {
-    keys[i] = item[cur][i].x;
-    order[i] = item[cur][i].y;
-  }
-}
-
 struct SortPass {
   const void* ids;         // first pass: the ids themselves
   const uint2* in;         // later passes: {key, position}
@@ -228,7 +205,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass a, 
   __shared__ uint32_t wave_at[kWaves << kMaxDigit];
   __shared__ uint32_t base[1 << kMaxDigit], wave_sum[kWaves];
   const int digits = 1 << a.bits;
-  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
+  const int64_t first = (int64_t)blockIdx.x * a.tile, last = min(first + a.tile, a.tokens);
   uint32_t total = 0, before = 0;
   if (threadIdx.x < digits) {
     for (int b0 = 0; b0 < blocks; b0 += 32) {
@@ -242,10 +219,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(SortPass a, 
       }
     }
   }
+  for (int i = threadIdx.x; i < kWaves * digits; i += kSortThreads) wave_at[i] = 0;
   const uint32_t at = digit_prefix(total, wave_sum);
   if (threadIdx.x < digits) base[threadIdx.x] = at + before;
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * a.tile, last = min(first + a.tile, a.tokens);
   for (int64_t i0 = first; i0 < last; i0 += kSortThreads) {
     const int64_t i = i0 + threadIdx.x;
     const bool valid = i < last;
@@ -277,7 +254,7 @@ struct SumArgs {
   float* pieces;             // [chunks][2][piece_ld]: the run that began before the chunk, the run that goes on behind it
   int64_t piece_ld;
   int64_t sum_blocks;        // blocks past these write the zeros of rows that do not occur
-  bool past;                 // the gradient is larger than the caches
+  bool past, g_past;         // the gradient (the upstream gradient) is larger than the caches: 131072 x 4096 860 -> 811 us
   int join_chunks;           // chunks whose crossing runs one block joins (at most 64: one lane looks at each)
 };
 
@@ -335,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
   Pack<float, N>* piece = reinterpret_cast<Pack<float, N>*>(a.pieces + chunk * 2 * a.piece_ld + (int64_t)pack * N);
   Pack<float, N> sum;
-  constexpr int kAhead = AHEAD;
+  constexpr int kAhead = 4;        // (8: 889 us instead of 862 at 131072 x 4096)
   for (int64_t i0 = first; i0 < last && run < a.rows; i0 += kAhead) {
     uint32_t key[kAhead];
     Pack<T, N> v[kAhead];
@@ -343,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(SumArgs a, const T* __res
     for (int j = 0; j < kAhead; ++j) key[j] = i0 + j < last ? a.keys[i0 + j] : a.rows;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (key[j] < a.rows) v[j] = *reinterpret_cast<const Pack<T, N>*>(column + (int64_t)a.order[i0 + j] * a.ldg);
+      if (key[j] < a.rows) v[j] = get<T, N>(column + (int64_t)a.order[i0 + j] * a.ldg, a.g_past);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j >= last) break;
@@ -456,6 +433,90 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(SumArgs a, T* __r
   }
 }
 
+// --- few tokens ----------------------------------------------------------------------------------------------------------
+// Block (t, s): slice s of the columns of the row ids[t], if t is its first occurrence.
+constexpr int kSmallLoops = 4;      // packs of a lane
+template <typename T, int N, bool UPDATE>
+__global__ __launch_bounds__(kSmallWaves * 64) void few_kernel(SumArgs a, const void* __restrict__ ids, int wide,
+                                                               const T* __restrict__ g, T* __restrict__ table) {
+  __shared__ int earlier, others;
+  __shared__ uint16_t list[kSmallWaves][kSmall / kSmallWaves];
+  __shared__ float part[kSmallWaves][64 * N];
+  const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tokens = (int)a.tokens;
+  const int64_t id = load_id(ids, wide, t);
+  if (id < 0 || id >= (int64_t)a.rows) return;
+  if (threadIdx.x == 0) earlier = others = 0;
+  __syncthreads();
+  for (int j0 = 0; j0 < t; j0 += kSmallWaves * 64) {
+    const int j = j0 + threadIdx.x;
+    if (__ballot(j < t && load_id(ids, wide, min(j, t)) == id)) {
+      if (lane == 0) earlier = 1;
+      break;
+    }
+  }
+  // this wave's range of the tokens from t on, and where the id occurs in it
+  const int range = (tokens - t + kSmallWaves - 1) / kSmallWaves, from = t + wave * range, to = min(from + range, tokens);
+  int count = 0;
+  for (int j0 = from; j0 < to; j0 += 64) {
+    const int j = j0 + lane;
+    const bool hit = j < to && load_id(ids, wide, min(j, tokens - 1)) == id;
+    const uint64_t mask = __ballot(hit);
+    if (hit) list[wave][count + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)j;
+    count += __popcll(mask);
+  }
+  if (wave > 0 && count > 0 && lane == 0) others = 1;
+  __syncthreads();
+  if (earlier) return;
+  const bool alone = !others;              // the first wave has all of them
+  if (alone && wave > 0) return;
+  const float f = UPDATE ? a.lr[0] * a.scale : a.scale;
+#pragma unroll 1
+  for (int k = 0; k < kSmallLoops; ++k) {
+    const int pack = (blockIdx.y * kSmallLoops + k) * 64 + lane;
+    if ((blockIdx.y * kSmallLoops + k) * 64 >= a.packs) break;
+    const T* column = g + (int64_t)min(pack, a.packs - 1) * N;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    for (int p = 0; p < count; p += 8) {
+      Pack<T, N> v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const Pack<T, N>*>(column + (int64_t)list[wave][min(p + q, count - 1)] * a.ldg);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (p + q < count) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] += (float)v[q].v[e];
+        }
+    }
+    if (!alone) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) part[wave][e * 64 + lane] = acc[e];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < kSmallWaves; ++w)
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] += part[w][e * 64 + lane];
+      }
+      __syncthreads();
+    }
+    if (wave == 0 && pack < a.packs) store_row<T, N, UPDATE>(a, table, (uint32_t)id, pack, acc, f);
+  }
+}
+
+// Zeros in front of few_kernel.
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void zero_rows_kernel(T* __restrict__ table, int64_t rows, int packs, int64_t ldt, int lanes_log2,
+                                                             bool past) {
+  const int groups = kThreads >> lanes_log2, lane = threadIdx.x & ((1 << lanes_log2) - 1);
+  Pack<T, N> zero;
+#pragma unroll
+  for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
+  for (int64_t r = (int64_t)blockIdx.x * groups + (threadIdx.x >> lanes_log2); r < rows; r += (int64_t)gridDim.x * groups)
+    for (int c = lane; c < packs; c += 1 << lanes_log2) put(table + r * ldt + (int64_t)c * N, zero, past);
+}
+
 inline int log2_lanes(int packs) {
   int l = 0;
   while ((1 << l) < packs && (1 << l) < kThreads) ++l;
@@ -482,25 +543,21 @@ Workspace plan(int64_t tokens, int dim) {
   w.chunk = chunk_of(tokens, (dim + 3) / 4);
   w.chunks = (tokens + w.chunk - 1) / w.chunk;
   w.piece_ld = (dim + 7) / 8 * 8;
-  const int64_t big = tokens > kSmall ? 1 : 0;
+  const int64_t big = tokens > kSmall ? 1 : 0;         // (fewer tokens need no workspace)
   w.keys = 0;
-  w.order = up(w.keys + 4 * tokens);
-  w.pairs = up(w.order + 4 * tokens);
+  w.order = up(w.keys + big * 4 * tokens);
+  w.pairs = up(w.order + big * 4 * tokens);
   w.counts = up(w.pairs + big * 16 * tokens);
   w.pieces = up(w.counts + big * 4 * kMaxSortBlocks * (1 << kMaxDigit));
-  w.total = up(w.pieces + w.chunks * 2 * w.piece_ld * 4) + 256;
+  w.total = up(w.pieces + big * w.chunks * 2 * w.piece_ld * 4) + 256;
   return w;
 }
 
-int sort_tokens(const void* ids, int wide, int64_t tokens, uint32_t rows, const Workspace& w, char* ws, hipStream_t s) {
+void sort_tokens(const void* ids, int wide, int64_t tokens, uint32_t rows, const Workspace& w, char* ws, hipStream_t s) {
   uint32_t* keys = reinterpret_cast<uint32_t*>(ws + w.keys);
   uint32_t* order = reinterpret_cast<uint32_t*>(ws + w.order);
   int key_bits = 1;
   while ((1ull << key_bits) <= (uint64_t)rows) ++key_bits;       // keys 0 .. rows
-  if (tokens <= kSmall) {
-    sort_small_kernel<<<1, kSortThreads, 0, s>>>(ids, wide, (int)tokens, rows, key_bits, keys, order);
-    return 0;
-  }
   uint2* pairs[2] = {reinterpret_cast<uint2*>(ws + w.pairs), reinterpret_cast<uint2*>(ws + w.pairs) + tokens};
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + w.counts);
   int64_t tile = (tokens + kMaxSortBlocks - 1) / kMaxSortBlocks;
@@ -513,13 +570,22 @@ int sort_tokens(const void* ids, int wide, int64_t tokens, uint32_t rows, const 
     sort_count_kernel<<<blocks, kSortThreads, 0, s>>>(a, counts);
     sort_scatter_kernel<<<blocks, kSortThreads, 0, s>>>(a, counts, blocks, p + 1 < passes ? pairs[p & 1] : nullptr, keys, order);
   }
-  return 0;
 }
 
 template <typename T, int N, bool UPDATE>
-void launch_sums(SumArgs a, const T* g, T* table, int64_t fill_rows, hipStream_t s) {
+void launch_sums(SumArgs a, const void* ids, int wide, const T* g, T* table, int64_t fill_rows, hipStream_t s) {
   a.packs = a.dim / N;
   a.lanes_log2 = log2_lanes(a.packs);
+  if (a.tokens <= kSmall) {
+    if (!UPDATE) {
+      const int64_t blocks = (fill_rows + (kThreads >> a.lanes_log2) - 1) / (kThreads >> a.lanes_log2);
+      zero_rows_kernel<T, N><<<(unsigned)(blocks > 16384 ? 16384 : blocks), kThreads, 0, s>>>(table, fill_rows, a.packs, a.ldt, a.lanes_log2, a.past);
+    }
+    if (a.tokens > 0)
+      few_kernel<T, N, UPDATE><<<dim3((unsigned)a.tokens, (a.packs + 64 * kSmallLoops - 1) / (64 * kSmallLoops)), kSmallWaves * 64, 0, s>>>(
+          a, ids, wide, g, table);
+    return;
+  }
   const int lanes = 1 << a.lanes_log2, groups = kThreads / lanes;
   a.sum_blocks = (a.chunks + groups - 1) / groups;
   const int64_t fill = (fill_rows + kFillRows - 1) / kFillRows;
@@ -539,7 +605,7 @@ int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const v
                  int64_t rows, int dim, float scale, const float* lr, void* workspace, hipStream_t s) {
   const Workspace w = plan(tokens, dim);
   char* ws = static_cast<char*>(workspace);
-  if (tokens > 0) sort_tokens(ids, wide, tokens, (uint32_t)rows, w, ws, s);
+  if (tokens > kSmall) sort_tokens(ids, wide, tokens, (uint32_t)rows, w, ws, s);
   SumArgs a{};
   a.keys = reinterpret_cast<uint32_t*>(ws + w.keys);
   a.order = reinterpret_cast<uint32_t*>(ws + w.order);
@@ -555,6 +621,7 @@ int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const v
   a.pieces = reinterpret_cast<float*>(ws + w.pieces);
   a.piece_ld = w.piece_ld;
   a.past = rows * dim * (int64_t)sizeof(T) > kCaches;
+  a.g_past = tokens * dim * (int64_t)sizeof(T) > kCaches;
   const T* gp = static_cast<const T*>(g);
   T* tp = static_cast<T*>(table);
   const int bytes = dtf_access_bytes((uint64_t)g | (uint64_t)table | (uint64_t)(ldg * sizeof(T)) | (uint64_t)(ldt * sizeof(T)) |
@@ -562,7 +629,7 @@ int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const v
   const int64_t fill = update ? 0 : rows;
   auto go = [&](auto n) {
     constexpr int N = decltype(n)::value;
-    if (update) launch_sums<T, N, true>(a, gp, tp, fill, s); else launch_sums<T, N, false>(a, gp, tp, fill, s);
+    if (update) launch_sums<T, N, true>(a, ids, wide, gp, tp, fill, s); else launch_sums<T, N, false>(a, ids, wide, gp, tp, fill, s);
   };
   if (bytes == 16) go(std::integral_constant<int, 16 / sizeof(T)>());
   else if (bytes == 8) go(std::integral_constant<int, 8 / sizeof(T)>());
