@@ -307,24 +307,42 @@ constexpr int kTurnWords = 2 * 32 * kTurnRow;     // two turning areas of a wave
 // Order of a wave's own LDS accesses (nobody else touches its areas).
 __device__ __forceinline__ void own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The linear term's lines (of A, or of X through its transpose).
+// What a stage reads and writes beside its sums, taken from the arguments once (inside the loops every use would be a trip to
+// memory again).
+struct Ends {
+  const char* linear;         // of the linear term: A, or X through its transpose
+  char *straight, *turned;    // the result, and its transpose
+  int straight_cols, mp;
+};
+template <int STAGE>
+__device__ __forceinline__ Ends ends_of(const Item& it, int parity) {
+  Ends e;
+  e.linear = STAGE == kPoly ? it.A : it.XT[parity];
+  e.straight = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.X;
+  e.turned = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.XT[parity ^ 1];
+  e.mp = it.mp;
+  e.straight_cols = STAGE <= kPoly ? it.mp : it.np;
+  return e;
+}
+
 struct Linear {
   u32x4 chunk[4];
-  __device__ __forceinline__ void read(const Item& it, int stage, int parity, int i0, int j0, int lane) {
-    const char* s = (stage == kPoly ? it.A : it.XT[parity]) + plane_at(j0 + (lane >> 3), i0, it.mp) + 16 * (lane & 7);
+  __device__ __forceinline__ void read(const Ends& ends, int i0, int j0, int lane) {
+    const char* s = ends.linear + plane_at(j0 + (lane >> 3), i0, ends.mp) + 16 * (lane & 7);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * it.mp * 4);
+    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * ends.mp * 4);
   }
 };
 
 // What becomes of the tile.  `area`: the wave's turning areas.  `mirror`: also store the transposed tile of a symmetric result.
-__device__ __forceinline__ void store_tile(const Call& c, const Item& it, int stage, int parity, int i0, int j0, bool mirror,
+template <int STAGE>
+__device__ __forceinline__ void store_tile(const Call& c, const Item& it, const Ends& ends, int i0, int j0, bool mirror,
                                            const f32x16& sum, const Linear& linear, uint32_t* area, int lane) {
   const int half = lane >> 5, jc = lane & 31;
   uint32_t* turn = area;
   uint32_t* lines = area + 32 * kTurnRow;
   float v[16];
-  if (stage == kGram) {
+  if (STAGE == kGram) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = sum[e] * (kScaleA / (kScaleX * kScaleX));
   } else {
@@ -332,9 +350,9 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int st
     for (int n = 0; n < 4; ++n)
       *reinterpret_cast<u32x4*>(lines + ((lane >> 3) + 8 * n) * kTurnRow + 4 * (lane & 7)) = linear.chunk[n];
     own_lds();
-    const float lin = stage == kPoly ? kB * (kScaleB / kScaleA) : stage == kStep ? kA : kA / kScaleX;
-    const float quad = stage == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
-                       : stage == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
+    const float lin = STAGE == kPoly ? kB * (kScaleB / kScaleA) : STAGE == kStep ? kA : kA / kScaleX;
+    const float quad = STAGE == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
+                       : STAGE == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
     const char* line = reinterpret_cast<const char*>(lines + jc * kTurnRow) + 8 * half;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -344,32 +362,32 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int st
         v[4 * g + x] = fmaf((float)hi[x], lin, fmaf((float)lo[x], lin, quad * sum[4 * g + x]));
     }
   }
-  if (stage == kLast) {
+  if (STAGE == kLast) {
+    // (places past the matrix are read as its last ones and not stored)
     const int64_t step_row = it.flip ? 1 : it.ldo, step_col = it.flip ? it.ldo : 1;
-    const int64_t at0 = (i0 + 4 * half) * step_row + (j0 + jc) * step_col;
-    auto inside = [&](int e) { return i0 + 8 * (e / 4) + 4 * half + e % 4 < it.m && j0 + jc < it.n; };
-    if (it.buf) {
-      const float step_size = c.lr[0] * it.shape_factor;
-      float* w = static_cast<float*>(it.out) + at0;
-      float old[16];                      // (all of them requested before the first store)
+    const int row0 = i0 + 4 * half, col = j0 + jc;
+    const int64_t at_col = min(col, it.n - 1) * step_col;
+    auto place = [&](int e) { return min(row0 + 8 * (e / 4) + e % 4, it.m - 1) * step_row + at_col; };
+    auto inside = [&](int e) { return row0 + 8 * (e / 4) + e % 4 < it.m && col < it.n; };
+    if (it.buf || c.dtype == DTF_F32) {
+      float* out = static_cast<float*>(it.out);
+      if (it.buf) {                       // the weights: all of them requested before the first store
+        const float step_size = c.lr[0] * it.shape_factor;
+        float old[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) old[e] = inside(e) ? w[(8 * (e / 4) + e % 4) * step_row] : 0.f;
+        for (int e = 0; e < 16; ++e) old[e] = out[place(e)];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = old[e] - step_size * v[e];
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (inside(e)) w[(8 * (e / 4) + e % 4) * step_row] = old[e] - step_size * v[e];
-      return;
-    }
+        if (inside(e)) out[place(e)] = v[e];
+    } else {
+      uint16_t* out = static_cast<uint16_t*>(it.out);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if (inside(e)) {
-        const int64_t at = at0 + (8 * (e / 4) + e % 4) * step_row;
-        if (c.dtype == DTF_F32) {
-          static_cast<float*>(it.out)[at] = v[e];
-        } else if (c.dtype == DTF_BF16) {
-          static_cast<bf16_t*>(it.out)[at] = (bf16_t)v[e];
-        } else {
-          static_cast<f16_t*>(it.out)[at] = (f16_t)v[e];
-        }
+      for (int e = 0; e < 16; ++e) {
+        const uint16_t bits = c.dtype == DTF_BF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v[e]) : __builtin_bit_cast(uint16_t, (f16_t)v[e]);
+        if (inside(e)) out[place(e)] = bits;
       }
     }
     return;
@@ -406,13 +424,13 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int st
   own_lds();
   const int l8 = lane >> 3, chunk = lane & 7;
   if (mirror) {
-    char* to = (stage == kGram ? it.A : stage == kPoly ? it.B : it.XT[parity ^ 1]) + plane_at(j0 + l8, i0, it.mp) + 16 * chunk;
+    char* to = ends.turned + plane_at(j0 + l8, i0, ends.mp) + 16 * chunk;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * it.mp * 4) = *reinterpret_cast<const u32x4*>(lines + (l8 + 8 * n) * kTurnRow + 4 * chunk);
+      *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * ends.mp * 4) = *reinterpret_cast<const u32x4*>(lines + (l8 + 8 * n) * kTurnRow + 4 * chunk);
   }
-  const int cols = stage <= kPoly ? it.mp : it.np;
-  char* to = (stage == kGram ? it.A : stage == kPoly ? it.B : it.X) + plane_at(i0 + l8, j0, cols) + 16 * chunk;
+  const int cols = ends.straight_cols;
+  char* to = ends.straight + plane_at(i0 + l8, j0, cols) + 16 * chunk;
 #pragma unroll
   for (int n = 0; n < 4; ++n)
     *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * cols * 4) = *reinterpret_cast<const u32x4*>(turn + (l8 + 8 * n) * kTurnRow + 4 * chunk);
@@ -420,8 +438,9 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, int st
 }
 
 // Tile `t` of a stage: rows and columns in tiles.  Symmetric results: t = tj (tj + 1) / 2 + ti, ti <= tj.
-__device__ __forceinline__ void tile_place(const Item& it, int stage, int edge, int t, int& ti, int& tj) {
-  if (stage <= kPoly) {
+template <int STAGE>
+__device__ __forceinline__ void tile_place(const Item& it, int edge, int t, int& ti, int& tj) {
+  if (STAGE <= kPoly) {
     tj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (tj * (tj + 1) / 2 > t) --tj;
     while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
@@ -528,8 +547,8 @@ struct Product {
   }
 };
 
-template <int TILE>
-__global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles tl, int stage, int parity) {
+template <int TILE, int STAGE>
+__global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles tl, int parity) {
   constexpr int MI = Product<TILE>::MI, NI = Product<TILE>::NI;
   Product<TILE> g;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -542,20 +561,22 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
   const int tiles = (tl.first[which + 1] - tl.first[which]) / tl.splits;
   const int local = id - tl.first[which], part = local / tiles, tile = local - part * tiles;
   int ti, tj;
-  tile_place(it, stage, TILE, tile, ti, tj);
-  const int depth = stage == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
+  tile_place<STAGE>(it, TILE, tile, ti, tj);
+  const int depth = STAGE == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
   const int64_t row_bytes = (int64_t)depth * 4;
-  g.p.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
-  g.q.init(stage == kGram ? it.X : stage == kPoly ? it.A : it.XT[parity], tj * TILE, stage <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
+  g.p.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
+  g.q.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity], tj * TILE, STAGE <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
   g.wave = wave, g.lane = lane;
   const int row_p = g.row_p = (wave >> 1) * (TILE / 2), row_q = g.row_q = (wave & 1) * (TILE / 2);
   const int pairs = depth / 64;
   const int k_first = 2 * (int)((int64_t)pairs * part / tl.splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / tl.splits);
 
-  const int columns = stage <= kPoly ? it.mp : it.np;
+  const int columns = STAGE <= kPoly ? it.mp : it.np, rows = it.mp;
+  const Ends ends = ends_of<STAGE>(it, parity);
+  // 32 x 32 tiles past the matrix are neither read nor stored (dimensions are whole multiples of 64: a wave has none, or full rows)
+  auto there = [&](int i, int j) { return ti * TILE + row_p + 32 * i < rows && tj * TILE + row_q + 32 * j < columns; };
   Linear early{};                         // (of the smallest tile: under way during the product)
-  if (MI * NI == 1 && stage != kGram && tl.splits == 1 && ti * TILE + row_p < it.mp && tj * TILE + row_q < columns)
-    early.read(it, stage, parity, ti * TILE + row_p, tj * TILE + row_q, lane);
+  if (MI * NI == 1 && STAGE != kGram && tl.splits == 1 && there(0, 0)) early.read(ends, ti * TILE + row_p, tj * TILE + row_q, lane);
   constexpr int kSums = Product<TILE>::kSums;
   typename Product<TILE>::Sums sums;
   f32x16 (&acc)[MI][NI] = sums[0];
@@ -586,41 +607,56 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
               f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
     return;
   }
-  // Nobody reads the images any more: image 0 becomes the waves' turning tiles, and a row of a wave's tiles at a time goes through
-  // image 1, so that the code of store_tile() is there MI times and not MI * NI times (with all of it unrolled the accumulators
-  // of the largest tile ended up in scratch memory).
+  // Nobody reads the images any more: image 0 becomes the waves' turning areas.  The linear terms of a row of tiles are under way
+  // while the row before is stored; straight-line code, so that waiting for them does not mean waiting for the stores behind them
+  // (a loop over the tiles took 1.7 us for each: its head waited for everything).
   uint32_t* turn = reinterpret_cast<uint32_t*>(image<TILE, 0>()) + wave * kTurnWords;
+  constexpr int kRows = TILE == 256 ? 1 : 2;          // (the largest tile has no registers left for a second row)
   f32x4* line = reinterpret_cast<f32x4*>(image<TILE, 1>() + wave * (2 * TILE * 128 / kWaves)) + lane;
+  Linear linear[kRows][NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    linear[0][j] = early;
+    if (MI * NI > 1 && STAGE != kGram && there(0, j)) linear[0][j].read(ends, ti * TILE + row_p, tj * TILE + row_q + 32 * j, lane);
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q;
-    if (i0 >= it.mp || j0 >= columns) break;
-    Linear next = early;
-    if (MI * NI > 1 && stage != kGram) next.read(it, stage, parity, i0, j0, lane);
+    if (kRows == 1) {         // (its sums go through image 1, a row of tiles at a time: straight from the accumulators they spilled)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) line[(j * 4 + e / 4) * 64] = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+      own_lds();
+    }
 #pragma unroll
     for (int j = 0; j < NI; ++j)
+      if (kRows == 2 && i + 1 < MI && STAGE != kGram && there(i + 1, j))
+        linear[(i + 1) % kRows][j].read(ends, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) line[(j * 4 + e / 4) * 64] = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-    own_lds();
-#pragma clang loop unroll(disable)
-    for (int j = 0; j < NI && j0 + 32 * j < columns; ++j) {
-      const Linear linear = next;
-      if (stage != kGram && j + 1 < NI && j0 + 32 * (j + 1) < columns) next.read(it, stage, parity, i0, j0 + 32 * (j + 1), lane);
+    for (int j = 0; j < NI; ++j) {
       f32x16 sum;
+      if (kRows == 1) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = line[(j * 4 + g) * 64];
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 v = line[(j * 4 + g) * 64];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sum[4 * g + x] = v[x];
+          for (int x = 0; x < 4; ++x) sum[4 * g + x] = v[x];
+        }
+      } else {
+        sum = acc[i][j];
       }
-      store_tile(c, it, stage, parity, i0, j0 + 32 * j, stage > kPoly || ti != tj, sum, linear, turn, lane);
+      if (there(i, j))
+        store_tile<STAGE>(c, it, ends, ti * TILE + row_p + 32 * i, tj * TILE + row_q + 32 * j, STAGE > kPoly || ti != tj, sum,
+                          linear[i % kRows][j], turn, lane);
+      if (kRows == 1 && i + 1 < MI && STAGE != kGram && there(i + 1, j))
+        linear[0][j].read(ends, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
     }
-    own_lds();
   }
 }
 
 // Split products: the sums of a 32 x 32 tile's parts in order, one wave each.  `edge`: of the product's tiles.
-__global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge, int stage, int parity) {
+template <int STAGE>
+__global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge, int parity) {
   __shared__ __attribute__((aligned(16))) uint32_t turns[4][kTurnWords];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x * 4 + wave;
@@ -631,13 +667,14 @@ __global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge,
   const int local = id - tl.first[which], tile = local / per_tile, sub = local - tile * per_tile;
   const int of_wave = sub / per_wave, ij = sub - of_wave * per_wave;
   int ti, tj;
-  tile_place(it, stage, edge, tile, ti, tj);
+  tile_place<STAGE>(it, edge, tile, ti, tj);
   const int i0 = ti * edge + (of_wave >> 1) * (edge / 2) + 32 * (ij / side), j0 = tj * edge + (of_wave & 1) * (edge / 2) + 32 * (ij % side);
-  if (i0 >= it.mp || j0 >= (stage <= kPoly ? it.mp : it.np)) return;
+  if (i0 >= it.mp || j0 >= (STAGE <= kPoly ? it.mp : it.np)) return;
   const int64_t elems = (int64_t)edge * edge;
   const float* from = c.partial + (tl.tile0[which] + tile) * tl.splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
+  const Ends ends = ends_of<STAGE>(it, parity);
   Linear linear{};
-  if (stage != kGram) linear.read(it, stage, parity, i0, j0, lane);
+  if (STAGE != kGram) linear.read(ends, i0, j0, lane);
   f32x16 sum;
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
@@ -652,7 +689,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge,
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[e] += s0 + k < tl.splits ? v[k][e / 4][e % 4] : 0.f;
   }
-  store_tile(c, it, stage, parity, i0, j0, stage > kPoly || ti != tj, sum, linear, turns[wave], lane);
+  store_tile<STAGE>(c, it, ends, i0, j0, STAGE > kPoly || ti != tj, sum, linear, turns[wave], lane);
 }
 
 // --- host ---------------------------------------------------------------------------------------------------------------
@@ -790,6 +827,17 @@ Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, cha
   return l;
 }
 
+template <int STAGE>
+void launch_stage(const Call& c, const StagePlan& p, int parity, hipStream_t s) {
+  switch (p.cut.edge) {
+    case 64: product_kernel<64, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
+    case 128: product_kernel<128, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
+    case 192: product_kernel<192, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
+    default: product_kernel<256, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity);
+  }
+  if (p.cut.splits > 1) finish_kernel<STAGE><<<(p.finish_waves + 3) / 4, 256, 0, s>>>(c, p.finish, p.cut.edge, parity);
+}
+
 template <typename T>
 int run(Call& c, const Layout& l, hipStream_t s) {
   norm_kernel<T><<<dim3(c.norm_blocks, c.count), 256, 0, s>>>(c);
@@ -799,18 +847,12 @@ int run(Call& c, const Layout& l, hipStream_t s) {
     most = t > most ? t : most;
   }
   split_kernel<T><<<dim3((unsigned)most, c.count), 256, 0, s>>>(c);
-  for (int k = 0; k < 5; ++k)
-    for (int stage = kGram; stage <= kStep; ++stage) {
-      const int what = stage == kStep && k == 4 ? kLast : stage;
-      const StagePlan& p = l.stage[stage];
-      switch (p.cut.edge) {
-        case 64: product_kernel<64><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
-        case 128: product_kernel<128><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
-        case 192: product_kernel<192><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1); break;
-        default: product_kernel<256><<<p.blocks, 256, 0, s>>>(c, p.product, what, k & 1);
-      }
-      if (p.cut.splits > 1) finish_kernel<<<(p.finish_waves + 3) / 4, 256, 0, s>>>(c, p.finish, p.cut.edge, what, k & 1);
-    }
+  for (int k = 0; k < 5; ++k) {
+    launch_stage<kGram>(c, l.stage[kGram], k & 1, s);
+    launch_stage<kPoly>(c, l.stage[kPoly], k & 1, s);
+    if (k < 4) launch_stage<kStep>(c, l.stage[kStep], k & 1, s);
+    else launch_stage<kLast>(c, l.stage[kStep], k & 1, s);
+  }
   return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
 }
 
