@@ -479,8 +479,13 @@ struct Product {
   static constexpr int kLoads = 2 * Fetcher<TILE>::kLoads;       // of a wave and step
   static constexpr int kReads = 2 * (MI + NI), kMfmas = 3 * MI * NI, kSums = MI * NI == 1 ? 3 : 1;
   typedef f32x16 Sums[kSums][MI][NI];
+  // Small tiles have registers for all fragments of two steps: the reads of step k are covered by the whole of step k - 1, and the
+  // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417: there it is the loads' way
+  // from memory, 2700 cycles that a ring of 128 KB has to cover, that sets the pace).
+  static constexpr bool kWhole = TILE <= 128;
   Fetcher<TILE> p, q;
-  Half<MI, NI> first, second;
+  Half<MI, NI> first, second;               // halves of a step, in turn
+  Half<MI, NI> whole[2][2];                 // kWhole: [step parity][half]
   int wave, lane, row_p, row_q;
 
   template <int I>
@@ -500,6 +505,15 @@ struct Product {
   __device__ __forceinline__ void step(Sums& acc, int k, int last) {
     wait_and_barrier<(kRing - 2) * kLoads>();          // step k has landed, every wave is done with step k - 1
     load<(I + kRing - 1) % kRing>(min(k + kRing - 1, last));
+    if constexpr (kWhole) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) whole[I & 1][h].read(image<TILE, I>(), image<TILE, I>() + TILE * 128, row_p, row_q, lane, h);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) whole[~I & 1][h].template multiply<kSums>(acc);      // step k - 1
+      interleave<0, 2 * kReads, 2 * kMfmas, kLoads>();
+      __builtin_amdgcn_sched_barrier(0);
+      return;
+    }
     first.read(image<TILE, I>(), image<TILE, I>() + TILE * 128, row_p, row_q, lane, 0);
     second.template multiply<kSums>(acc);                              // the second half of step k - 1
     interleave<0, kReads, kMfmas, kLoads>();
@@ -514,7 +528,7 @@ struct Product {
   template <int I>
   __device__ __forceinline__ bool turn(Sums& acc, int k, int last) {
     step<I % kRing>(acc, k + I, last);
-    if (k + I == last) return false;
+    if (I % 2 == 1 && k + I == last) return false;      // (ranges are whole pairs of steps)
     if constexpr (I + 1 < kSteps) return turn<I + 1>(acc, k, last);
     return true;
   }
@@ -526,11 +540,12 @@ struct Product {
 #pragma unroll
       for (int j = 0; j < NI; ++j) second.b[j][h] = half8{};
     }
+    whole[1][0] = whole[1][1] = second;
     preload<0>(first_step, last);
     int k = first_step;
-    if constexpr (kRing == 2) {                        // (ranges are whole pairs of steps: one way out, which the accumulators
+    if constexpr (kRing == 2) {                        // (one way out, which the accumulators of the largest tile need to stay
 #pragma clang loop unroll(disable)
-      for (; k < last; k += 2) {                       //  of the largest tile need to stay where they are)
+      for (; k < last; k += 2) {                       //  where they are)
         step<0>(acc, k, last);
         step<1>(acc, k + 1, last);
       }
@@ -542,7 +557,12 @@ struct Product {
         while (turn<0>(acc, k, last)) k += kSteps;
       }
     }
-    second.template multiply<kSums>(acc);
+    if constexpr (kWhole) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) whole[1][h].template multiply<kSums>(acc);
+    } else {
+      second.template multiply<kSums>(acc);
+    }
     wait_and_barrier<0>();                             // nothing is on its way to the images any more, and nobody reads them
   }
 };
