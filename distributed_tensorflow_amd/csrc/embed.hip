@@ -11,8 +11,8 @@
 //
 // Up to 4096 tokens, where launches and trips to memory count: one launch, a block per token.  The block of an id's FIRST
 // occurrence finds the others by comparing (T^2 / 64 wave steps in all), each wave in a range of tokens of its own, and the
-// waves' sums meet in order; the other blocks end at once.  (Sorting these few tokens by one workgroup, summing and joining
-// took 22 us at 3001 tokens; this takes 10.)
+// waves' sums meet in order; the other blocks end at once.  (3001 tokens x 101, the whole pass: sorting by one workgroup, summing and
+// joining took 23.6 us, this takes 13.3.)
 //
 // More tokens are SORTED by id (stable, least significant digit first) and equal ids are summed as runs of the sorted order, in
 // ascending t:
@@ -26,7 +26,7 @@
 //             that crosses chunks go to an fp32 workspace row of their chunk.  Further blocks of the same launch look up
 //             (binary search in the sorted ids) which rows of the table do not occur and store their zeros, so no row of
 //             the gradient is written twice.
-//   joins     a wave per run that crosses chunks and slice of columns adds its pieces in order; all sixteen waves of a block
+//   joins     a wave per run that crosses chunks and slice of columns adds its pieces in order; all eight waves of a block
 //             share a run of more than 32 pieces (a frequent token).  The chunk borders depend on the sizes alone: the result
 //             is the same bits every time.
 #include "dtf_api.h"
@@ -45,7 +45,7 @@ constexpr int kMaxSortBlocks = 64;
 constexpr int kThreads = 256;
 constexpr int64_t kCaches = (int64_t)256 << 20;     // bytes: a result of more does not stay in the last cache anyway
 constexpr int kFillRows = 32;       // rows of the table per zero-filling block
-constexpr int kJoinWaves = 16;
+constexpr int kJoinWaves = 8;       // (32768 tokens x 256: 16 waves 12.0 us, 8 waves 8.0, 4 waves 9.7)
 constexpr int kLongRun = 32;        // pieces
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t t) {
@@ -371,7 +371,7 @@ __device__ __forceinline__ int64_t run_of_chunks(const SumArgs& a, int64_t c0, u
 
 // Runs that cross chunks: the chunk a run begins in names it; its pieces are that chunk's second workspace row and the
 // first rows of the chunks behind it.
-template <typename T, bool UPDATE>
+template <typename T, int N, bool UPDATE>
 __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(SumArgs a, T* __restrict__ table) {
   __shared__ f32x4 part[kJoinWaves][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -404,6 +404,15 @@ __global__ __launch_bounds__(kJoinWaves * 64) void join_kernel(SumArgs a, T* __r
   };
   auto store = [&](uint32_t run, f32x4 sum) {
     T* row = table + (int64_t)run * a.ldt + col;
+    if (N >= 4) {                            // whole, aligned quads
+      if (col >= a.dim) return;
+      Pack<T, 4> q;
+      if (UPDATE) q = *reinterpret_cast<const Pack<T, 4>*>(row);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q.v[e] = UPDATE ? (T)((float)q.v[e] - f * sum[e]) : (T)(f * sum[e]);
+      *reinterpret_cast<Pack<T, 4>*>(row) = q;
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (col + e < a.dim) row[e] = UPDATE ? (T)((float)row[e] - f * sum[e]) : (T)(f * sum[e]);
@@ -593,10 +602,10 @@ void launch_sums(SumArgs a, const void* ids, int wide, const T* g, T* table, int
   if (grid.x) sum_kernel<T, N, UPDATE><<<grid, kThreads, 0, s>>>(a, g, table);
   if (a.chunks > 1) {
     // few enough chunks per block that a thousand blocks share the runs: they are a chain of trips to memory each, and the
-    // frequent tokens' runs lie side by side (32768 tokens x 256: 64 chunks a block 23 us, 4 chunks 8 us)
+    // frequent tokens' runs lie side by side (32768 tokens x 256: 64 chunks a block 23 us, 4 to 16 chunks 8 us)
     const int64_t slices = (a.dim + 255) / 256, per = a.chunks * slices / 1024;
     a.join_chunks = per < 4 ? 4 : per > 64 ? 64 : (int)per;
-    join_kernel<T, UPDATE><<<dim3((unsigned)((a.chunks + a.join_chunks - 1) / a.join_chunks), (unsigned)slices), kJoinWaves * 64, 0, s>>>(a, table);
+    join_kernel<T, N, UPDATE><<<dim3((unsigned)((a.chunks + a.join_chunks - 1) / a.join_chunks), (unsigned)slices), kJoinWaves * 64, 0, s>>>(a, table);
   }
 }
 

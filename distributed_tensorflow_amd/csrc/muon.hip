@@ -141,16 +141,21 @@ __device__ __forceinline__ uint32_t split_pair(float scaled) {       // hi | lo 
 __device__ __forceinline__ int64_t plane_at(int64_t row, int col, int cols) {
   return row * cols * 4 + (col >> 5) * 128 + (col & 31) * 2;
 }
-// 32 pairs, `step` words apart in LDS, to the hi (part 0) or lo (part 1) half of a 128-byte group.
-__device__ __forceinline__ void store_group(char* group, const uint32_t* pairs, int step, int part) {
-  const int shift = part * 16;
+// A 64 x 64 tile of pairs in LDS, its rows `line` and its columns `step` words apart, to row0, col0 of a plane pair: 256 bytes a
+// row, sixteen bytes a thread and turn, consecutive threads one behind the other (64 bytes a thread: the kernel took 23 us
+// for 1024 x 4096 instead of 17).
+__device__ __forceinline__ void store_tile(char* plane, int row0, int col0, int cols, const uint32_t* pairs, int line, int step) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t w[4];
+  for (int k = 0; k < 4; ++k) {
+    const int row = k * 16 + (threadIdx.x >> 4), chunk = threadIdx.x & 15;      // chunk: group of 32 columns, hi or lo, 8 columns
+    const int col = (chunk >> 3) * 32 + (chunk & 3) * 8, shift = (chunk >> 2 & 1) * 16;
+    u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = ((pairs[(8 * q + 2 * e) * step] >> shift) & 0xffffu) | ((pairs[(8 * q + 2 * e + 1) * step] >> shift) << 16);
-    *reinterpret_cast<uint4*>(group + part * 64 + q * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t* at = pairs + row * line + (col + 2 * e) * step;
+      w[e] = (at[0] >> shift & 0xffffu) | (at[step] >> shift) << 16;
+    }
+    *reinterpret_cast<u32x4*>(plane + plane_at(row0 + row, col0, cols) + chunk * 16) = w;
   }
 }
 
@@ -197,9 +202,8 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
   __syncthreads();
   char* straight = it.flip ? it.XT[0] : it.X;          // [pr][pc]
   char* turned = it.flip ? it.X : it.XT[0];            // [pc][pr]
-  const int line = threadIdx.x >> 2, group = (threadIdx.x >> 1) & 1, part = threadIdx.x & 1;
-  store_group(straight + plane_at(r0 + line, c0 + 32 * group, pc), &tile[line][32 * group], 1, part);
-  store_group(turned + plane_at(c0 + line, r0 + 32 * group, pr), &tile[32 * group][line], 65, part);
+  store_tile(straight, r0, c0, pc, &tile[0][0], 65, 1);
+  store_tile(turned, c0, r0, pr, &tile[0][0], 1, 65);
 }
 
 // --- products -----------------------------------------------------------------------------------------------------------
@@ -480,8 +484,8 @@ struct Product {
   static constexpr int kReads = 2 * (MI + NI), kMfmas = 3 * MI * NI, kSums = MI * NI == 1 ? 3 : 1;
   typedef f32x16 Sums[kSums][MI][NI];
   // Small tiles have registers for all fragments of two steps: the reads of step k are covered by the whole of step k - 1, and the
-  // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417: there it is the loads' way
-  // from memory, 2700 cycles that a ring of 128 KB has to cover, that sets the pace).
+  // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417, 2.4 times its MFMAs: its 16 KB
+  // of loads a step set the pace there, 39 bytes a cycle and CU).
   static constexpr bool kWhole = TILE <= 128;
   Fetcher<TILE> p, q;
   Half<MI, NI> first, second;               // halves of a step, in turn

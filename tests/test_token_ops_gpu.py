@@ -53,7 +53,7 @@ def exact_sums(ids, g, rows):
     return total[:rows], size[:rows], torch.bincount(at, minlength=rows + 1)[:rows]
 
 
-# tokens around a chunk, the one-workgroup sort and its limit, a block of the multi-block sort, and more than one of its tiles
+# tokens around a chunk, the largest number that is compared in pairs, a block of the multi-block sort, and more than one of its tiles
 TOKENS = [0, 1, 2, 31, 64, 65, 1000, 4095, 4096, 4097, 9001, 140001]
 DIMS = [1, 3, 8, 101, 256, 257, 1030]
 
