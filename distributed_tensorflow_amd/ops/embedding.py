@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import hip_backend as hb
 
@@ -121,6 +122,7 @@ class _Lookup(torch.autograd.Function):
         return lookup(table.detach(), ids, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
         return lookup_grad(ids, g, ctx.rows, ctx.scale), None, None

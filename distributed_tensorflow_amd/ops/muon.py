@@ -29,7 +29,8 @@ def _workspace(lib, shapes, device) -> torch.Tensor:
 
 
 def orthogonalize(x: torch.Tensor, eps: float = EPS, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The Newton-Schulz factor of a matrix, in its type; the zero matrix for a zero matrix.  ``out`` may be ``x`` itself."""
+    """The Newton-Schulz factor of a matrix, in its type; the zero matrix for a zero matrix.  ``out`` may be ``x`` itself.  A matrix
+    whose norm is so far below ``eps`` that ``x / eps`` has entries under 2^-40 gives zeros there."""
     lib = hb.require()
     ldx = hb.typed_rows(x, "x")
     if out is None:
@@ -45,7 +46,8 @@ def orthogonalize(x: torch.Tensor, eps: float = EPS, out: Optional[torch.Tensor]
 
 class MuonPlan:
     """A fixed list of float32 matrices ``[in, out]`` with their gradients and momentum buffers, and the workspace their steps use.
-    One step of a plan at a time: two streams, or two captured graphs that may overlap, need a plan each."""
+    The steps read and write the memory that the tensors have when the plan is made (and keep it alive): write new gradients
+    into the same tensors.  One step of a plan at a time: two streams, or two captured graphs that may overlap, need a plan each."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]):
         params, grads, momenta = list(params), list(grads), list(momenta)
@@ -62,7 +64,7 @@ class MuonPlan:
             if any(hb.overlap(a, b) for b in written[i + 1:] + grads):
                 raise hb.HipKernelError("MuonPlan: weights and momentum buffers must not overlap each other or the gradients")
         lib = hb.require()
-        self.params, self.grads, self.momenta = params, grads, momenta
+        self.params, self.grads, self.momenta = ([t.detach() for t in ts] for ts in (params, grads, momenta))
         self.device = params[0].device
         self._groups = []
         for i in range(0, len(params), GROUP):

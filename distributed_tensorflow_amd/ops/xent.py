@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import hip_backend as hb
 
@@ -62,6 +63,7 @@ class _SparseXent(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         logits, flat, stats = ctx.saved_tensors
         z = logits.detach()

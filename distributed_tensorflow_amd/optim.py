@@ -120,6 +120,8 @@ class MuonOptimizer(Optimizer):
             if len(v.shape) == 2 and v not in tables:
                 # (one momentum per variable, also where two train ops update it)
                 slot = next((s for s in v.graph.variables if s.op_name == f"{v.op_name}/Muon"), None)
+                if slot is not None and (slot.trainable or tuple(slot.shape) != tuple(v.shape)):
+                    raise ValueError(f"MuonOptimizer: {slot.op_name} is taken by a variable that is not the momentum of {v.op_name}")
                 slots[v] = slot if slot is not None else G.Variable(trainable=False, name=f"{v.op_name}/Muon", _init_spec=("zeros",),
                                                                     _shape=v.shape, _scoped=False)
         op.attrs["slots"] = slots

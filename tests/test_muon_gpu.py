@@ -205,3 +205,37 @@ def test_refusals():
         with pytest.raises(hb.HipKernelError):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+def test_a_plan_keeps_the_memory_it_was_made_on():
+    w, g, b = torch.zeros(70, 40, device="cuda"), gradient(70, 40, seed=1), torch.zeros(70, 40, device="cuda")
+    plan = muon.MuonPlan([w], [g], [b])
+    want = -0.5 * muon.orthogonalize(g)
+    w.data, g.data, b.data = (torch.ones(70, 40, device="cuda") for _ in range(3))
+    muon.muon_step(plan, torch.full((1,), 0.5, device="cuda"), momentum=0.0)
+    assert bool((w == 1).all()) and bool((g == 1).all()) and bool((b == 1).all())
+    # (the same iteration on the same matrix; the update rounds once more, the halving does not)
+    assert float((plan.params[0] - want).norm()) <= 2.0 ** -23 * float(want.norm())
+
+
+def test_plans_on_two_streams_at_once():
+    made = []
+    for k in range(2):
+        g = gradient(300, 500, seed=20 + k)
+        made.append(([torch.zeros(300, 500, device="cuda")], [g], [torch.zeros(300, 500, device="cuda")]))
+    lr = torch.full((1,), 0.25, device="cuda")
+    want = []
+    for ws, gs, bs in made:
+        plan = muon.MuonPlan([w.clone() for w in ws], gs, [b.clone() for b in bs])
+        for _ in range(5):
+            muon.muon_step(plan, lr)
+        want.append(plan.params[0])
+    plans = [muon.MuonPlan(*m) for m in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for plan, s in zip(plans, streams):
+            with torch.cuda.stream(s):
+                muon.muon_step(plan, lr)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p.params[0], x) for p, x in zip(plans, want))

@@ -220,6 +220,41 @@ def test_refusals_of_the_graph():
             tf.train.SyncReplicasOptimizer(tf.train.MuonOptimizer(0.1), replicas_to_aggregate=2)
 
 
+def test_the_momentum_is_saved_with_the_model(tmp_path):
+    with tf.Graph().as_default():
+        ids, labels, var, step, loss, train = build(tf.train.MuonOptimizer(0.05))
+        saver = tf.train.Saver()
+        feeds = [dict(zip((ids, labels), batch(s))) for s in range(3)]
+
+        def state(sess):
+            return {v.op_name: sess.var_tensor(v).clone() for v in tf.global_variables()}
+
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(train, feed_dict=feeds[0])
+            path = saver.save(sess, str(tmp_path / "model"))
+            for f in feeds[1:]:
+                sess.run(train, feed_dict=f)
+            want = state(sess)
+        with tf.Session() as sess:
+            saver.restore(sess, path)
+            for f in feeds[1:]:
+                sess.run(train, feed_dict=f)
+            got = state(sess)
+        assert float(want["W1/Muon"].abs().max()) > 0
+        assert set(got) == set(want) and all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_a_variable_in_the_place_of_a_momentum_is_refused():
+    with tf.Graph().as_default():
+        x, y = tf.placeholder(tf.float32, [None, 4]), tf.placeholder(tf.float32, [None, 3])
+        w = tf.Variable(tf.zeros([4, 3]), name="w")
+        tf.Variable(tf.zeros([4, 3]), name="w/Muon")
+        loss = tf.reduce_mean(tf.nn.softmax_cross_entropy_with_logits(labels=y, logits=tf.matmul(x, w)))
+        with pytest.raises(ValueError):
+            tf.train.MuonOptimizer(0.1).minimize(loss)
+
+
 @pytest.mark.parametrize("kind", ["sgd", "muon"])
 def test_token_model_on_a_parameter_server(kind):
     """One shard and one worker over TCP: the table's gradient travels like any other; MuonOptimizer is refused before a push."""

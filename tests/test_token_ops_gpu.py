@@ -375,3 +375,59 @@ def test_refusals_of_gpu_operands():
         with pytest.raises(hb.HipKernelError):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+def test_forward_and_backward_in_a_replayed_graph():
+    """Fresh leaves inside the capture, so that no eager graph of them lives next to it.  (The rows of the table are the logits.)"""
+    rows, classes, tokens = 700, 333, 4500
+    table = torch.randn(rows, classes, device="cuda", generator=gen(70))
+    ids = make_ids(tokens, rows, 71)
+    labels = torch.randint(-1, classes, (tokens,), device="cuda", generator=gen(73))
+
+    def step():
+        leaf = table.detach().requires_grad_(True)
+        losses = xent.sparse_softmax_xent(embedding.embedding_lookup(leaf, ids, 2.0), labels)
+        return (losses.detach(), *torch.autograd.grad(losses, leaf, torch.full_like(losses, 0.25)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for k in range(3):
+        ids.copy_(make_ids(tokens, rows, 80 + k))
+        labels.copy_(torch.randint(-1, classes, (tokens,), device="cuda", generator=gen(90 + k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_calls_on_two_streams_at_once():
+    """Workspaces belong to a call: two row updates and gradients side by side do what they do one after the other."""
+    rows, dim, tokens = 2000, 128, 20000
+    args = [(make_ids(tokens, rows, 100 + k), torch.randn(tokens, dim, device="cuda", generator=gen(110 + k))) for k in range(2)]
+    want = [embedding.lookup_grad(i, g, rows) for i, g in args]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(embedding.lookup_grad(*args[k], rows))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(x, want[k]) for x in got[k])
+
+
+def test_no_second_derivatives():
+    """The backward passes are launches, not graphs: a second derivative is refused, not silently left out."""
+    table = torch.randn(5, 4, device="cuda", generator=gen(120)).requires_grad_(True)
+    ids = torch.tensor([0, 1, 1], device="cuda")
+    for losses in (embedding.embedding_lookup(table, ids).square().sum(1), xent.sparse_softmax_xent(table[:3] * 2, ids)):
+        (g,) = torch.autograd.grad(losses.sum(), table, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), table)
