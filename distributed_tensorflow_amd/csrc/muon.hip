@@ -218,26 +218,26 @@ struct Tiles {
 // At most `LEFT` of this wave's loads are still under way and its LDS reads are done, then the workgroup's.  (A barrier alone does
 // not wait for loads that go to LDS, and __syncthreads() would wait for all of them.  The empty statements keep the compiler's
 // own memory accesses on their side.)
-template <int LEFT>
+template <int LEFT, bool BARRIER = true>
 __device__ __forceinline__ void wait_and_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4) << 14 | 7 << 4);     // vmcnt LEFT, lgkmcnt 0, expcnt untouched
-  __builtin_amdgcn_s_barrier();
+  if (BARRIER) __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
 // ROWS rows of a plane pair from a tile's first row on; rows past the last one are read as the last one (their products are not
 // stored).
-template <int ROWS>
+template <int ROWS, int WAVES>
 struct Fetcher {
-  static constexpr int kLoads = ROWS / (8 * kWaves);
+  static constexpr int kLoads = ROWS / (8 * WAVES);
   const char* base;
   unsigned at[kLoads];
   __device__ __forceinline__ void init(const char* plane, int row0, int rows, int64_t row_bytes, int wave, int lane) {
     base = plane + row0 * row_bytes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+      const int r = (i * WAVES + wave) * 8 + (lane >> 3);
       at[i] = (unsigned)(min(r, rows - 1 - row0) * row_bytes) + (unsigned)(((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
   }
@@ -247,7 +247,7 @@ struct Fetcher {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)0xffffffffu, 0x00020000);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + (i * kWaves + wave) * 1024), 16, at[i], k * 128, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(lds + (i * WAVES + wave) * 1024), 16, at[i], k * 128, 0, 0);
 #endif
   }
 };
@@ -480,14 +480,14 @@ __device__ __forceinline__ char* image() {
 template <int TILE>
 struct Product {
   static constexpr int kRing = ring_of(TILE), MI = TILE / 64, NI = TILE / 64;
-  static constexpr int kLoads = 2 * Fetcher<TILE>::kLoads;       // of a wave and step
+  static constexpr int kLoads = 2 * Fetcher<TILE, kWaves>::kLoads;       // of a wave and step
   static constexpr int kReads = 2 * (MI + NI), kMfmas = 3 * MI * NI, kSums = MI * NI == 1 ? 3 : 1;
   typedef f32x16 Sums[kSums][MI][NI];
   // Small tiles have registers for all fragments of two steps: the reads of step k are covered by the whole of step k - 1, and the
   // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417, 2.4 times its MFMAs: its 16 KB
   // of loads a step set the pace there, 39 bytes a cycle and CU).
   static constexpr bool kWhole = TILE <= 128;
-  Fetcher<TILE> p, q;
+  Fetcher<TILE, kWaves> p, q;
   Half<MI, NI> first, second;               // halves of a step, in turn
   Half<MI, NI> whole[2][2];                 // kWhole: [step parity][half]
   int wave, lane, row_p, row_q;
@@ -571,19 +571,119 @@ struct Product {
   }
 };
 
+// Where a product workgroup works: matrix, part of k, tile.  Workgroups go round the eight XCDs; numbered so that those of one XCD
+// follow each other, and with the tiles of one range of k next to each other, the workgroups that share an L2 read the same rows.
+struct Place {
+  int which, part, tile;
+};
+__device__ __forceinline__ Place place_of(const Tiles& tl) {
+  const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
+  const int id = xcd * per + min(xcd, extra) + (int)(blockIdx.x >> 3);
+  Place at;
+  at.which = owner(tl, id);
+  const int tiles = (tl.first[at.which + 1] - tl.first[at.which]) / tl.splits, local = id - tl.first[at.which];
+  at.part = local / tiles, at.tile = local - at.part * tiles;
+  return at;
+}
+
+// Tiles of 32, for launches that leave most CUs without a larger one: their time is the way from memory, so the four waves share
+// the tile's steps, each with a ring of its own (sixteen steps under way instead of eight) and nothing to wait for but its own loads.
+struct Narrow {
+  static constexpr int kRing = 4;
+  Fetcher<32, 1> p, q;
+  int wave, lane;
+  static constexpr int kLoads = 2 * Fetcher<32, 1>::kLoads;
+  template <int I>
+  __device__ __forceinline__ char* mine() const { return image<128, I>() + wave * 8192; }
+  template <int I>
+  __device__ __forceinline__ void load(int k) const {
+    p.go(mine<I>(), 0, k);
+    q.go(mine<I>() + 4096, 0, k);
+  }
+  template <int I>
+  __device__ __forceinline__ void preload(int k, int last) const {
+    if constexpr (I < kRing - 1) {
+      load<I>(min(k + I * kWaves, last));
+      preload<I + 1>(k, last);
+    }
+  }
+  // Steps k, k + kWaves, ... up to `last`, a round of the ring; whether the range goes on behind them.
+  template <int I>
+  __device__ __forceinline__ bool turn(f32x16 (&acc)[3][1][1], int k, int last) const {
+    wait_and_barrier<(kRing - 2) * kLoads, false>();        // this step has landed, the fragments of the one before are in registers
+    load<(I + kRing - 1) % kRing>(min(k + (I + kRing - 1) * kWaves, last));
+    Half<1, 1> half[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) half[h].read(mine<I>(), mine<I>() + 4096, 0, 0, lane, h);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) half[h].template multiply<3>(acc);
+    if (k + (I + 1) * kWaves > last) return false;
+    if constexpr (I + 1 < kRing) return turn<I + 1>(acc, k, last);
+    return true;
+  }
+  __device__ __forceinline__ void run(f32x16 (&acc)[3][1][1], int k, int last) const {
+    preload<0>(k, last);
+    if (turn<0>(acc, k, last)) {
+      k += kRing * kWaves;
+#pragma clang loop unroll(disable)
+      while (turn<0>(acc, k, last)) k += kRing * kWaves;
+    }
+  }
+};
+
+template <int STAGE>
+__global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Call c, Tiles tl, int parity) {
+  Narrow g;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Place at = place_of(tl);
+  const Item& it = c.item[at.which];
+  int ti, tj;
+  tile_place<STAGE>(it, 32, at.tile, ti, tj);
+  const int depth = STAGE == kGram ? it.np : it.mp;
+  const int64_t row_bytes = (int64_t)depth * 4;
+  g.p.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B, ti * 32, it.mp, row_bytes, 0, lane);
+  g.q.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity], tj * 32, STAGE <= kPoly ? it.mp : it.np, row_bytes, 0, lane);
+  g.wave = wave, g.lane = lane;
+  const Ends ends = ends_of<STAGE>(it, parity);
+  Linear linear{};
+  if (STAGE != kGram && wave == 0) linear.read(ends, ti * 32, tj * 32, lane);
+  f32x16 sums[3][1][1];
+#pragma unroll
+  for (int t = 0; t < 3; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[t][0][0][e] = 0.f;
+  if (wave < depth / 32) g.run(sums, wave, depth / 32 - 1);
+  f32x16& sum = sums[0][0][0];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] += sums[1][0][0][e] + sums[2][0][0][e];
+  wait_and_barrier<0>();                  // nothing is on its way to the images any more, and nobody reads them
+  f32x4* line = reinterpret_cast<f32x4*>(image<128, 1>()) + lane;
+  if (wave > 0) {
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      line[(wave * 4 + g4) * 64] = f32x4{sum[4 * g4], sum[4 * g4 + 1], sum[4 * g4 + 2], sum[4 * g4 + 3]};
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const f32x4 v = line[(w * 4 + g4) * 64];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum[4 * g4 + x] += v[x];
+    }
+  store_tile<STAGE>(c, it, ends, ti * 32, tj * 32, STAGE > kPoly || ti != tj, sum, linear, reinterpret_cast<uint32_t*>(image<128, 0>()), lane);
+}
+
 template <int TILE, int STAGE>
 __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles tl, int parity) {
   constexpr int MI = Product<TILE>::MI, NI = Product<TILE>::NI;
   Product<TILE> g;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups go round the eight XCDs; numbered so that those of one XCD follow each other, and with the tiles of one range of k
-  // next to each other, the workgroups that share an L2 read the same rows.
-  const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
-  const int id = xcd * per + min(xcd, extra) + (int)(blockIdx.x >> 3);
-  const int which = owner(tl, id);
+  const Place at = place_of(tl);
+  const int which = at.which, part = at.part, tile = at.tile;
   const Item& it = c.item[which];
-  const int tiles = (tl.first[which + 1] - tl.first[which]) / tl.splits;
-  const int local = id - tl.first[which], part = local / tiles, tile = local - part * tiles;
   int ti, tj;
   tile_place<STAGE>(it, TILE, tile, ti, tj);
   const int depth = STAGE == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
@@ -754,7 +854,7 @@ int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut
 // 128/1 359, 64/1 472); 1024 x 4096 x 1024 128/1 33 (256/1 72, 64/1 44); 1024^2 x 1024 symmetric 64/1 12 (128/4 19, 256/1 70).
 Cut choose(const Call& c, int stage) {
   static const struct { int edge; double step, loaded, rest; } kinds[] = {
-      {256, 1.34, 2.3, 18.0}, {192, 0.755, 1.3, 11.5}, {128, 0.39, 0.65, 6.0}, {64, 0.175, 0.24, 2.0}};
+      {256, 1.34, 2.3, 18.0}, {192, 0.755, 1.3, 11.5}, {128, 0.39, 0.65, 6.0}, {64, 0.175, 0.24, 2.0}, {32, 0.085, 0.12, 1.5}};
   Cut best{64, 1};
   double least = 1e300;
   int depth = 0;
@@ -768,7 +868,7 @@ Cut choose(const Call& c, int stage) {
     for (int i = 0; i < c.count; ++i) tiles += tiles_of(c, i, stage, kind.edge);
     for (int s = 1; s <= 16; ++s) {
       if (g_force_splits && s != g_force_splits && s != 1) continue;
-      if (s > 1 && depth / 64 < 2 * s) break;
+      if (s > 1 && (depth / 64 < 2 * s || kind.edge == 32)) break;
       const int64_t groups = tiles * s, full = groups / 256;
       const double steps = 2.0 * ((depth / 64 + s - 1) / s), share = (groups - full * 256) / 256.0;
       double us = 3.5 + full * (steps * kind.loaded + kind.rest);
@@ -854,6 +954,7 @@ Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, cha
 template <int STAGE>
 void launch_stage(const Call& c, const StagePlan& p, int parity, hipStream_t s) {
   switch (p.cut.edge) {
+    case 32: narrow_kernel<STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
     case 64: product_kernel<64, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
     case 128: product_kernel<128, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
     case 192: product_kernel<192, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
@@ -924,9 +1025,9 @@ extern "C" int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols
   return run<float>(c, l, (hipStream_t)stream);
 }
 
-// Tuning and tests: products of the next calls in tiles of this edge (64, 128, 192, 256) with this many parts of k where k is long
+// Tuning and tests: products of the next calls in tiles of this edge (32, 64, 128, 192, 256) with this many parts of k where k is long
 // enough; 0: chosen from the shapes.  (The workspace of a plan has to be made under the same setting.)
 extern "C" void dtf_debug_set_muon_cut(int edge, int splits) {
-  g_force_edge = edge == 64 || edge == 128 || edge == 192 || edge == 256 ? edge : 0;
+  g_force_edge = edge == 32 || edge == 64 || edge == 128 || edge == 192 || edge == 256 ? edge : 0;
   g_force_splits = splits > 0 && splits <= 16 ? splits : 0;
 }

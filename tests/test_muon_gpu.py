@@ -62,7 +62,7 @@ def test_factor_against_64_bits(shape, dtype):
         assert torch.equal(got, muon.orthogonalize(x))
 
 
-@pytest.mark.parametrize("edge", [64, 128, 192, 256])
+@pytest.mark.parametrize("edge", [32, 64, 128, 192, 256])
 @pytest.mark.parametrize("splits", [1, 2, 5])
 def test_every_cut_of_the_products(edge, splits):
     """Tile edges and parts of k that the shapes alone would not choose: tiles that stick out on either side, parts without a
