@@ -49,6 +49,7 @@ typedef f16_t half4 __attribute__((ext_vector_type(4)));
 typedef f16_t half2 __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -77,7 +78,6 @@ struct Call {
   int nesterov;
   int norm_blocks;
   const float* lr;
-  float* partial;       // split products: [tile][split][elements of a tile]
 };
 
 // --- momentum and norm ----------------------------------------------------------------------------------------------
@@ -176,6 +176,11 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
   float u[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) u[k] = (float)gp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.ldu];
+  float b[16];
+  if (it.buf) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) b[k] = bp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.cols];
+  }
   double total = 0;
 #pragma unroll
   for (int i = 0; i < kNormBlocks; i += 256) {
@@ -183,9 +188,6 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
     total += i + (int)threadIdx.x < c.norm_blocks ? part : 0.0;
   }
   if (it.buf) {
-    float b[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) b[k] = bp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.cols];
 #pragma unroll
     for (int k = 0; k < 16; ++k) u[k] = c.nesterov ? u[k] + c.mu * b[k] : b[k];
   }
@@ -209,11 +211,74 @@ __global__ __launch_bounds__(256) void split_kernel(Call c) {
 // --- products -----------------------------------------------------------------------------------------------------------
 enum Stage { kGram = 0, kPoly = 1, kStep = 2, kLast = 3 };     // A = X X^T;  B = bA + cAA;  X = aX + BX;  the same, to the output
 
-struct Tiles {
-  int first[kMax + 1];     // first workgroup (finish: first wave) of every matrix
-  int64_t tile0[kMax];     // first tile of the partial sums
-  int splits;              // workgroups per tile
+// What the launches of a stage read beside the planes themselves: 64 bytes a matrix, 512 for all of them, so that one load
+// instruction brings them into a wave's registers, whichever its matrix is (see find()).
+struct Job {
+  const char *p, *q;          // the operands: rows of k
+  const char* linear;         // of the linear term: A, or X through its transpose
+  char *straight, *turned;    // the result, and its transpose
+  int rows, cols, depth;      // of the product, padded
+  int first, tiles;           // first tile and number of tiles
+  int spare;
 };
+static_assert(sizeof(Job) == 64, "find() counts words");
+struct Jobs {
+  Job job[kMax];
+  float* partial;             // split products: [tile][split][elements of a tile]
+  int splits;                 // workgroups per tile, a range of k each
+};
+// Where the last product goes.
+struct Final {
+  void* out;
+  int64_t ld;
+  int m, n, flip;
+  float shape_factor;
+};
+struct Finals {
+  Final of[kMax];
+  const float* lr;            // null: the factor itself, in `dtype`
+  int dtype;
+};
+struct None {};
+template <int STAGE>
+struct EndOf {
+  typedef None Args;
+  struct Mine {};
+  static __device__ __forceinline__ Mine take(const Args&, int) { return Mine{}; }
+};
+template <>
+struct EndOf<kLast> {
+  typedef Finals Args;
+  struct Mine {
+    Final f;
+    const float* lr;
+    int dtype;
+  };
+  static __device__ __forceinline__ Mine take(const Args& a, int which) { return Mine{a.of[which], a.lr, a.dtype}; }
+};
+
+// The matrix that workgroup (or wave) `id` works for, with `per` of them to a tile.  Looked up field by field the arguments were
+// several trips to memory one behind the other: here every lane loads two words and the rest are reads of lanes (stack of three
+// matrices 130 -> 127 us).
+struct Task : Job {
+  int which;
+};
+__device__ __forceinline__ Task find(const Jobs& jobs, int id, int per, int lane) {
+  const uint2v mine = reinterpret_cast<const uint2v*>(&jobs)[lane];
+  auto word = [&](int i, int k) { return (uint32_t)__builtin_amdgcn_readlane(k & 1 ? mine[1] : mine[0], 8 * i + (k >> 1)); };
+  auto address = [&](int i, int k) {
+    return (char*)(__attribute__((address_space(1))) char*)((uint64_t)word(i, k + 1) << 32 | word(i, k));
+  };
+  Task t;
+  t.which = 0;
+#pragma unroll
+  for (int i = 1; i < kMax; ++i) t.which += id >= (int)word(i, 13) * per ? 1 : 0;
+  t.p = address(t.which, 0), t.q = address(t.which, 2), t.linear = address(t.which, 4);
+  t.straight = address(t.which, 6), t.turned = address(t.which, 8);
+  t.rows = (int)word(t.which, 10), t.cols = (int)word(t.which, 11), t.depth = (int)word(t.which, 12);
+  t.first = (int)word(t.which, 13), t.tiles = (int)word(t.which, 14);
+  return t;
+}
 
 // At most `LEFT` of this wave's loads are still under way and its LDS reads are done, then the workgroup's.  (A barrier alone does
 // not wait for loads that go to LDS, and __syncthreads() would wait for all of them.  The empty statements keep the compiler's
@@ -311,36 +376,18 @@ constexpr int kTurnWords = 2 * 32 * kTurnRow;     // two turning areas of a wave
 // Order of a wave's own LDS accesses (nobody else touches its areas).
 __device__ __forceinline__ void own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// What a stage reads and writes beside its sums, taken from the arguments once (inside the loops every use would be a trip to
-// memory again).
-struct Ends {
-  const char* linear;         // of the linear term: A, or X through its transpose
-  char *straight, *turned;    // the result, and its transpose
-  int straight_cols, mp;
-};
-template <int STAGE>
-__device__ __forceinline__ Ends ends_of(const Item& it, int parity) {
-  Ends e;
-  e.linear = STAGE == kPoly ? it.A : it.XT[parity];
-  e.straight = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.X;
-  e.turned = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.XT[parity ^ 1];
-  e.mp = it.mp;
-  e.straight_cols = STAGE <= kPoly ? it.mp : it.np;
-  return e;
-}
-
 struct Linear {
   u32x4 chunk[4];
-  __device__ __forceinline__ void read(const Ends& ends, int i0, int j0, int lane) {
-    const char* s = ends.linear + plane_at(j0 + (lane >> 3), i0, ends.mp) + 16 * (lane & 7);
+  __device__ __forceinline__ void read(const Task& t, int i0, int j0, int lane) {
+    const char* s = t.linear + plane_at(j0 + (lane >> 3), i0, t.rows) + 16 * (lane & 7);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * ends.mp * 4);
+    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * t.rows * 4);
   }
 };
 
 // What becomes of the tile.  `area`: the wave's turning areas.  `mirror`: also store the transposed tile of a symmetric result.
 template <int STAGE>
-__device__ __forceinline__ void store_tile(const Call& c, const Item& it, const Ends& ends, int i0, int j0, bool mirror,
+__device__ __forceinline__ void store_tile(const Task& t, const typename EndOf<STAGE>::Mine& end, int i0, int j0, bool mirror,
                                            const f32x16& sum, const Linear& linear, uint32_t* area, int lane) {
   const int half = lane >> 5, jc = lane & 31;
   uint32_t* turn = area;
@@ -366,17 +413,18 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, const 
         v[4 * g + x] = fmaf((float)hi[x], lin, fmaf((float)lo[x], lin, quad * sum[4 * g + x]));
     }
   }
-  if (STAGE == kLast) {
+  if constexpr (STAGE == kLast) {
+    const Final& it = end.f;
     // (places past the matrix are read as its last ones and not stored)
-    const int64_t step_row = it.flip ? 1 : it.ldo, step_col = it.flip ? it.ldo : 1;
+    const int64_t step_row = it.flip ? 1 : it.ld, step_col = it.flip ? it.ld : 1;
     const int row0 = i0 + 4 * half, col = j0 + jc;
     const int64_t at_col = min(col, it.n - 1) * step_col;
     auto place = [&](int e) { return min(row0 + 8 * (e / 4) + e % 4, it.m - 1) * step_row + at_col; };
     auto inside = [&](int e) { return row0 + 8 * (e / 4) + e % 4 < it.m && col < it.n; };
-    if (it.buf || c.dtype == DTF_F32) {
+    if (end.lr || end.dtype == DTF_F32) {
       float* out = static_cast<float*>(it.out);
-      if (it.buf) {                       // the weights: all of them requested before the first store
-        const float step_size = c.lr[0] * it.shape_factor;
+      if (end.lr) {                       // the weights: all of them requested before the first store
+        const float step_size = end.lr[0] * it.shape_factor;
         float old[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) old[e] = out[place(e)];
@@ -390,7 +438,7 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, const 
       uint16_t* out = static_cast<uint16_t*>(it.out);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint16_t bits = c.dtype == DTF_BF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v[e]) : __builtin_bit_cast(uint16_t, (f16_t)v[e]);
+        const uint16_t bits = end.dtype == DTF_BF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v[e]) : __builtin_bit_cast(uint16_t, (f16_t)v[e]);
         if (inside(e)) out[place(e)] = bits;
       }
     }
@@ -428,13 +476,13 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, const 
   own_lds();
   const int l8 = lane >> 3, chunk = lane & 7;
   if (mirror) {
-    char* to = ends.turned + plane_at(j0 + l8, i0, ends.mp) + 16 * chunk;
+    char* to = t.turned + plane_at(j0 + l8, i0, t.rows) + 16 * chunk;
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * ends.mp * 4) = *reinterpret_cast<const u32x4*>(lines + (l8 + 8 * n) * kTurnRow + 4 * chunk);
+      *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * t.rows * 4) = *reinterpret_cast<const u32x4*>(lines + (l8 + 8 * n) * kTurnRow + 4 * chunk);
   }
-  const int cols = ends.straight_cols;
-  char* to = ends.straight + plane_at(i0 + l8, j0, cols) + 16 * chunk;
+  const int cols = t.cols;
+  char* to = t.straight + plane_at(i0 + l8, j0, cols) + 16 * chunk;
 #pragma unroll
   for (int n = 0; n < 4; ++n)
     *reinterpret_cast<u32x4*>(to + (int64_t)n * 8 * cols * 4) = *reinterpret_cast<const u32x4*>(turn + (l8 + 8 * n) * kTurnRow + 4 * chunk);
@@ -443,7 +491,7 @@ __device__ __forceinline__ void store_tile(const Call& c, const Item& it, const 
 
 // Tile `t` of a stage: rows and columns in tiles.  Symmetric results: t = tj (tj + 1) / 2 + ti, ti <= tj.
 template <int STAGE>
-__device__ __forceinline__ void tile_place(const Item& it, int edge, int t, int& ti, int& tj) {
+__device__ __forceinline__ void tile_place(const Task& task, int edge, int t, int& ti, int& tj) {
   if (STAGE <= kPoly) {
     tj = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (tj * (tj + 1) / 2 > t) --tj;
@@ -451,19 +499,11 @@ __device__ __forceinline__ void tile_place(const Item& it, int edge, int t, int&
     ti = t - tj * (tj + 1) / 2;
   } else {
     // groups of eight tile rows, column by column inside: neighbours share rows of both operands
-    const int tiles_m = (it.mp + edge - 1) / edge, tiles_n = (it.np + edge - 1) / edge;
+    const int tiles_m = (task.rows + edge - 1) / edge, tiles_n = (task.cols + edge - 1) / edge;
     const int group = t / (8 * tiles_n), high = min(8, tiles_m - 8 * group), in = t - group * 8 * tiles_n;
     tj = in / high;
     ti = 8 * group + in - tj * high;
   }
-}
-
-// The matrix that workgroup (wave) `id` works for.  (Compared with all bounds at once: one by one each would be a trip to memory.)
-__device__ __forceinline__ int owner(const Tiles& tl, int id) {
-  int which = 0;
-#pragma unroll
-  for (int i = 1; i < kMax; ++i) which += id >= tl.first[i] ? 1 : 0;
-  return which;
 }
 
 constexpr int ring_of(int tile) { return tile == 256 ? 2 : tile == 192 ? 3 : tile == 128 ? 4 : 8; }
@@ -574,15 +614,16 @@ struct Product {
 // Where a product workgroup works: matrix, part of k, tile.  Workgroups go round the eight XCDs; numbered so that those of one XCD
 // follow each other, and with the tiles of one range of k next to each other, the workgroups that share an L2 read the same rows.
 struct Place {
-  int which, part, tile;
+  Task task;
+  int part, tile;
 };
-__device__ __forceinline__ Place place_of(const Tiles& tl) {
+__device__ __forceinline__ Place place_of(const Jobs& jobs, int lane) {
   const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
   const int id = xcd * per + min(xcd, extra) + (int)(blockIdx.x >> 3);
   Place at;
-  at.which = owner(tl, id);
-  const int tiles = (tl.first[at.which + 1] - tl.first[at.which]) / tl.splits, local = id - tl.first[at.which];
-  at.part = local / tiles, at.tile = local - at.part * tiles;
+  at.task = find(jobs, id, jobs.splits, lane);
+  const int local = id - at.task.first * jobs.splits;
+  at.part = local / at.task.tiles, at.tile = local - at.part * at.task.tiles;
   return at;
 }
 
@@ -632,27 +673,26 @@ struct Narrow {
 };
 
 template <int STAGE>
-__global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Call c, Tiles tl, int parity) {
+__global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Jobs jobs, typename EndOf<STAGE>::Args ends) {
   Narrow g;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(tl);
-  const Item& it = c.item[at.which];
+  const Place at = place_of(jobs, lane);
+  const Task& task = at.task;
+  const auto end = EndOf<STAGE>::take(ends, task.which);
   int ti, tj;
-  tile_place<STAGE>(it, 32, at.tile, ti, tj);
-  const int depth = STAGE == kGram ? it.np : it.mp;
-  const int64_t row_bytes = (int64_t)depth * 4;
-  g.p.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B, ti * 32, it.mp, row_bytes, 0, lane);
-  g.q.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity], tj * 32, STAGE <= kPoly ? it.mp : it.np, row_bytes, 0, lane);
+  tile_place<STAGE>(task, 32, at.tile, ti, tj);
+  const int64_t row_bytes = (int64_t)task.depth * 4;
+  g.p.init(task.p, ti * 32, task.rows, row_bytes, 0, lane);
+  g.q.init(task.q, tj * 32, task.cols, row_bytes, 0, lane);
   g.wave = wave, g.lane = lane;
-  const Ends ends = ends_of<STAGE>(it, parity);
   Linear linear{};
-  if (STAGE != kGram && wave == 0) linear.read(ends, ti * 32, tj * 32, lane);
+  if (STAGE != kGram && wave == 0) linear.read(task, ti * 32, tj * 32, lane);
   f32x16 sums[3][1][1];
 #pragma unroll
   for (int t = 0; t < 3; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) sums[t][0][0][e] = 0.f;
-  if (wave < depth / 32) g.run(sums, wave, depth / 32 - 1);
+  if (wave < task.depth / 32) g.run(sums, wave, task.depth / 32 - 1);
   f32x16& sum = sums[0][0][0];
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] += sums[1][0][0][e] + sums[2][0][0][e];
@@ -673,34 +713,31 @@ __global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Call c, Tiles tl
 #pragma unroll
       for (int x = 0; x < 4; ++x) sum[4 * g4 + x] += v[x];
     }
-  store_tile<STAGE>(c, it, ends, ti * 32, tj * 32, STAGE > kPoly || ti != tj, sum, linear, reinterpret_cast<uint32_t*>(image<128, 0>()), lane);
+  store_tile<STAGE>(task, end, ti * 32, tj * 32, STAGE > kPoly || ti != tj, sum, linear, reinterpret_cast<uint32_t*>(image<128, 0>()), lane);
 }
 
 template <int TILE, int STAGE>
-__global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles tl, int parity) {
+__global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, typename EndOf<STAGE>::Args all_ends) {
   constexpr int MI = Product<TILE>::MI, NI = Product<TILE>::NI;
   Product<TILE> g;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Place at = place_of(tl);
-  const int which = at.which, part = at.part, tile = at.tile;
-  const Item& it = c.item[which];
+  const Place at = place_of(jobs, lane);
+  const Task& task = at.task;
+  const auto end = EndOf<STAGE>::take(all_ends, task.which);
+  const int part = at.part, tile = at.tile, splits = jobs.splits;
   int ti, tj;
-  tile_place<STAGE>(it, TILE, tile, ti, tj);
-  const int depth = STAGE == kGram ? it.np : it.mp;              // k, padded: an even number of steps of 32
-  const int64_t row_bytes = (int64_t)depth * 4;
-  g.p.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B, ti * TILE, it.mp, row_bytes, wave, lane);
-  g.q.init(STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity], tj * TILE, STAGE <= kPoly ? it.mp : it.np, row_bytes, wave, lane);
+  tile_place<STAGE>(task, TILE, tile, ti, tj);
+  const int64_t row_bytes = (int64_t)task.depth * 4;            // (an even number of steps of 32)
+  g.p.init(task.p, ti * TILE, task.rows, row_bytes, wave, lane);
+  g.q.init(task.q, tj * TILE, task.cols, row_bytes, wave, lane);
   g.wave = wave, g.lane = lane;
   const int row_p = g.row_p = (wave >> 1) * (TILE / 2), row_q = g.row_q = (wave & 1) * (TILE / 2);
-  const int pairs = depth / 64;
-  const int k_first = 2 * (int)((int64_t)pairs * part / tl.splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / tl.splits);
-
-  const int columns = STAGE <= kPoly ? it.mp : it.np, rows = it.mp;
-  const Ends ends = ends_of<STAGE>(it, parity);
+  const int pairs = task.depth / 64;
+  const int k_first = 2 * (int)((int64_t)pairs * part / splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / splits);
   // 32 x 32 tiles past the matrix are neither read nor stored (dimensions are whole multiples of 64: a wave has none, or full rows)
-  auto there = [&](int i, int j) { return ti * TILE + row_p + 32 * i < rows && tj * TILE + row_q + 32 * j < columns; };
+  auto there = [&](int i, int j) { return ti * TILE + row_p + 32 * i < task.rows && tj * TILE + row_q + 32 * j < task.cols; };
   Linear early{};                         // (of the smallest tile: under way during the product)
-  if (MI * NI == 1 && STAGE != kGram && tl.splits == 1 && there(0, 0)) early.read(ends, ti * TILE + row_p, tj * TILE + row_q, lane);
+  if (MI * NI == 1 && STAGE != kGram && splits == 1 && there(0, 0)) early.read(task, ti * TILE + row_p, tj * TILE + row_q, lane);
   constexpr int kSums = Product<TILE>::kSums;
   typename Product<TILE>::Sums sums;
   f32x16 (&acc)[MI][NI] = sums[0];
@@ -719,8 +756,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
     for (int e = 0; e < 16; ++e) acc[0][0][e] += sums[1][0][0][e] + sums[2][0][0][e];
   }
 
-  if (tl.splits > 1) {
-    float* to = c.partial + ((tl.tile0[which] + tile) * tl.splits + part) * (TILE * TILE) + wave * (TILE * TILE / 4) + lane * 4;
+  if (splits > 1) {
+    float* to = jobs.partial + ((int64_t)(task.first + tile) * splits + part) * (TILE * TILE) + wave * (TILE * TILE / 4) + lane * 4;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -741,7 +778,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     linear[0][j] = early;
-    if (MI * NI > 1 && STAGE != kGram && there(0, j)) linear[0][j].read(ends, ti * TILE + row_p, tj * TILE + row_q + 32 * j, lane);
+    if (MI * NI > 1 && STAGE != kGram && there(0, j)) linear[0][j].read(task, ti * TILE + row_p, tj * TILE + row_q + 32 * j, lane);
   }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
@@ -755,7 +792,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
 #pragma unroll
     for (int j = 0; j < NI; ++j)
       if (kRows == 2 && i + 1 < MI && STAGE != kGram && there(i + 1, j))
-        linear[(i + 1) % kRows][j].read(ends, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
+        linear[(i + 1) % kRows][j].read(task, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       f32x16 sum;
@@ -770,50 +807,49 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Call c, Tiles t
         sum = acc[i][j];
       }
       if (there(i, j))
-        store_tile<STAGE>(c, it, ends, ti * TILE + row_p + 32 * i, tj * TILE + row_q + 32 * j, STAGE > kPoly || ti != tj, sum,
+        store_tile<STAGE>(task, end, ti * TILE + row_p + 32 * i, tj * TILE + row_q + 32 * j, STAGE > kPoly || ti != tj, sum,
                           linear[i % kRows][j], turn, lane);
       if (kRows == 1 && i + 1 < MI && STAGE != kGram && there(i + 1, j))
-        linear[0][j].read(ends, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
+        linear[0][j].read(task, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
     }
   }
 }
 
 // Split products: the sums of a 32 x 32 tile's parts in order, one wave each.  `edge`: of the product's tiles.
 template <int STAGE>
-__global__ __launch_bounds__(256) void finish_kernel(Call c, Tiles tl, int edge, int parity) {
+__global__ __launch_bounds__(256) void finish_kernel(Jobs jobs, typename EndOf<STAGE>::Args ends, int edge, int waves) {
   __shared__ __attribute__((aligned(16))) uint32_t turns[4][kTurnWords];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x * 4 + wave;
-  if (id >= tl.first[kMax]) return;
-  const int which = owner(tl, id);
-  const Item& it = c.item[which];
+  if (id >= waves) return;
   const int side = edge / 64, per_wave = side * side, per_tile = 4 * per_wave;      // (of a product wave: side x side tiles)
-  const int local = id - tl.first[which], tile = local / per_tile, sub = local - tile * per_tile;
-  const int of_wave = sub / per_wave, ij = sub - of_wave * per_wave;
+  const Task task = find(jobs, id, per_tile, lane);
+  const auto end = EndOf<STAGE>::take(ends, task.which);
+  const int local = id - task.first * per_tile, tile = local / per_tile, sub = local - tile * per_tile;
+  const int of_wave = sub / per_wave, ij = sub - of_wave * per_wave, splits = jobs.splits;
   int ti, tj;
-  tile_place<STAGE>(it, edge, tile, ti, tj);
+  tile_place<STAGE>(task, edge, tile, ti, tj);
   const int i0 = ti * edge + (of_wave >> 1) * (edge / 2) + 32 * (ij / side), j0 = tj * edge + (of_wave & 1) * (edge / 2) + 32 * (ij % side);
-  if (i0 >= it.mp || j0 >= (STAGE <= kPoly ? it.mp : it.np)) return;
+  if (i0 >= task.rows || j0 >= task.cols) return;
   const int64_t elems = (int64_t)edge * edge;
-  const float* from = c.partial + (tl.tile0[which] + tile) * tl.splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
-  const Ends ends = ends_of<STAGE>(it, parity);
+  const float* from = jobs.partial + (int64_t)(task.first + tile) * splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
   Linear linear{};
-  if (STAGE != kGram) linear.read(ends, i0, j0, lane);
+  if (STAGE != kGram) linear.read(task, i0, j0, lane);
   f32x16 sum;
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-  for (int s0 = 0; s0 < tl.splits; s0 += 4) {
+  for (int s0 = 0; s0 < splits; s0 += 4) {
     f32x4 v[4][4];                         // (four parts requested together; past the end the last one again)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) v[k][g] = *reinterpret_cast<const f32x4*>(from + min(s0 + k, tl.splits - 1) * elems + g * 256);
+      for (int g = 0; g < 4; ++g) v[k][g] = *reinterpret_cast<const f32x4*>(from + min(s0 + k, splits - 1) * elems + g * 256);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum[e] += s0 + k < tl.splits ? v[k][e / 4][e % 4] : 0.f;
+      for (int e = 0; e < 16; ++e) sum[e] += s0 + k < splits ? v[k][e / 4][e % 4] : 0.f;
   }
-  store_tile<STAGE>(c, it, ends, i0, j0, STAGE > kPoly || ti != tj, sum, linear, turns[wave], lane);
+  store_tile<STAGE>(task, end, i0, j0, STAGE > kPoly || ti != tj, sum, linear, turns[wave], lane);
 }
 
 // --- host ---------------------------------------------------------------------------------------------------------------
@@ -834,8 +870,7 @@ struct Cut {
 };
 struct StagePlan {
   Cut cut;
-  Tiles product, finish;
-  int blocks, finish_waves;
+  int first[kMax + 1];      // first tile of every matrix
   int64_t partial_floats;
 };
 
@@ -891,29 +926,20 @@ Cut choose(const Call& c, int stage) {
 StagePlan plan_stage(const Call& c, int stage) {
   StagePlan r{};
   r.cut = choose(c, stage);
-  const int edge = r.cut.edge, subs = (edge / 32) * (edge / 32);
   int64_t at = 0;
-  for (int i = 0; i < c.count; ++i) {
-    const int64_t tiles = tiles_of(c, i, stage, edge);
-    r.product.first[i] = (int)(at * r.cut.splits);
-    r.finish.first[i] = (int)(at * subs);
-    r.product.tile0[i] = r.finish.tile0[i] = at;
-    at += tiles;
+  for (int i = 0; i < kMax; ++i) {
+    r.first[i] = (int)at;
+    if (i < c.count) at += tiles_of(c, i, stage, r.cut.edge);
   }
-  for (int i = c.count; i <= kMax; ++i) {
-    r.product.first[i] = (int)(at * r.cut.splits);
-    r.finish.first[i] = (int)(at * subs);
-  }
-  r.product.splits = r.finish.splits = r.cut.splits;
-  r.blocks = (int)(at * r.cut.splits);
-  r.finish_waves = (int)(at * subs);
-  r.partial_floats = r.cut.splits > 1 ? at * r.cut.splits * edge * edge : 0;
+  r.first[kMax] = (int)at;
+  r.partial_floats = r.cut.splits > 1 ? at * r.cut.splits * r.cut.edge * r.cut.edge : 0;
   return r;
 }
 
 struct Layout {
   int64_t total;
   StagePlan stage[3];
+  float* partial;
 };
 // Fills the workspace part of `c` (from `base`, which may be null when only the size is asked for) and cuts the products.
 Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, char* base) {
@@ -946,21 +972,43 @@ Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, cha
     l.stage[stage] = plan_stage(c, stage);
     partial = l.stage[stage].partial_floats > partial ? l.stage[stage].partial_floats : partial;
   }
-  c.partial = reinterpret_cast<float*>(take(partial * 4));
+  l.partial = reinterpret_cast<float*>(take(partial * 4));
   l.total = at;
   return l;
 }
 
 template <int STAGE>
-void launch_stage(const Call& c, const StagePlan& p, int parity, hipStream_t s) {
-  switch (p.cut.edge) {
-    case 32: narrow_kernel<STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
-    case 64: product_kernel<64, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
-    case 128: product_kernel<128, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
-    case 192: product_kernel<192, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity); break;
-    default: product_kernel<256, STAGE><<<p.blocks, 256, 0, s>>>(c, p.product, parity);
+void launch_stage(const Call& c, const Layout& l, int parity, const typename EndOf<STAGE>::Args& ends, hipStream_t s) {
+  const StagePlan& p = l.stage[STAGE == kLast ? kStep : STAGE];
+  Jobs jobs{};
+  jobs.partial = l.partial;
+  jobs.splits = p.cut.splits;
+  for (int i = 0; i < kMax; ++i) {
+    Job& j = jobs.job[i];
+    j.first = p.first[i], j.tiles = p.first[i + 1] - p.first[i];
+    if (i >= c.count) continue;              // (behind every workgroup)
+    const Item& it = c.item[i];
+    j.p = STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B;
+    j.q = STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity];
+    j.linear = STAGE == kPoly ? it.A : it.XT[parity];
+    j.straight = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.X;
+    j.turned = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.XT[parity ^ 1];
+    j.rows = it.mp;
+    j.cols = STAGE <= kPoly ? it.mp : it.np;
+    j.depth = STAGE == kGram ? it.np : it.mp;
   }
-  if (p.cut.splits > 1) finish_kernel<STAGE><<<(p.finish_waves + 3) / 4, 256, 0, s>>>(c, p.finish, p.cut.edge, parity);
+  const int edge = p.cut.edge, blocks = p.first[kMax] * p.cut.splits;
+  switch (edge) {
+    case 32: narrow_kernel<STAGE><<<blocks, 256, 0, s>>>(jobs, ends); break;
+    case 64: product_kernel<64, STAGE><<<blocks, 256, 0, s>>>(jobs, ends); break;
+    case 128: product_kernel<128, STAGE><<<blocks, 256, 0, s>>>(jobs, ends); break;
+    case 192: product_kernel<192, STAGE><<<blocks, 256, 0, s>>>(jobs, ends); break;
+    default: product_kernel<256, STAGE><<<blocks, 256, 0, s>>>(jobs, ends);
+  }
+  if (p.cut.splits > 1) {
+    const int waves = p.first[kMax] * (edge / 32) * (edge / 32);
+    finish_kernel<STAGE><<<(waves + 3) / 4, 256, 0, s>>>(jobs, ends, edge, waves);
+  }
 }
 
 template <typename T>
@@ -972,11 +1020,17 @@ int run(Call& c, const Layout& l, hipStream_t s) {
     most = t > most ? t : most;
   }
   split_kernel<T><<<dim3((unsigned)most, c.count), 256, 0, s>>>(c);
+  Finals finals{};
+  for (int i = 0; i < c.count; ++i) {
+    const Item& it = c.item[i];
+    finals.of[i] = Final{it.out, it.ldo, it.m, it.n, it.flip, it.shape_factor};
+  }
+  finals.lr = c.lr, finals.dtype = c.dtype;
   for (int k = 0; k < 5; ++k) {
-    launch_stage<kGram>(c, l.stage[kGram], k & 1, s);
-    launch_stage<kPoly>(c, l.stage[kPoly], k & 1, s);
-    if (k < 4) launch_stage<kStep>(c, l.stage[kStep], k & 1, s);
-    else launch_stage<kLast>(c, l.stage[kStep], k & 1, s);
+    launch_stage<kGram>(c, l, k & 1, None{}, s);
+    launch_stage<kPoly>(c, l, k & 1, None{}, s);
+    if (k < 4) launch_stage<kStep>(c, l, k & 1, None{}, s);
+    else launch_stage<kLast>(c, l, k & 1, finals, s);
   }
   return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
 }
