@@ -24,8 +24,8 @@
 // GEMM form (row times row) serves all.  A row of a plane pair is groups of 32 columns: 32 hi halves then 32 lo halves, 128
 // bytes, one cache line per row and k-step.  Dimensions are padded with zeros to whole tiles: the products need no bounds.
 //
-// GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 and walks k in steps of 32 through a ring of 8, 4, 3
-// or 2 LDS images filled by direct buffer-to-LDS loads: 130 to 140 KB, one workgroup per CU, the loads of a step requested one
+// GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 (or 32, see Narrow) and walks k in steps of 32 through a
+// ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 130 to 140 KB, one workgroup per CU, the loads of a step requested one
 // to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away, against 0.1 to 1.8 us of products per
 // step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so the 16-byte chunks of a row are
 // permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the sixteen rows that a quarter of a fragment
@@ -886,7 +886,8 @@ int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut
 // rate at 2.4 GHz) and what a workgroup spends outside its steps, both measured.  One workgroup per CU at a time.  Long launches
 // stay near the power limit even when some CUs have no work.  A split product pays a second launch and its sums' traffic.
 // Against the choice, in us: 4096^2 x 4096 symmetric 192/1 178 (256/1 242, 128/1 233, 128/2 224); 4096^3 256/1 313 (192/1 345,
-// 128/1 359, 64/1 472); 1024 x 4096 x 1024 128/1 33 (256/1 72, 64/1 44); 1024^2 x 1024 symmetric 64/1 12 (128/4 19, 256/1 70).
+// 128/1 359, 64/1 472); 1024 x 4096 x 1024 128/1 33 (256/1 72, 64/1 44); 1024^2 x 1024 symmetric 64/1 11 (32/1 19,
+// 128/4 19, 256/1 70); 512^2 x 832 symmetric 32/1 7.3 (64/1 9.9, 64/2 12, 128/2 16).
 Cut choose(const Call& c, int stage) {
   static const struct { int edge; double step, loaded, rest; } kinds[] = {
       {256, 1.34, 2.3, 18.0}, {192, 0.755, 1.3, 11.5}, {128, 0.39, 0.65, 6.0}, {64, 0.175, 0.24, 2.0}, {32, 0.085, 0.12, 1.5}};
