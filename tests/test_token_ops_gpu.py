@@ -431,3 +431,19 @@ def test_no_second_derivatives():
         (g,) = torch.autograd.grad(losses.sum(), table, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), table)
+
+
+@pytest.mark.parametrize("gap", [0, 4])
+@pytest.mark.parametrize("rows", [300, 60000])
+def test_gradient_of_a_table_over_what_was_there(rows, gap):
+    """Rows that do not occur become zeros whoever clears them (60000 x 1024 is more than the sort's launches take), the
+    elements between the rows stay as they were."""
+    dim, tokens = 1024, 4100
+    ids = make_ids(tokens, rows, 130, kind="uniform")
+    g = torch.randn(tokens, dim, device="cuda", generator=gen(131))
+    room = torch.full((rows, dim + gap), float("nan"), device="cuda")
+    embedding.lookup_grad(ids, g, rows, out=room[:, :dim])
+    want, size, count = exact_sums(ids, g, rows)
+    # (an fp32 sum of n terms is off by less than n 2^-24 of the sum of their magnitudes)
+    assert bool(((room[:, :dim].double() - want).abs() <= count[:, None] * 2.0 ** -24 * size).all())
+    assert bool(room[:, dim:].isnan().all()) and (rows == 300 or bool((count == 0).any()))
