@@ -9,7 +9,7 @@
 // All three are bound by memory.  The gradient must not depend on the order in which atomics land, and a frequent token
 // must not serialise on its row.
 //
-// Up to 4096 tokens, where launches and trips to memory count: one launch, a block per token.  The block of an id's FIRST
+// Few tokens and elements, where launches and trips to memory count (see few()): one launch, a block per token.  The block of an id's FIRST
 // occurrence finds the others by comparing (T^2 / 64 wave steps in all), each wave in a range of tokens of its own, and the
 // waves' sums meet in order; the other blocks end at once.  (3001 tokens x 101, the whole pass: sorting by one workgroup, summing and
 // joining took 23.6 us, this takes 13.3.)
@@ -37,7 +37,7 @@
 
 namespace {
 
-constexpr int kSmall = 4096;        // tokens compared with each other instead of sorted
+constexpr int kSmall = 4096;        // tokens compared with each other instead of sorted, at most (see few())
 constexpr int kSmallWaves = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kWaves = kSortThreads / 64;
@@ -557,6 +557,15 @@ inline int chunk_of(int64_t tokens, int64_t lanes) {
   return c < 4 ? 4 : c > 64 ? 64 : (int)c;
 }
 
+// Whether tokens are compared with each other (one launch, 13 us while little is moved) or sorted (20 to 25 us, and the rows of a
+// frequent token are shared out).  Measured with ids as words occur, row update, fp32: 4096 x 512 of 2000 rows 16 us against 27, 1000 x
+// 2048 of 250 rows 13 against 20, 300 x 8192 13 against 24; but 2000 x 2048 of 30 rows 29 against 20, 4096 x 2048 of 2000 rows
+// 42 against 36, 4096 x 8192 155 against 60; of four rows 2000 x 512 19 against 20, 4096 x 512 46 against 25.
+inline bool few(int64_t tokens, int64_t packs, int64_t rows) {
+  return tokens <= kSmall && tokens * packs <= (rows < 16 ? 1 << 18 : 3 << 18);
+}
+inline bool surely_few(int64_t tokens, int64_t dim) { return few(tokens, dim, 1); }      // whatever the alignment and the rows
+
 struct Workspace {
   int64_t keys, order, pairs, counts, pieces, total;    // byte offsets
   int64_t chunks, piece_ld;
@@ -571,7 +580,7 @@ Workspace plan(int64_t tokens, int dim) {
   w.chunk = chunk_of(tokens, (dim + 3) / 4);
   w.chunks = (tokens + w.chunk - 1) / w.chunk;
   w.piece_ld = (dim + 7) / 8 * 8;
-  const int64_t big = tokens > kSmall ? 1 : 0;         // (fewer tokens need no workspace)
+  const int64_t big = surely_few(tokens, dim) ? 0 : 1;         // (these need no workspace)
   w.keys = 0;
   w.order = up(w.keys + big * 4 * tokens);
   w.pairs = up(w.order + big * 4 * tokens);
@@ -634,7 +643,7 @@ template <typename T, int N, bool UPDATE>
 void launch_sums(SumArgs a, const void* ids, int wide, const T* g, T* table, int64_t fill_rows, hipStream_t s) {
   a.packs = a.dim / N;
   a.lanes_log2 = log2_lanes(a.packs);
-  if (a.tokens <= kSmall) {
+  if (few(a.tokens, a.packs, a.rows)) {
     if (!UPDATE) {
       const int64_t blocks = (fill_rows + (kThreads >> a.lanes_log2) - 1) / (kThreads >> a.lanes_log2);
       zero_rows_kernel<T, N><<<(unsigned)(blocks > 16384 ? 16384 : blocks), kThreads, 0, s>>>(table, fill_rows, a.packs, a.ldt, a.lanes_log2, a.past);
@@ -684,7 +693,7 @@ int scatter_sums(bool update, const void* ids, int wide, int64_t tokens, const v
   const int bytes = dtf_access_bytes((uint64_t)g | (uint64_t)table | (uint64_t)(ldg * sizeof(T)) | (uint64_t)(ldt * sizeof(T)) |
                                      (uint64_t)(dim * sizeof(T)));
   int64_t fill = update ? 0 : rows;
-  if (tokens > kSmall) {
+  if (!few(tokens, dim / std::max<int>(bytes / (int)sizeof(T), 1), rows)) {
     Clear c{};
     if (!update && bytes == 16) c = Clear{static_cast<char*>(table), rows, (int64_t)(dim * sizeof(T)), (int64_t)(ldt * sizeof(T)), a.past};
     fill -= sort_tokens(ids, wide, tokens, (uint32_t)rows, w, ws, c, s);
