@@ -270,6 +270,12 @@ int dtf_embed_sgd(const void* ids, int ids_wide, int64_t tokens, const void* g, 
 // relative to it, what dtf_sparse_xent_grad needs.  A negative label is padding (loss 0, gradient 0), one >= classes gives NaN.
 int dtf_sparse_xent(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
                     int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats, void* stream);
+// The same for few long rows, several blocks a row: workspace of dtf_sparse_xent_workspace bytes (0: nothing to gain), 8-byte
+// aligned, contents unimportant.
+int64_t dtf_sparse_xent_workspace(int dtype, int64_t tokens, int64_t classes);
+int dtf_sparse_xent_cut(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                        int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats,
+                        void* workspace, int64_t workspace_bytes, void* stream);
 // dz = g[t * g_stride] * d(row loss t)/dz
 int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
                          int labels_wide, const float* stats, const float* g, int64_t g_stride, void* dz, int64_t ldz,

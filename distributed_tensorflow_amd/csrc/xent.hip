@@ -13,7 +13,7 @@
 // REGISTERS between the sums and the gradient (64 bytes to 256 KB a row: up to 16 packs of 16 bytes for each of up to 1024 threads),
 // so the second use of a row costs no traffic.  Every thread finds the maximum of its own elements first and sums
 // exponentials relative to it; the pairs (maximum, sum) meet in one exchange: one barrier per row and not two.  Rows that do
-// not fit are streamed twice.  Rows may start at any element: packs are aligned to 16 bytes of memory, and the first and last
+// not fit are streamed twice, or, where they are few, cut into slices for a block each.  Rows may start at any element: packs are aligned to 16 bytes of memory, and the first and last
 // pack of a row are taken element by element.
 #include "dtf_api.h"
 #include "dtf_types.h"
@@ -272,10 +272,44 @@ __global__ __launch_bounds__(kStream) void xent_stream_kernel(XentArgs a, T* log
   }
 }
 
-// The backward pass alone, from the statistics of the forward pass: a block takes kSlice packs of a row.
+// Few long rows: one block per row would leave most CUs without work, so a block takes kSlice packs of a row.  First the maximum and
+// the sum of every slice and the label's logit (before a gradient can lie on top of it), then, in a second launch, every block joins
+// its row's pairs in the same order and writes its slice of the gradient.
 constexpr int kGradPacks = 4, kGradThreads = 256, kSlice = kGradPacks * kGradThreads;
-template <typename T, bool SAME>
-__global__ __launch_bounds__(kGradThreads) void xent_grad_kernel(XentArgs a, T* logits, T* dz) {
+struct Parts {
+  float2* pair;       // [tokens][slices]
+  float* z_label;     // [tokens]
+  int slices;
+};
+template <typename T>
+__global__ __launch_bounds__(kGradThreads) void xent_part_kernel(XentArgs a, T* logits, Parts parts) {
+  typedef typename Row<T>::P P;
+  const int64_t t = blockIdx.x;
+  const Row<T> row(logits + t * a.ld, a.classes);
+  const int64_t label = label_of(a, t);
+  if (label < 0 || label >= a.classes) return;
+  P z[kGradPacks];
+  row.load(blockIdx.y * kSlice + threadIdx.x, kGradThreads, z);
+  float m = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int k = 0; k < kGradPacks; ++k)
+#pragma unroll
+    for (int e = 0; e < Row<T>::N; ++e) m = fmaxf(m, (float)z[k].v[e]);
+  const float own = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int k = 0; k < kGradPacks; ++k)
+#pragma unroll
+    for (int e = 0; e < Row<T>::N; ++e) s += exp_of((float)z[k].v[e] - own);
+  merge_row<kGradThreads>(m, s);
+  if (threadIdx.x == 0) {
+    parts.pair[t * parts.slices + blockIdx.y] = make_float2(m, s);
+    if (((int)label + row.lead) / Row<T>::N / kSlice == (int)blockIdx.y) parts.z_label[t] = (float)row.first[label];
+  }
+}
+
+// The backward pass: from the statistics of the forward pass, or (JOIN) as the second launch of few rows.
+template <typename T, bool SAME, bool JOIN>
+__global__ __launch_bounds__(kGradThreads) void xent_grad_kernel(XentArgs a, T* logits, T* dz, Parts parts) {
   typedef typename Row<T>::P P;
   const int64_t t = blockIdx.x;
   const Row<T> row(logits + t * a.ld, a.classes);
@@ -284,9 +318,26 @@ __global__ __launch_bounds__(kGradThreads) void xent_grad_kernel(XentArgs a, T* 
   const int i0 = blockIdx.y * kSlice + threadIdx.x;
   const bool use = label >= 0 && label < a.classes;
   P z[kGradPacks];
-  if (use) row.load(i0, kGradThreads, z);
-  const float weight = a.g[t * a.g_stride];
-  const float m = a.stats[2 * t], factor = weight / a.stats[2 * t + 1];
+  if (use && dz) row.load(i0, kGradThreads, z);
+  float weight, m, total;
+  if (JOIN) {
+    weight = a.grad_scale, m = -INFINITY, total = 0.f;
+    if (use) {
+      for (int i = threadIdx.x; i < parts.slices; i += kGradThreads) {
+        const float2 pair = parts.pair[t * parts.slices + i];
+        merge(m, total, pair.x, pair.y);
+      }
+      merge_row<kGradThreads>(m, total);
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) {
+      if (a.row_loss) a.row_loss[t] = use ? (m - parts.z_label[t]) + logf(total) : label < 0 ? 0.f : NAN;
+      if (a.stats) a.stats[2 * t] = use ? m : 0.f, a.stats[2 * t + 1] = use ? total : 1.f;
+    }
+    if (!dz) return;
+  } else {
+    weight = a.g[t * a.g_stride], m = a.stats[2 * t], total = a.stats[2 * t + 1];
+  }
+  const float factor = weight / total;
 #pragma unroll
   for (int k = 0; k < kGradPacks; ++k) {
     const int i = i0 + k * kGradThreads;
@@ -328,22 +379,38 @@ int launch_xent(const XentArgs& a, T* logits, T* dz, hipStream_t s) {
   return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
 }
 
+// Slices of a row that starts anywhere in a pack.
+inline int64_t slices_of(int64_t classes, int per_pack) { return ((classes + 2 * per_pack - 2) / per_pack + kSlice - 1) / kSlice; }
+
+// Rows are cut where one block a row takes longer than a second launch (cut: 13.5 us a call up to 64 x 131072 bf16).  One block a
+// row, fp32: 1 x 50001 10 us, 1 x 131072 20, 1 x 1000000 133, 64 x 262144 44 (cut 33), 128 x 131072 32 (cut 34).
+bool cut_rows(int64_t tokens, int64_t slices) { return tokens <= 64 && slices > 16; }
+
 template <typename T>
-int run_xent(const XentArgs& a, const void* logits, void* dz, bool backward, hipStream_t s) {
+int run_xent(const XentArgs& a, const void* logits, void* dz, bool backward, const Parts& parts, hipStream_t s) {
   T* z = static_cast<T*>(const_cast<void*>(logits));
   T* d = static_cast<T*>(dz);
   const bool same = !d || ((((uintptr_t)z ^ (uintptr_t)d) & 15u) == 0 && ((a.ld - a.ldz) * (int64_t)sizeof(T)) % 16 == 0);
   if (backward) {
     constexpr int N = 16 / sizeof(T);
-    const dim3 grid((unsigned)a.tokens, (unsigned)(((a.classes + 2 * N - 2) / N + kSlice - 1) / kSlice));
-    if (same) xent_grad_kernel<T, true><<<grid, kGradThreads, 0, s>>>(a, z, d);
-    else xent_grad_kernel<T, false><<<grid, kGradThreads, 0, s>>>(a, z, d);
+    const dim3 grid((unsigned)a.tokens, (unsigned)slices_of(a.classes, N));
+    if (same) xent_grad_kernel<T, true, false><<<grid, kGradThreads, 0, s>>>(a, z, d, Parts{});
+    else xent_grad_kernel<T, false, false><<<grid, kGradThreads, 0, s>>>(a, z, d, Parts{});
+    return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
+  }
+  if (parts.slices) {
+    const dim3 grid((unsigned)a.tokens, (unsigned)parts.slices);
+    xent_part_kernel<T><<<grid, kGradThreads, 0, s>>>(a, z, parts);
+    const dim3 second((unsigned)a.tokens, d ? (unsigned)parts.slices : 1u);
+    if (same) xent_grad_kernel<T, true, true><<<second, kGradThreads, 0, s>>>(a, z, d, parts);
+    else xent_grad_kernel<T, false, true><<<second, kGradThreads, 0, s>>>(a, z, d, parts);
     return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
   }
   return same ? launch_xent<T, true>(a, z, d, s) : launch_xent<T, false>(a, z, d, s);
 }
 
-int checked(const XentArgs& a, const void* logits, int dtype, void* dz, bool backward, void* stream) {
+int checked(const XentArgs& a, const void* logits, int dtype, void* dz, bool backward, void* stream, void* workspace = nullptr,
+            int64_t workspace_bytes = 0) {
   // (grids stay below 2^32 threads, the class index of a row below 2^31)
   if (a.tokens < 0 || a.tokens > (1 << 21) || a.classes < 1 || a.classes > (1 << 26) || dtype < 0 || dtype > 2 ||
       a.ld < a.classes || (dz && a.ldz < a.classes))
@@ -351,20 +418,38 @@ int checked(const XentArgs& a, const void* logits, int dtype, void* dz, bool bac
   if (a.tokens == 0) return DTF_OK;
   if (!logits || !a.labels || (backward && (!dz || !a.stats || !a.g))) return DTF_ERR_NULL;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DTF_F32) return run_xent<float>(a, logits, dz, backward, s);
-  if (dtype == DTF_BF16) return run_xent<bf16_t>(a, logits, dz, backward, s);
-  return run_xent<f16_t>(a, logits, dz, backward, s);
+  Parts parts{};
+  const int64_t slices = slices_of(a.classes, 16 / dtf_type_size(dtype));
+  if (workspace && cut_rows(a.tokens, slices)) {
+    if (workspace_bytes < a.tokens * (slices * 8 + 4) || ((uintptr_t)workspace & 7u)) return DTF_ERR_SHAPE;
+    parts = Parts{static_cast<float2*>(workspace), reinterpret_cast<float*>(static_cast<float2*>(workspace) + a.tokens * slices), (int)slices};
+  }
+  if (dtype == DTF_F32) return run_xent<float>(a, logits, dz, backward, parts, s);
+  if (dtype == DTF_BF16) return run_xent<bf16_t>(a, logits, dz, backward, parts, s);
+  return run_xent<f16_t>(a, logits, dz, backward, parts, s);
 }
 
 }  // namespace
 
+extern "C" int64_t dtf_sparse_xent_workspace(int dtype, int64_t tokens, int64_t classes) {
+  if (tokens < 0 || classes < 1 || classes > (1 << 26) || dtype < 0 || dtype > 2) return -1;
+  const int64_t slices = slices_of(classes, 16 / dtf_type_size(dtype));
+  return cut_rows(tokens, slices) ? tokens * (slices * 8 + 4) : 0;
+}
+
 extern "C" int dtf_sparse_xent(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
                                int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats,
                                void* stream) {
+  return dtf_sparse_xent_cut(logits, dtype, tokens, classes, ld, labels, labels_wide, dz, ldz, grad_scale, row_loss, stats, nullptr, 0, stream);
+}
+
+extern "C" int dtf_sparse_xent_cut(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,
+                                   int labels_wide, void* dz, int64_t ldz, float grad_scale, float* row_loss, float* stats,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
   XentArgs a{};
   a.tokens = tokens, a.classes = classes, a.ld = ld, a.ldz = dz ? ldz : ld;
   a.labels = labels, a.wide = labels_wide, a.grad_scale = grad_scale, a.row_loss = row_loss, a.stats = stats;
-  return checked(a, logits, dtype, dz, false, stream);
+  return checked(a, logits, dtype, dz, false, stream, workspace, workspace_bytes);
 }
 
 extern "C" int dtf_sparse_xent_grad(const void* logits, int dtype, int64_t tokens, int64_t classes, int64_t ld, const void* labels,

@@ -14,7 +14,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_backend as hb
 
@@ -119,10 +118,10 @@ class _Lookup(torch.autograd.Function):
     def forward(ctx, table, ids, scale):
         ctx.save_for_backward(ids)
         ctx.rows, ctx.scale = table.shape[0], scale
-        return lookup(table.detach(), ids, scale)
+        return lookup(table, ids, scale)
 
     @staticmethod
-    @once_differentiable
+    @hb.first_order
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
         return lookup_grad(ids, g, ctx.rows, ctx.scale), None, None

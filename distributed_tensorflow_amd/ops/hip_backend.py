@@ -7,11 +7,13 @@ there is no silent PyTorch fallback for CUDA tensors.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _LIB_PATH = Path(os.environ.get("DTF_HIP_LIB") or Path(__file__).resolve().parent.parent / "_lib" / "libdtf_hip.so")   # DTF_HIP_LIB: a variant build (tuning experiments)
 _lib: Optional[C.CDLL] = None
@@ -167,6 +169,9 @@ def _declare(lib: C.CDLL) -> None:
     lib.dtf_embed_grad.argtypes = [vp, i32, i64, vp, i64, vp, i32, i64, i32, i64, f32, vp, i64, vp]
     lib.dtf_embed_sgd.argtypes = [vp, i32, i64, vp, i64, vp, i32, i64, i32, i64, f32, vp, vp, i64, vp]
     lib.dtf_sparse_xent.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, f32, vp, vp, vp]
+    lib.dtf_sparse_xent_cut.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, f32, vp, vp, vp, i64, vp]
+    lib.dtf_sparse_xent_workspace.argtypes = [i32, i64, i64]
+    lib.dtf_sparse_xent_workspace.restype = i64
     lib.dtf_sparse_xent_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, vp, i64, vp, i64, vp]
     lib.dtf_muon_workspace.argtypes = [i32, vp, vp]
     lib.dtf_muon_workspace.restype = i64
@@ -174,7 +179,7 @@ def _declare(lib: C.CDLL) -> None:
     lib.dtf_debug_set_muon_cut.restype = None
     lib.dtf_muon_step.argtypes = [i32, vp, vp, vp, vp, vp, vp, f32, i32, f32, vp, i64, vp]
     lib.dtf_orthogonalize.argtypes = [vp, i32, i32, i32, i64, vp, i64, f32, vp, i64, vp]
-    for name in ("dtf_muon_step", "dtf_orthogonalize", "dtf_embed_lookup", "dtf_embed_grad", "dtf_embed_sgd", "dtf_sparse_xent", "dtf_sparse_xent_grad"):
+    for name in ("dtf_muon_step", "dtf_orthogonalize", "dtf_embed_lookup", "dtf_embed_grad", "dtf_embed_sgd", "dtf_sparse_xent", "dtf_sparse_xent_cut", "dtf_sparse_xent_grad"):
         getattr(lib, name).restype = C.c_int
     lib.dtf_debug_force_generic_path.argtypes = [i32]
     lib.dtf_debug_force_generic_path.restype = None
@@ -287,6 +292,13 @@ def _f32c(t: torch.Tensor, name: str) -> torch.Tensor:
 # operands of the token-model operators (ops/embedding.py, ops/xent.py, ops/muon.py)
 # ---------------------------------------------------------------------------
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # DTF_F32, DTF_BF16, DTF_F16
+
+
+def first_order(backward):
+    """A ``backward`` of launches: differentiating its result is an error.  (torch's ``once_differentiable``, whose context costs 3 us,
+    only where a graph of the gradient is being recorded.)"""
+    recorded = once_differentiable(backward)
+    return functools.wraps(backward)(lambda ctx, *g: recorded(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g))
 
 
 def typed_rows(t: torch.Tensor, name: str) -> int:

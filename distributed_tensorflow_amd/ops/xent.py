@@ -3,7 +3,8 @@ labels of ``hip_backend.softmax_xent`` would be a matrix as large as the logits.
 
 ``sparse_softmax_xent(logits, labels)`` is the differentiable operator: the loss of every row
 (``tf.nn.sparse_softmax_cross_entropy_with_logits`` of a graph evaluates to it).  ``sparse_softmax_xent_step`` is the training
-step's form: losses and gradient in ONE launch that reads the logits once and keeps each row in registers in between.
+step's form: losses and gradient in ONE launch that reads the logits once and keeps each row in registers in between (two
+launches for up to 64 rows of more than 256 KB).
 
 A negative label is padding: loss 0, a gradient row of zeros, the row's logits are not looked at.  A label that is no class
 (``>= classes``) gives NaN.  Logits in float32, bfloat16 or float16 with contiguous rows; losses in float32.
@@ -13,7 +14,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip_backend as hb
 
@@ -39,10 +39,18 @@ def _forward(logits, labels, dz, grad_scale, stats):
     lib = hb.require()
     ld, flat = _operands(logits, labels)
     ldz = 0 if dz is None else _dz_rows(dz, logits)
-    loss = torch.empty((logits.shape[0],), device=logits.device, dtype=torch.float32)
-    hb._check(lib.dtf_sparse_xent(logits.data_ptr(), hb.TYPE_CODES[logits.dtype], logits.shape[0], logits.shape[1], ld,
-                                  flat.data_ptr(), int(flat.dtype == torch.int64), hb._ptr(dz), ldz, float(grad_scale),
-                                  loss.data_ptr(), hb._ptr(stats), hb._stream(logits)), "dtf_sparse_xent")
+    rows, classes = logits.shape
+    code = hb.TYPE_CODES[logits.dtype]
+    loss = torch.empty((rows,), device=logits.device, dtype=torch.float32)
+    args = (logits.data_ptr(), code, rows, classes, ld, flat.data_ptr(), int(flat.dtype == torch.int64), hb._ptr(dz), ldz,
+            float(grad_scale), loss.data_ptr(), hb._ptr(stats))
+    # few long rows: several blocks each, which need a workspace
+    need = lib.dtf_sparse_xent_workspace(code, rows, classes) if rows <= 64 and classes >= 1 << 16 else 0
+    if need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        hb._check(lib.dtf_sparse_xent_cut(*args, ws.data_ptr(), need, hb._stream(logits)), "dtf_sparse_xent_cut")
+    else:
+        hb._check(lib.dtf_sparse_xent(*args, hb._stream(logits)), "dtf_sparse_xent")
     return loss, flat
 
 
@@ -56,17 +64,15 @@ def sparse_softmax_xent_step(logits: torch.Tensor, labels: torch.Tensor, *, dz: 
 class _SparseXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels):
-        z = logits.detach()
-        stats = torch.empty((z.shape[0], 2), device=z.device, dtype=torch.float32)
-        loss, flat = _forward(z, labels, None, 1.0, stats)
+        stats = torch.empty((logits.shape[0], 2), device=logits.device, dtype=torch.float32)
+        loss, flat = _forward(logits, labels, None, 1.0, stats)
         ctx.save_for_backward(logits, flat, stats)
         return loss
 
     @staticmethod
-    @once_differentiable
+    @hb.first_order
     def backward(ctx, g):
-        logits, flat, stats = ctx.saved_tensors
-        z = logits.detach()
+        z, flat, stats = ctx.saved_tensors
         g = g.to(torch.float32)
         dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
         hb._check(hb.require().dtf_sparse_xent_grad(z.data_ptr(), hb.TYPE_CODES[z.dtype], z.shape[0], z.shape[1],

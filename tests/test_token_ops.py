@@ -122,3 +122,17 @@ def test_native_refusals_of_the_orthogonalised_update():
         muon.orthogonalize(torch.zeros(3, 4))
     with pytest.raises(hb.HipKernelError):
         muon.MuonPlan([torch.zeros(3, 4)], [torch.zeros(3, 4)], [torch.zeros(3, 4)])
+
+
+def test_native_refusals_of_few_long_rows():
+    lib = hb.load()
+    need = lib.dtf_sparse_xent_workspace(0, 3, 300000)
+    assert need > 0 and lib.dtf_sparse_xent_workspace(0, 65, 300000) == 0 and lib.dtf_sparse_xent_workspace(0, 3, 300) == 0
+    assert lib.dtf_sparse_xent_workspace(3, 3, 300000) < 0 and lib.dtf_sparse_xent_workspace(0, -1, 300000) < 0
+    assert lib.dtf_sparse_xent_workspace(0, 3, (1 << 26) + 1) < 0 and lib.dtf_sparse_xent_workspace(0, 3, 0) < 0
+    one = 4096
+
+    def step(ws=one, size=need, dtype=0, ld=300000):
+        return lib.dtf_sparse_xent_cut(one, dtype, 3, 300000, ld, one, 1, one, 300000, 1.0, one, None, ws, size, None)
+
+    assert step(size=need - 1) == step(ws=one + 4) == step(dtype=3) == step(ld=299999) == SHAPE

@@ -447,3 +447,38 @@ def test_gradient_of_a_table_over_what_was_there(rows, gap):
     # (an fp32 sum of n terms is off by less than n 2^-24 of the sum of their magnitudes)
     assert bool(((room[:, :dim].double() - want).abs() <= count[:, None] * 2.0 ** -24 * size).all())
     assert bool(room[:, dim:].isnan().all()) and (rows == 300 or bool((count == 0).any()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [66000, 131080, 262147])
+def test_xent_of_many_long_rows(dtype, classes):
+    """65 rows: one block each (64 would be cut into slices)."""
+    logits = (3 * torch.randn(65, classes, device="cuda", generator=gen(140))).to(dtype)
+    labels = torch.randint(0, classes, (65,), device="cuda", generator=gen(141))
+    labels[1] = -1
+    dz = torch.empty_like(logits)
+    loss = xent.sparse_softmax_xent_step(logits, labels, dz=dz, grad_scale=0.5)
+    for rows in (slice(0, 9), slice(56, 65)):            # (64-bit copies of all of them would take gigabytes)
+        n = rows.stop - rows.start
+        check_xent(logits[rows], labels[rows], torch.full((n,), 0.5, device="cuda", dtype=torch.float64), loss[rows], dz[rows])
+    inplace = logits.clone()
+    assert torch.equal(xent.sparse_softmax_xent_step(inplace, labels, dz=inplace, grad_scale=0.5), loss) and torch.equal(inplace, dz)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_xent_of_rows_in_slices_labels_at_their_ends(dtype, shift):
+    """Slices are 1024 packs of 16 bytes of memory: labels on either side of their borders, in a row that starts inside a pack."""
+    per_slice = 1024 * 16 // dtype.itemsize
+    classes = 20 * per_slice + 5
+    at = [0, classes - 1, classes - 5] + [k * per_slice - shift + d for k in (1, 7, 20) for d in (-1, 0, 1)]
+    room = (2 * torch.randn(classes + shift, device="cuda", generator=gen(142))).to(dtype)
+    logits = room[shift:].unsqueeze(0)
+    for label in at:
+        labels = torch.tensor([label], device="cuda")
+        dz = torch.empty_like(logits)
+        loss = xent.sparse_softmax_xent_step(logits, labels, dz=dz)
+        check_xent(logits, labels, torch.ones(1, device="cuda", dtype=torch.float64), loss, dz)
+        assert torch.equal(xent.sparse_softmax_xent_step(logits, labels), loss)
+        inplace = room.clone()[shift:].unsqueeze(0)
+        assert torch.equal(xent.sparse_softmax_xent_step(inplace, labels, dz=inplace), loss) and torch.equal(inplace, dz)
