@@ -524,8 +524,8 @@ struct Product {
   static constexpr int kReads = 2 * (MI + NI), kMfmas = 3 * MI * NI, kSums = MI * NI == 1 ? 3 : 1;
   typedef f32x16 Sums[kSums][MI][NI];
   // Small tiles have registers for all fragments of two steps: the reads of step k are covered by the whole of step k - 1, and the
-  // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417, 2.4 times its MFMAs: its 16 KB
-  // of loads a step set the pace there, 39 bytes a cycle and CU).
+  // wait in front of the barrier finds them done (128: 931 -> 890 cycles a step; 64 stays at 417, of which
+  // its LDS accesses take 384).
   static constexpr bool kWhole = TILE <= 128;
   Fetcher<TILE, kWaves> p, q;
   Half<MI, NI> first, second;               // halves of a step, in turn
