@@ -911,6 +911,9 @@ class Session:
         if applied:
             return
         if not plain:
+            if sparse_grads is None:
+                # (of the op's own variables alone: elsewhere in the slab may lie what another train op has left)
+                sparse_grads = {v.op_name: self.layout.view(self.grad, v.op_name) for v in train_op.attrs["var_list"]}
             with span("muon"):
                 self._muon_update(train_op, opt, sparse_grads)
         if sparse_grads is not None:
@@ -938,16 +941,16 @@ class Session:
                 self.store.push_apply(self.grad, lr, opt.use_locking,
                                       bump_step=train_op.attrs["global_step"] is not None)
 
-    def _muon_update(self, train_op, opt: MuonOptimizer, grads: Optional[Dict[str, torch.Tensor]]):
-        """The matrices of a train op: momentum, orthogonalised direction, weights, all in place; their gradients then are
-        out of what plain gradient descent applies (``grads`` by name, or the gradient slab if None)."""
+    def _muon_update(self, train_op, opt: MuonOptimizer, grads: Dict[str, torch.Tensor]):
+        """The matrices of a train op: momentum, orthogonalised direction, weights, all in place.  ``grads`` by name; what is left in
+        it afterwards is for plain gradient descent."""
         slots = train_op.attrs["slots"]
-        if grads is not None:
-            for v in slots:                       # (a plan's tensors stay: the gradients go to the slab)
-                if v.op_name in grads:
-                    self.layout.view(self.grad, v.op_name).copy_(grads.pop(v.op_name))
-                else:
-                    self.layout.view(self.grad, v.op_name).zero_()
+        for v in slots:                           # (a plan's tensors stay: the gradients go to the slab)
+            own, g = self.layout.view(self.grad, v.op_name), grads.pop(v.op_name, None)
+            if g is None:
+                own.zero_()
+            elif g.data_ptr() != own.data_ptr():
+                own.copy_(g)
         triples = [(self._var_view(v), self.layout.view(self.grad, v.op_name), self._var_view(s)) for v, s in slots.items()]
         if not triples:
             return
@@ -964,8 +967,6 @@ class Session:
         else:
             for w, g, buf in triples:
                 reference_op.muon_step(w, g, buf, opt.learning_rate, opt.momentum, opt.use_nesterov)
-        for _, g, _ in triples:
-            g.zero_()
 
     def _stats_to_host(self, stats: torch.Tensor) -> torch.Tensor:
         """The two statistics of a fused step on the host; waits for the step."""

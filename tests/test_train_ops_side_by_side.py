@@ -1,0 +1,66 @@
+"""Several train ops in one session: a step of one leaves alone what the others train.  (CPU sessions here, the same on a GPU with
+``-m gpu``.)"""
+import numpy as np
+import pytest
+import torch
+
+import distributed_tensorflow_amd as tf
+
+
+def stack(widths, batch=16):
+    """A graph that the engines recognise: placeholders, variables, loss and a feed for them."""
+    rng = np.random.RandomState(5)
+    x, y = tf.placeholder(tf.float32, [None, widths[0]]), tf.placeholder(tf.float32, [None, widths[-1]])
+    w = [tf.Variable(tf.random_normal([a, b], stddev=a ** -0.5), name=f"w{k}") for k, (a, b) in enumerate(zip(widths, widths[1:]))]
+    b = [tf.Variable(tf.zeros([m]), name=f"b{k}") for k, m in enumerate(widths[1:])]
+    h = x
+    for k in range(len(w)):
+        h = tf.add(tf.matmul(h, w[k]), b[k])
+        h = tf.nn.relu(h) if k + 1 < len(w) else h
+    loss = tf.reduce_mean(tf.nn.softmax_cross_entropy_with_logits(labels=y, logits=h))
+    feed = {x: rng.rand(batch, widths[0]).astype(np.float32),
+            y: np.eye(widths[-1], dtype=np.float32)[rng.randint(0, widths[-1], batch)]}
+    return w, b, loss, feed
+
+
+def _engine_step_beside_another_op(make, widths):
+    """An engine's gradient pass writes its own slices of the gradient slab: what an earlier step of another op left next to them
+    must not be applied again."""
+    with tf.Graph().as_default():
+        w, b, loss, feed = stack(widths)
+        other = tf.Variable(tf.zeros([5, 3]), name="other")
+        pull = tf.reduce_sum(tf.square(tf.subtract(other, tf.constant(np.ones((5, 3), np.float32)))))
+        step = tf.train.get_or_create_global_step()
+        aside = tf.train.GradientDescentOptimizer(0.1).minimize(pull, var_list=[other])
+        train = make().minimize(loss, global_step=step, var_list=w + b)
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            for k in range(3):
+                sess.run(aside)
+                kept = sess.var_tensor(other).clone()
+                before = [sess.var_tensor(v).clone() for v in w + b]
+                sess.run(train, feed_dict=feed)
+                sess.run([train, loss], feed_dict=feed)
+                assert torch.equal(sess.var_tensor(other), kept), k
+                assert not any(torch.equal(sess.var_tensor(v), p) for v, p in zip(w + b, before))
+                assert sess.run(step) == 2 * (k + 1)
+            # 1 - (1 - 2 * 0.1)^3 of the way, in three fp32 steps
+            assert float((sess.var_tensor(other).cpu().double() - (1 - 0.8 ** 3)).abs().max()) < 1e-6
+            assert sess.fused_steps == 6
+
+
+MAKERS = {"muon": lambda: tf.train.MuonOptimizer(0.1, sgd_learning_rate=0.3), "sgd": lambda: tf.train.GradientDescentOptimizer(0.3)}
+
+
+@pytest.mark.parametrize("kind", sorted(MAKERS))
+@pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
+def test_engine_step_beside_another_op_on_the_cpu(kind, widths):
+    with tf.device("/cpu:0"):
+        _engine_step_beside_another_op(MAKERS[kind], widths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(MAKERS))
+@pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
+def test_engine_step_beside_another_op_on_the_gpu(kind, widths):
+    _engine_step_beside_another_op(MAKERS[kind], widths)
