@@ -339,6 +339,7 @@ class PsDenseResidentTrainer:
         capturable = (self.device.type == "cuda" and not self.use_locking
                       and type(self.store).__name__ in ("IpcVariableStore", "LocalVariableStore"))
         self.use_graph = bool(use_graph) and capturable
+        sess.own_gradients(train_op)
         self.params, self.grads = sess.theta, sess.grad
         view = lambda slab, v: None if v is None else sess.layout.view(slab, v.op_name)  # noqa: E731
         self.engine = DenseStackEngine([view(self.params, W) for W, _ in d["layers"]],

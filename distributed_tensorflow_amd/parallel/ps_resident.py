@@ -59,6 +59,7 @@ class PsResidentTrainer(_BaseTrainer):
                       and not self.use_locking)
         self.use_graph = bool(use_graph) and capturable
         self.layout = sess.layout
+        sess.own_gradients(train_op)
         self.params, self.grads = sess.theta, sess.grad
         names = {r: m[r].op_name for r in ("W1", "b1", "W2", "b2")}
         self.engine = MLPEngine({r: self.layout.view(self.params, n) for r, n in names.items()},

@@ -211,6 +211,7 @@ class Session:
             self.store = LocalVariableStore(self.layout, self.device)
             self.theta = self.store.bind_local()
         self.grad = self.layout.new_slab(self.device)
+        self._grad_of = None                      # the train op whose gradients lie in it
         self._engines: Dict[Any, MLPEngine] = {}
         self._plans: Dict[int, Any] = {}          # train op -> what runs it (fused model, dense stack, accuracy nodes)
         self._reads_vars: Dict[Any, bool] = {}    # node -> whether evaluating it reads variables
@@ -793,6 +794,13 @@ class Session:
             return all(self._served_by_step(i, m, plan, _depth + 1) for i in f.inputs)
         return False
 
+    def own_gradients(self, train_op):
+        """Clears the gradient slab unless what lies in it are gradients of this train op.  A push applies the whole slab, and an
+        engine writes the gradients of its own variables alone: those that another op has left would be applied again."""
+        if self._grad_of is not train_op:
+            self.grad.zero_()
+            self._grad_of = train_op
+
     def _run_train(self, train_op, feed, cache):
         opt: Optimizer = train_op.attrs["optimizer"]
         plan = self._plan(train_op)
@@ -830,6 +838,7 @@ class Session:
                     applied = "pushed"
                     self.pushed_steps += 1
                 else:
+                    self.own_gradients(train_op)
                     eng.step_grad(0, 1.0)
             with span("fetch_stats"):
                 # the step's only wait for the device
@@ -856,6 +865,7 @@ class Session:
                     eng.step_fused(0)
                     applied = True
                 else:
+                    self.own_gradients(train_op)
                     eng.step_grad(0, 1.0)
             with span("fetch_stats"):
                 host = self._stats_to_host(torch.stack((eng.loss_sum[0], eng.correct[0].to(torch.float32)))) / float(eng.B)
@@ -887,7 +897,8 @@ class Session:
                 cache[k] = val.detach() if isinstance(val, torch.Tensor) else val
             self.generic_steps += 1
         else:
-            self.grad.zero_()
+            self._grad_of = None                  # (also what an earlier step of this op has left)
+            self.own_gradients(train_op)
             var_list = train_op.attrs["var_list"]
             leaves = {v: self._var_view(v).detach().clone().requires_grad_(True) for v in var_list}
             fcache: Dict[G.Tensor, Any] = {}
@@ -912,7 +923,7 @@ class Session:
             return
         if not plain:
             if sparse_grads is None:
-                # (of the op's own variables alone: elsewhere in the slab may lie what another train op has left)
+                # (of the op's own variables alone: the momenta and the other variables are not read or written)
                 sparse_grads = {v.op_name: self.layout.view(self.grad, v.op_name) for v in train_op.attrs["var_list"]}
             with span("muon"):
                 self._muon_update(train_op, opt, sparse_grads)
@@ -945,6 +956,7 @@ class Session:
         """The matrices of a train op: momentum, orthogonalised direction, weights, all in place.  ``grads`` by name; what is left in
         it afterwards is for plain gradient descent."""
         slots = train_op.attrs["slots"]
+        self.own_gradients(train_op)
         for v in slots:                           # (a plan's tensors stay: the gradients go to the slab)
             own, g = self.layout.view(self.grad, v.op_name), grads.pop(v.op_name, None)
             if g is None:

@@ -64,3 +64,50 @@ def test_engine_step_beside_another_op_on_the_cpu(kind, widths):
 @pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
 def test_engine_step_beside_another_op_on_the_gpu(kind, widths):
     _engine_step_beside_another_op(MAKERS[kind], widths)
+
+
+@pytest.mark.parametrize("resident", [False, True])
+@pytest.mark.parametrize("widths", [(20, 30, 6), (20, 30, 24, 6)])
+def test_engine_step_beside_another_op_on_a_parameter_server(widths, resident):
+    """The same over TCP, where every step pushes the gradient slab: through ``sess.run``, and by the device-resident trainers."""
+    from cluster_utils import cluster_dict
+
+    from distributed_tensorflow_amd.data import DeviceDataset
+    from distributed_tensorflow_amd.parallel.dense_trainer import PsDenseResidentTrainer
+    from distributed_tensorflow_amd.parallel.ps_resident import PsResidentTrainer
+
+    cluster = tf.train.ClusterSpec(cluster_dict(1, 1))
+    cfg = tf.ConfigProto(allow_soft_placement=True, operation_timeout_in_ms=20000)
+    ps, worker = tf.train.Server(cluster, "ps", 0, config=cfg), tf.train.Server(cluster, "worker", 0, config=cfg)
+    try:
+        g = tf.Graph()
+        with g.as_default(), tf.device(tf.train.replica_device_setter(worker_device="/job:worker/task:0/cpu:0", cluster=cluster)):
+            w, b, loss, feed = stack(widths)
+            other = tf.Variable(tf.zeros([5, 3]), name="other")
+            pull = tf.reduce_sum(tf.square(tf.subtract(other, tf.constant(np.ones((5, 3), np.float32)))))
+            step = tf.train.get_or_create_global_step()
+            aside = tf.train.GradientDescentOptimizer(0.1).minimize(pull, var_list=[other])
+            train = tf.train.GradientDescentOptimizer(0.3).minimize(loss, global_step=step, var_list=w + b)
+            init = tf.global_variables_initializer()
+        sv = tf.train.Supervisor(graph=g, is_chief=True, global_step=step, init_op=init)
+        sess = sv.prepare_or_wait_for_session(worker.target)
+        sess.run(aside)
+        kept, before = sess.run(other).copy(), sess.run(w[0]).copy()       # (a CPU session hands out its memory)
+        if resident:
+            ds = DeviceDataset(*feed.values(), sess.device, 8, seed=3)
+            trainer = (PsResidentTrainer if len(widths) == 3 else PsDenseResidentTrainer)(sess, train, ds, 8)
+            trainer.run_steps(2)
+        else:
+            sess.run(train, feed_dict=feed)
+            sess.run([train, loss], feed_dict=feed)
+        assert np.array_equal(sess.run(other), kept)
+        after = sess.run(w[0]).copy()
+        assert not np.array_equal(after, before)
+        sess.run(aside)
+        assert np.array_equal(sess.run(w[0]), after) and abs(float(sess.run(other)[0, 0]) - 0.36) < 1e-6
+        assert sess.run(step) == 2
+        sv.stop()
+        sess.close()
+    finally:
+        worker.stop()
+        ps.stop()
