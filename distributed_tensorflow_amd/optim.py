@@ -128,6 +128,13 @@ class MuonOptimizer(Optimizer):
         return op
 
 
+def refuse_muon(train_op: G.Tensor, trainer: str) -> None:
+    """For trainers whose steps are ``p -= lr * g`` for every variable."""
+    if isinstance(train_op.attrs["optimizer"], MuonOptimizer):
+        raise NotImplementedError(f"{trainer}: plain gradient descent only; run a MuonOptimizer train op through sess.run of a "
+                                  "local session")
+
+
 class QueueRunner:
     """The chief's aggregation loop, runnable on a thread (``Supervisor.start_queue_runners``)."""
 

@@ -21,6 +21,9 @@ class DenseResidentTrainer:
     name = "dense"
 
     def __init__(self, sess, train_op, dataset, batch: int, chunk: int = 50, use_graph: bool = True):
+        from ..optim import refuse_muon
+
+        refuse_muon(train_op, type(self).__name__)
         if sess.store.is_remote:
             raise ValueError("the resident dense trainer runs against a local session (no parameter-server tasks)")
         plan = sess._plan(train_op)
@@ -325,6 +328,9 @@ class PsDenseResidentTrainer:
     name = "ps-dense-resident"
 
     def __init__(self, sess, train_op, dataset, batch: int, chunk: int = 50, use_graph: bool = True):
+        from ..optim import refuse_muon
+
+        refuse_muon(train_op, type(self).__name__)
         plan = sess._plan(train_op)
         d = plan.get("dense")
         if d is None:

@@ -42,6 +42,9 @@ class PsResidentTrainer(_BaseTrainer):
 
     def __init__(self, sess, train_op, dataset, batch: int, chunk: int = 50, use_graph: bool = True,
                  fused_push="auto"):
+        from ..optim import refuse_muon
+
+        refuse_muon(train_op, type(self).__name__)
         plan = sess._plan(train_op)
         m = plan["mlp"]
         if m is None:

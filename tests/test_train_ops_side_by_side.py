@@ -111,3 +111,45 @@ def test_engine_step_beside_another_op_on_a_parameter_server(widths, resident):
     finally:
         worker.stop()
         ps.stop()
+
+
+def test_resident_trainers_refuse_muon():
+    """Their steps are plain gradient descent: a MuonOptimizer op must not be trained with it instead."""
+    from cluster_utils import cluster_dict
+
+    from distributed_tensorflow_amd.data import DeviceDataset
+    from distributed_tensorflow_amd.parallel.dense_trainer import DenseResidentTrainer, PsDenseResidentTrainer
+    from distributed_tensorflow_amd.parallel.ps_resident import PsResidentTrainer
+
+    for widths in ((20, 30, 6), (20, 30, 24, 6)):
+        with tf.Graph().as_default(), tf.device("/cpu:0"):
+            w, b, loss, feed = stack(widths)
+            train = tf.train.MuonOptimizer(0.1).minimize(loss, global_step=tf.train.get_or_create_global_step())
+            with tf.Session() as sess:
+                sess.run(tf.global_variables_initializer())
+                ds = DeviceDataset(*feed.values(), sess.device, 8, seed=3)
+                start = sess.theta.clone()
+                for trainer in (DenseResidentTrainer, PsDenseResidentTrainer, PsResidentTrainer):
+                    with pytest.raises(NotImplementedError):
+                        trainer(sess, train, ds, 8)
+                assert torch.equal(sess.theta, start)
+    cluster = tf.train.ClusterSpec(cluster_dict(1, 1))
+    cfg = tf.ConfigProto(allow_soft_placement=True, operation_timeout_in_ms=20000)
+    ps, worker = tf.train.Server(cluster, "ps", 0, config=cfg), tf.train.Server(cluster, "worker", 0, config=cfg)
+    try:
+        g = tf.Graph()
+        with g.as_default(), tf.device(tf.train.replica_device_setter(worker_device="/job:worker/task:0/cpu:0", cluster=cluster)):
+            w, b, loss, feed = stack((20, 30, 24, 6))
+            step = tf.train.get_or_create_global_step()
+            train = tf.train.MuonOptimizer(0.1).minimize(loss, global_step=step)
+            init = tf.global_variables_initializer()
+        sv = tf.train.Supervisor(graph=g, is_chief=True, global_step=step, init_op=init)
+        sess = sv.prepare_or_wait_for_session(worker.target)
+        with pytest.raises(NotImplementedError):
+            PsDenseResidentTrainer(sess, train, DeviceDataset(*feed.values(), sess.device, 8, seed=3), 8)
+        assert sess.run(step) == 0
+        sv.stop()
+        sess.close()
+    finally:
+        worker.stop()
+        ps.stop()
