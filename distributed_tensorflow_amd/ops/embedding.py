@@ -130,7 +130,7 @@ class _Lookup(torch.autograd.Function):
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * table[ids]`` with the gradient of the table (GPU: the kernels above; CPU tensors: torch, same rules)."""
     if table.is_cuda:
-        return _Lookup.apply(table, ids, float(scale))
+        return _Lookup.apply(hb.with_rows(table), ids, float(scale))
     inside = (ids >= 0) & (ids < table.shape[0])
     rows = torch.nn.functional.embedding(torch.where(inside, ids, torch.zeros_like(ids)).long(), table) * scale
     return torch.where(inside.unsqueeze(-1), rows, torch.zeros_like(rows))

@@ -315,6 +315,15 @@ def typed_rows(t: torch.Tensor, name: str) -> int:
     return t.stride(0) if rows > 1 else max(cols, 1)
 
 
+def with_rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D operand as ``typed_rows`` takes it: itself, or a copy where its rows are not contiguous (a transposed table) or
+    overlap (expanded logits).  Differentiable; for the operators that are, the launches behind them refuse such operands."""
+    if t.dim() != 2 or t.is_contiguous():
+        return t
+    rows, cols = t.shape
+    return t.contiguous() if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols else t
+
+
 def int_vector(t: torch.Tensor, name: str, device) -> torch.Tensor:
     """``t`` (int32 or int64, any shape, on ``device``) as a contiguous vector."""
     if t.dtype not in (torch.int32, torch.int64) or t.device != device:

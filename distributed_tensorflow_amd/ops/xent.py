@@ -85,8 +85,7 @@ class _SparseXent(torch.autograd.Function):
 def sparse_softmax_xent(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     """Loss of every row, differentiable in the logits (GPU: the kernels above; CPU tensors: torch, same rules)."""
     if logits.is_cuda:
-        rows = logits if logits.dim() != 2 or logits.shape[1] == 1 or logits.stride(1) == 1 else logits.contiguous()
-        return _SparseXent.apply(rows, labels)
+        return _SparseXent.apply(hb.with_rows(logits), labels)
     if logits.dim() != 2 or labels.dim() != 1 or labels.shape[0] != logits.shape[0]:
         raise ValueError("sparse_softmax_xent: one label per row of 2-D logits")
     classes = logits.shape[1]
