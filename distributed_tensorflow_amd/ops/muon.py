@@ -47,7 +47,8 @@ def orthogonalize(x: torch.Tensor, eps: float = EPS, out: Optional[torch.Tensor]
 class MuonPlan:
     """A fixed list of float32 matrices ``[in, out]`` with their gradients and momentum buffers, and the workspace their steps use.
     The steps read and write the memory that the tensors have when the plan is made (and keep it alive): write new gradients
-    into the same tensors.  One step of a plan at a time: two streams, or two captured graphs that may overlap, need a plan each."""
+    into the same tensors.  One step of a plan at a time: two streams, or two captured graphs that may overlap, need a plan each.
+    A plan may be dropped while a step is under way on any stream; one whose steps a graph has captured has to outlive the graph."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]):
         params, grads, momenta = list(params), list(grads), list(momenta)
@@ -67,6 +68,7 @@ class MuonPlan:
         self.params, self.grads, self.momenta = ([t.detach() for t in ts] for ts in (params, grads, momenta))
         self.device = params[0].device
         self._groups = []
+        self._streams = {hb._stream(params[0])}         # whose work the allocator waits for before it gives the memory away
         for i in range(0, len(params), GROUP):
             ws, gs, bs = params[i:i + GROUP], grads[i:i + GROUP], momenta[i:i + GROUP]
             n = len(ws)
@@ -82,6 +84,11 @@ def muon_step(plan: MuonPlan, lr: torch.Tensor, *, momentum: float = 0.95, neste
     if hb._f32c(lr, "lr").numel() != 1 or lr.device != plan.device:
         raise hb.HipKernelError("muon_step: lr is one float32 on the plan's device")
     stream = hb._stream(lr)
+    if stream not in plan._streams:
+        side = torch.cuda.current_stream(plan.device)
+        for t in (*plan.params, *plan.grads, *plan.momenta, *[group[-1] for group in plan._groups]):
+            t.record_stream(side)
+        plan._streams.add(stream)
     for n, rows, cols, w, g, b, ws in plan._groups:
         hb._check(lib.dtf_muon_step(n, rows, cols, w, g, b, lr.data_ptr(), float(momentum), int(bool(nesterov)), float(eps),
                                     ws.data_ptr(), ws.numel(), stream), "dtf_muon_step")
