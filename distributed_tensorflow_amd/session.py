@@ -586,7 +586,11 @@ class Session:
         elif op == "gradient":
             loss, var = ins[0], node.attrs["wrt"]
             leaf = self._var_view(var).detach().clone().requires_grad_(True)
-            val = self._eval(loss, feed, {}, {var: leaf})
+            during, self._lookups = self._lookups, None       # (inside a loss: this gradient is the variable's, not its rows')
+            try:
+                val = self._eval(loss, feed, {}, {var: leaf})
+            finally:
+                self._lookups = during
             (r,) = torch.autograd.grad(val, [leaf], allow_unused=True)
             if r is None:
                 r = torch.zeros_like(leaf)

@@ -153,3 +153,37 @@ def test_resident_trainers_refuse_muon():
     finally:
         worker.stop()
         ps.stop()
+
+
+def _gradient_of_a_table_inside_a_loss():
+    """A loss that holds the gradient of another one: while the train op looks rows up as leaves, that gradient is still the
+    table's."""
+    with tf.Graph().as_default():
+        ids = tf.placeholder(tf.int64, [None])
+        table = tf.Variable(tf.random_normal([5, 3]), name="table")
+        inner = tf.reduce_sum(tf.square(tf.nn.embedding_lookup(table, ids)))
+        opt = tf.train.GradientDescentOptimizer(0.1)
+        (g, _), = opt.compute_gradients(inner, [table])
+        loss = tf.add(tf.reduce_sum(tf.nn.embedding_lookup(table, ids)), tf.reduce_sum(tf.square(g)))
+        train = opt.minimize(loss)
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            start = sess.var_tensor(table).cpu().double().clone()
+            count = torch.tensor([0.0, 2.0, 0.0, 1.0, 0.0]).double()[:, None]
+            want = float((count * start).sum() + (2 * count * start).square().sum())
+            feed = {ids: np.array([1, 3, 1])}
+            assert abs(sess.run(loss, feed_dict=feed) - want) < 1e-5 * abs(want) + 1e-5
+            _, got = sess.run([train, loss], feed_dict=feed)
+            assert abs(got - want) < 1e-5 * abs(want) + 1e-5
+            # (a gradient is a constant of the step: the sum of the rows alone moves them)
+            assert float((sess.var_tensor(table).cpu().double() - (start - 0.1 * count)).abs().max()) < 1e-6
+
+
+def test_gradient_of_a_table_inside_a_loss_on_the_cpu():
+    with tf.device("/cpu:0"):
+        _gradient_of_a_table_inside_a_loss()
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_table_inside_a_loss_on_the_gpu():
+    _gradient_of_a_table_inside_a_loss()
