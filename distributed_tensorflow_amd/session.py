@@ -815,6 +815,7 @@ class Session:
         if not plain and self.store.is_remote:
             raise NotImplementedError("MuonOptimizer: variables on parameter servers take plain gradient descent; use a local session")
         sparse_grads = None
+        without = set()          # variables that the loss does not depend on
         applied = False
         if m is not None and m["x"] in feed:
             xv = feed[m["x"]]
@@ -912,6 +913,8 @@ class Session:
             for v, g in zip(var_list, grads):
                 if g is not None:
                     self.layout.view(self.grad, v.op_name).copy_(g)
+                else:
+                    without.add(v)
             for k, val in fcache.items():   # forward values seen by the other fetches
                 cache[k] = val.detach() if isinstance(val, torch.Tensor) else val
             self.generic_steps += 1
@@ -928,7 +931,8 @@ class Session:
         if not plain:
             if sparse_grads is None:
                 # (of the op's own variables alone: the momenta and the other variables are not read or written)
-                sparse_grads = {v.op_name: self.layout.view(self.grad, v.op_name) for v in train_op.attrs["var_list"]}
+                sparse_grads = {v.op_name: self.layout.view(self.grad, v.op_name) for v in train_op.attrs["var_list"]
+                                if v not in without}
             with span("muon"):
                 self._muon_update(train_op, opt, sparse_grads)
         if sparse_grads is not None:
@@ -959,19 +963,17 @@ class Session:
     def _muon_update(self, train_op, opt: MuonOptimizer, grads: Dict[str, torch.Tensor]):
         """The matrices of a train op: momentum, orthogonalised direction, weights, all in place.  ``grads`` by name; what is left in
         it afterwards is for plain gradient descent."""
-        slots = train_op.attrs["slots"]
+        slots = {v: s for v, s in train_op.attrs["slots"].items() if v.op_name in grads}     # (the others rest, their momenta too)
         self.own_gradients(train_op)
         for v in slots:                           # (a plan's tensors stay: the gradients go to the slab)
-            own, g = self.layout.view(self.grad, v.op_name), grads.pop(v.op_name, None)
-            if g is None:
-                own.zero_()
-            elif g.data_ptr() != own.data_ptr():
+            own, g = self.layout.view(self.grad, v.op_name), grads.pop(v.op_name)
+            if g.data_ptr() != own.data_ptr():
                 own.copy_(g)
         triples = [(self._var_view(v), self.layout.view(self.grad, v.op_name), self._var_view(s)) for v, s in slots.items()]
         if not triples:
             return
         if self.device.type == "cuda":
-            key = ("muon", id(train_op))
+            key = ("muon", id(train_op), *slots)
             plan = self._engines.get(key)
             if plan is None:
                 plan = self._engines[key] = muon_op.MuonPlan(*zip(*triples))

@@ -187,3 +187,41 @@ def test_gradient_of_a_table_inside_a_loss_on_the_cpu():
 @pytest.mark.gpu
 def test_gradient_of_a_table_inside_a_loss_on_the_gpu():
     _gradient_of_a_table_inside_a_loss()
+
+
+def _muon_leaves_alone_what_its_loss_does_not_read(with_table):
+    """A matrix in the var_list of a train op whose loss does not depend on it has no gradient: neither it nor its momentum moves,
+    also when another op has left that momentum behind."""
+    with tf.Graph().as_default():
+        ids = tf.placeholder(tf.int64, [None])
+        x = tf.constant(np.random.RandomState(1).rand(7, 8).astype(np.float32))
+        read = tf.nn.embedding_lookup(tf.Variable(tf.random_normal([9, 8]), name="table"), ids) if with_table else x
+        w = [tf.Variable(tf.random_normal([8, 5]), name=f"w{k}") for k in range(2)]
+        losses = [tf.reduce_mean(tf.square(tf.matmul(r, v))) for r, v in zip((x, read), w)]
+        opt = tf.train.MuonOptimizer(0.1)
+        first = opt.minimize(losses[0], var_list=w[:1])
+        both = opt.minimize(losses[1])                  # every trainable variable, w[0] among them
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            sess.run(first)
+            slot = next(v for v in tf.global_variables() if v.op_name == "w0/Muon")
+            start = [sess.var_tensor(v).clone() for v in (w[0], slot, w[1])]
+            assert float(start[1].abs().max()) > 0
+            for _ in range(2):
+                sess.run(both, feed_dict={ids: np.array([1, 2, 2])})
+            now = [sess.var_tensor(v) for v in (w[0], slot, w[1])]
+            assert torch.equal(now[0], start[0]) and torch.equal(now[1], start[1]) and not torch.equal(now[2], start[2])
+            sess.run(first)
+            assert not torch.equal(sess.var_tensor(w[0]), start[0])
+
+
+@pytest.mark.parametrize("with_table", [False, True])
+def test_muon_leaves_alone_what_its_loss_does_not_read_on_the_cpu(with_table):
+    with tf.device("/cpu:0"):
+        _muon_leaves_alone_what_its_loss_does_not_read(with_table)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_table", [False, True])
+def test_muon_leaves_alone_what_its_loss_does_not_read_on_the_gpu(with_table):
+    _muon_leaves_alone_what_its_loss_does_not_read(with_table)
