@@ -4,7 +4,7 @@ labels of ``hip_backend.softmax_xent`` would be a matrix as large as the logits.
 ``sparse_softmax_xent(logits, labels)`` is the differentiable operator: the loss of every row
 (``tf.nn.sparse_softmax_cross_entropy_with_logits`` of a graph evaluates to it).  ``sparse_softmax_xent_step`` is the training
 step's form: losses and gradient in ONE launch that reads the logits once and keeps each row in registers in between (two
-launches for up to 64 rows of more than 256 KB).
+launches for up to 64 rows of more than 256 KB, one for every 2^21 rows).
 
 A negative label is padding: loss 0, a gradient row of zeros, the row's logits are not looked at.  A label that is no class
 (``>= classes``) gives NaN.  Logits in float32, bfloat16 or float16 with contiguous rows; losses in float32.
@@ -35,13 +35,16 @@ def _dz_rows(dz: torch.Tensor, logits: torch.Tensor) -> int:
     return hb.typed_rows(dz, "dz")
 
 
-def _forward(logits, labels, dz, grad_scale, stats):
-    lib = hb.require()
-    ld, flat = _operands(logits, labels)
-    ldz = 0 if dz is None else _dz_rows(dz, logits)
+LAUNCH_ROWS = 1 << 21        # of one native call
+
+
+def _parts(rows: int):
+    return [slice(a, min(a + LAUNCH_ROWS, rows)) for a in range(0, rows, LAUNCH_ROWS)]
+
+
+def _launch(lib, logits, ld, flat, dz, ldz, grad_scale, loss, stats):
     rows, classes = logits.shape
     code = hb.TYPE_CODES[logits.dtype]
-    loss = torch.empty((rows,), device=logits.device, dtype=torch.float32)
     args = (logits.data_ptr(), code, rows, classes, ld, flat.data_ptr(), int(flat.dtype == torch.int64), hb._ptr(dz), ldz,
             float(grad_scale), loss.data_ptr(), hb._ptr(stats))
     # few long rows: several blocks each, which need a workspace
@@ -51,6 +54,19 @@ def _forward(logits, labels, dz, grad_scale, stats):
         hb._check(lib.dtf_sparse_xent_cut(*args, ws.data_ptr(), need, hb._stream(logits)), "dtf_sparse_xent_cut")
     else:
         hb._check(lib.dtf_sparse_xent(*args, hb._stream(logits)), "dtf_sparse_xent")
+
+
+def _forward(logits, labels, dz, grad_scale, stats):
+    lib = hb.require()
+    ld, flat = _operands(logits, labels)
+    ldz = 0 if dz is None else _dz_rows(dz, logits)
+    loss = torch.empty((logits.shape[0],), device=logits.device, dtype=torch.float32)
+    if logits.shape[0] <= LAUNCH_ROWS:
+        _launch(lib, logits, ld, flat, dz, ldz, grad_scale, loss, stats)
+    else:
+        for r in _parts(logits.shape[0]):
+            _launch(lib, logits[r], ld, flat[r], None if dz is None else dz[r], ldz, grad_scale, loss[r],
+                    None if stats is None else stats[r])
     return loss, flat
 
 
@@ -75,10 +91,12 @@ class _SparseXent(torch.autograd.Function):
         z, flat, stats = ctx.saved_tensors
         g = g.to(torch.float32)
         dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
-        hb._check(hb.require().dtf_sparse_xent_grad(z.data_ptr(), hb.TYPE_CODES[z.dtype], z.shape[0], z.shape[1],
-                                                    hb.typed_rows(z, "logits"), flat.data_ptr(), int(flat.dtype == torch.int64),
-                                                    stats.data_ptr(), g.data_ptr(), g.stride(0), dz.data_ptr(), z.shape[1],
-                                                    hb._stream(z)), "dtf_sparse_xent_grad")
+        lib, ld = hb.require(), hb.typed_rows(z, "logits")
+        whole = (z, flat, stats, g, dz)
+        for z, flat, stats, g, to in [whole] if dz.shape[0] <= LAUNCH_ROWS else [[t[r] for t in whole] for r in _parts(dz.shape[0])]:
+            hb._check(lib.dtf_sparse_xent_grad(z.data_ptr(), hb.TYPE_CODES[z.dtype], z.shape[0], z.shape[1], ld, flat.data_ptr(),
+                                               int(flat.dtype == torch.int64), stats.data_ptr(), g.data_ptr(), g.stride(0),
+                                               to.data_ptr(), z.shape[1], hb._stream(z)), "dtf_sparse_xent_grad")
         return dz, None
 
 
