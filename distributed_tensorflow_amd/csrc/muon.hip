@@ -879,7 +879,7 @@ int64_t tiles_of(const Call& c, int i, int stage, int edge) {
   return stage <= kPoly ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut)
+thread_local int g_force_edge = 0, g_force_splits = 0;      // tuning (dtf_debug_set_muon_cut): of the calling thread's calls
 
 // The cheapest cut by an estimate in microseconds.  By tile edge: a k-step with few and with all CUs at work (a full chip runs
 // into its power limit: 1.3 PFLOP/s of fp16 products at 1.4 to 1.6 GHz, where a lone workgroup does a step at 96 % of the matrix
@@ -1080,7 +1080,7 @@ extern "C" int dtf_muon_step(int count, const int32_t* rows, const int32_t* cols
   return run<float>(c, l, (hipStream_t)stream);
 }
 
-// Tuning and tests: products of the next calls in tiles of this edge (32, 64, 128, 192, 256) with this many parts of k where k is long
+// Tuning and tests: products of this thread's next calls in tiles of this edge (32, 64, 128, 192, 256) with this many parts of k where k is long
 // enough; 0: chosen from the shapes.  (The workspace of a plan has to be made under the same setting.)
 extern "C" void dtf_debug_set_muon_cut(int edge, int splits) {
   g_force_edge = edge == 32 || edge == 64 || edge == 128 || edge == 192 || edge == 256 ? edge : 0;
