@@ -25,8 +25,8 @@
 // bytes, one cache line per row and k-step.  Dimensions are padded with zeros to whole tiles: the products need no bounds.
 //
 // GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 (or 32, see Narrow) and walks k in steps of 32 through a
-// ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 130 to 140 KB, one workgroup per CU, the loads of a step requested one
-// to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away, against 0.1 to 1.8 us of products per
+// ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 148, 132, 144 or 128 KB (ring_bytes()), one workgroup per CU, the
+// loads of a step requested one to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away, against 0.1 to 1.8 us of products per
 // step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so the 16-byte chunks of a row are
 // permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the sixteen rows that a quarter of a fragment
 // read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
@@ -508,6 +508,12 @@ __device__ __forceinline__ void tile_place(const Task& task, int edge, int t, in
 
 constexpr int ring_of(int tile) { return tile == 256 ? 2 : tile == 192 ? 3 : tile == 128 ? 4 : 8; }
 constexpr int kTurn = kWaves * kTurnWords * 4;      // all waves' turning areas, in bytes
+
+constexpr int ring_bytes(int tile) {                // (image 0 becomes the turning areas, and is as large as those)
+  return (2 * tile * 128 < kTurn ? kTurn : 2 * tile * 128) + (ring_of(tile) - 1) * 2 * tile * 128;
+}
+static_assert(ring_bytes(64) == 148 << 10 && ring_bytes(128) == 132 << 10 && ring_bytes(192) == 144 << 10 && ring_bytes(256) == 128 << 10,
+              "a CU has 160 KB");
 
 // LDS image I of the ring: the rows of one operand, then the other's.  (One variable each: the compiler must see that a load to
 // one image does not concern the reads of another.)
