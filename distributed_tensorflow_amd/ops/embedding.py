@@ -53,6 +53,8 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, out: Opti
     hb._check(lib.dtf_embed_lookup(table.data_ptr(), hb.TYPE_CODES[table.dtype], rows, dim, ld, flat.data_ptr(),
                                    int(flat.dtype == torch.int64), flat.numel(), float(scale), dst.data_ptr(), ldo,
                                    hb._stream(table)), "dtf_embed_lookup")
+    if out is not None:
+        hb.written(out)
     return dst
 
 
@@ -80,6 +82,7 @@ def lookup_grad(ids: torch.Tensor, grad: torch.Tensor, rows: int, scale: float =
     hb._check(lib.dtf_embed_grad(flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(), g.data_ptr(), ldg, out.data_ptr(),
                                  hb.TYPE_CODES[g.dtype], rows, dim, ldt, float(scale), ws.data_ptr(), ws.numel(),
                                  hb._stream(g)), "dtf_embed_grad")
+    hb.written(out)
     return out
 
 
@@ -101,6 +104,7 @@ def lookup_sgd(table: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, lr: t
     hb._check(lib.dtf_embed_sgd(flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(), g.data_ptr(), ldg, table.data_ptr(),
                                 hb.TYPE_CODES[table.dtype], table.shape[0], table.shape[1], ldt, float(scale), lr.data_ptr(),
                                 ws.data_ptr(), ws.numel(), hb._stream(table)), "dtf_embed_sgd")
+    hb.written(table)
     return table
 
 

@@ -315,6 +315,11 @@ def typed_rows(t: torch.Tensor, name: str) -> int:
     return t.stride(0) if rows > 1 else max(cols, 1)
 
 
+# Tells autograd that tensors were written in place: a launch does not, and a backward pass that saved one of them would use the
+# new values without a word.
+written = torch.autograd.graph.increment_version
+
+
 def with_rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D operand as ``typed_rows`` takes it: itself, or a copy where its rows are not contiguous (a transposed table) or
     overlap (expanded logits).  Differentiable; for the operators that are, the launches behind them refuse such operands."""

@@ -41,6 +41,7 @@ def orthogonalize(x: torch.Tensor, eps: float = EPS, out: Optional[torch.Tensor]
     ws = _workspace(lib, [x.shape], x.device)
     hb._check(lib.dtf_orthogonalize(x.data_ptr(), hb.TYPE_CODES[x.dtype], x.shape[0], x.shape[1], ldx, out.data_ptr(), ldo,
                                     float(eps), ws.data_ptr(), ws.numel(), hb._stream(x)), "dtf_orthogonalize")
+    hb.written(out)
     return out
 
 
@@ -92,3 +93,4 @@ def muon_step(plan: MuonPlan, lr: torch.Tensor, *, momentum: float = 0.95, neste
     for n, rows, cols, w, g, b, ws in plan._groups:
         hb._check(lib.dtf_muon_step(n, rows, cols, w, g, b, lr.data_ptr(), float(momentum), int(bool(nesterov)), float(eps),
                                     ws.data_ptr(), ws.numel(), stream), "dtf_muon_step")
+    hb.written(plan.params + plan.momenta)

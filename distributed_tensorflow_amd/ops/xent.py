@@ -74,7 +74,10 @@ def sparse_softmax_xent_step(logits: torch.Tensor, labels: torch.Tensor, *, dz: 
                              grad_scale: float = 1.0) -> torch.Tensor:
     """Row losses (float32 ``[rows]``); ``dz`` (shaped like the logits, or the logits themselves) receives
     ``grad_scale * d(row loss)/d(logits)`` in the same launch."""
-    return _forward(logits, labels, dz, grad_scale, None)[0]
+    loss = _forward(logits, labels, dz, grad_scale, None)[0]
+    if dz is not None:
+        hb.written(dz)
+    return loss
 
 
 class _SparseXent(torch.autograd.Function):
