@@ -12,22 +12,25 @@
 // Bound by the matrix cores: 5 (m^2 n + m^3 + 2 m^2 n) flops (A and B are symmetric: only the tiles on and above the
 // diagonal are computed, and stored twice).  The small singular values are amplified by up to 3.4^5 = 485, and with them
 // every rounding, so 16-bit products alone are not enough for an fp32 result, and fp32 MFMA has 1/16 of the fp16 rate.
-// Every matrix is therefore kept as TWO fp16 planes, hi + lo = the value times a power of two: 22 significant bits, fewer only
-// below 2^-16 of the largest possible entry (all entries are bounded: |X| <= 1.2, |A| <= 1.45, |B| <= 2.9 by the quintic).
-// A product is three fp16 MFMAs, hi hi + hi lo + lo hi, summed in fp32; what is dropped, lo lo, is 2^-22 of the product, less
-// than the rounding of an fp32 sum of a few terms.  Simulated and measured, the result is as far from the 64-bit iteration
-// as that of fp32 matrix products (the fp32 sums dominate both).  (Iterating in the m x m space of the Gram matrix needs fewer
-// flops for n > m but squares the condition: 5 to 16 times the error on gradients with a decaying spectrum; not used.)
+// Every matrix is therefore kept as TWO fp16 planes, hi + lo = the value times a power of two of its row: 22 significant bits, fewer
+// only below 2^-16 of the largest entry that the row may have (see Scales).  A product is three fp16 MFMAs, hi hi + hi lo + lo hi,
+// summed in fp32; what is dropped, lo lo, is 2^-22 of the product, less than the rounding of an fp32 sum of a few terms.
+// Simulated and measured, the result is as far from the 64-bit iteration as that of fp32 matrix products, as a whole and in rows and
+// columns of 10^-14 of the others (the fp32 sums dominate both; 256 x 512 with half the rows at 10^-9: 1.9e-7 of those rows,
+// 3.5e-7 in fp32).  (Iterating in the m x m space of the Gram matrix needs fewer flops for n > m but squares the condition: 5 to 16
+// times the error on gradients with a decaying spectrum; not used.)
 //
 // Layout.  Both operands of every product are read along k: A = X X^T takes rows of X twice, A A takes rows of the symmetric
 // A, B X takes rows of B and rows of X^T.  So X is kept together with its transpose, each step's product writes both, and one
-// GEMM form (row times row) serves all.  A row of a plane pair is groups of 32 columns: 32 hi halves then 32 lo halves, 128
-// bytes, one cache line per row and k-step.  Dimensions are padded with zeros to whole tiles: the products need no bounds.
+// GEMM form (row times row) serves all.  The linear terms a X and b A are read as fp32 (see Linear).  A row of a plane pair is
+// groups of 32 columns: 32 hi halves then 32 lo halves, 128 bytes, one cache line per row and k-step.  Dimensions are padded with
+// zeros to whole tiles: the products need no bounds.
 //
 // GEMM.  A workgroup of four waves owns a square tile of 64, 128, 192 or 256 (or 32, see Narrow) and walks k in steps of 32 through a
-// ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 148, 132, 144 or 128 KB (ring_bytes()), one workgroup per CU, the
-// loads of a step requested one to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away, against 0.1 to 1.8 us of products per
-// step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at 16 l), so the 16-byte chunks of a row are
+// ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 148, 132, 144 or 128 KB (ring_bytes()), one workgroup per
+// CU, the loads of a step requested one to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away,
+// against 0.1 to 1.8 us of products per step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at
+// 16 l), so the 16-byte chunks of a row are
 // permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the sixteen rows that a quarter of a fragment
 // read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
 // A step's two halves of 16 k alternate between two sets of fragment registers: the LDS reads of one half and the loads are
@@ -42,21 +45,24 @@
 #include "dtf_api.h"
 #include "dtf_types.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef f16_t half8 __attribute__((ext_vector_type(8)));
-typedef f16_t half4 __attribute__((ext_vector_type(4)));
 typedef f16_t half2 __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kMax = DTF_MUON_MAX;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleX = 32768.f, kScaleA = 16384.f, kScaleB = 8192.f;    // powers of two: entries stay below 65504
-constexpr int kNormBlocks = 1024;     // at most: four partial sums a thread of split_kernel
+constexpr int kParts = 16;            // of the rows, and of the columns, for the norm and the maxima: at most, unless there are few of the other
+constexpr int kBlocks = kParts * kParts;
+constexpr int kMaxDim = 1 << 16;
+constexpr int kNormThreads = 1024;
 constexpr int kWaves = 4;              // of a product workgroup
 
 // One matrix of a call.  `rows` x `cols` as the caller has it; m <= n its shape (or its transpose's) padded to mp x np.
@@ -68,7 +74,11 @@ struct Item {
   int rows, cols, m, n, mp, np, flip;
   float shape_factor;   // sqrt(max(1, cols / rows))
   char *X, *XT[2], *A, *B;
-  double* norm;         // partial sums of squares
+  float *d, *e;         // scales of the m rows and the n columns (see Scales)
+  float *linear_a, *linear_x;     // A without its scales and X, fp32 (see Linear)
+  int edge_r, edge_c, parts_r, parts_c;      // parts of the matrix for the norm and the maxima
+  double* norm;         // [parts_r][parts_c]: sums of squares
+  float *row_max, *col_max;       // [parts_c][padded rows], [parts_r][padded columns]: largest magnitudes
 };
 
 struct Call {
@@ -76,60 +86,128 @@ struct Call {
   int count, dtype;
   float mu, eps;
   int nesterov;
-  int norm_blocks;
   const float* lr;
 };
 
-// --- momentum and norm ----------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float direction(const Call& c, const Item& it, int64_t at_u, int64_t at_buf) {
-  const float g = (float)static_cast<const T*>(it.u)[at_u];
-  if (!it.buf) return g;
-  const float b = it.buf[at_buf];
-  return c.nesterov ? g + c.mu * b : b;
+// --- momentum, norm and scales ------------------------------------------------------------------------------------------
+// The largest of a row of sixteen lanes, in each of them.
+template <int ROTATE>
+__device__ __forceinline__ float most_of_rotated(float v) {
+  const int other = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + ROTATE, 15, 15, false);      // row_ror
+  return fmaxf(v, __builtin_bit_cast(float, other));
+}
+__device__ __forceinline__ float most_of_16(float v) {
+  return most_of_rotated<1>(most_of_rotated<2>(most_of_rotated<4>(most_of_rotated<8>(v))));
 }
 
+// A part of the matrix per block, 64 x 64 elements at a time, four columns a thread: the momentum, the sum of squares, and the largest
+// magnitude of every row and column (exact, so that their order does not matter).
 template <typename T>
-__global__ __launch_bounds__(256) void norm_kernel(Call c) {
+__global__ __launch_bounds__(kNormThreads) void norm_kernel(Call c) {
   const Item& it = c.item[blockIdx.y];
-  const int64_t total = (int64_t)it.rows * it.cols, stride = (int64_t)gridDim.x * 256;
-  const int64_t me = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if ((int)blockIdx.x >= it.parts_r * it.parts_c) return;
+  __shared__ uint32_t row_max[kMaxDim / kParts], col_max[kMaxDim / kParts];
+  __shared__ double of_wave[kNormThreads / 64];
+  const int part_r = blockIdx.x / it.parts_c, part_c = blockIdx.x - part_r * it.parts_c;
+  const int r0 = part_r * it.edge_r, c0 = part_c * it.edge_c;
+  const int r1 = min(r0 + it.edge_r, it.rows), c1 = min(c0 + it.edge_c, it.cols);
+  for (int i = threadIdx.x; i < it.edge_r; i += kNormThreads) row_max[i] = 0;
+  for (int i = threadIdx.x; i < it.edge_c; i += kNormThreads) col_max[i] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, row = threadIdx.x >> 4;
+  // whole quads where every row is aligned
+  const bool aligned = it.ldu % 4 == 0 && (reinterpret_cast<uintptr_t>(it.u) % (4 * sizeof(T))) == 0 &&
+                       (!it.buf || (it.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(it.buf) & 15u) == 0));
   double sum = 0;
-  // four elements at a time where the matrix has no gaps and is aligned; the rest, or all of a strided one, one by one
-  const bool flat = it.ldu == it.cols && (reinterpret_cast<uintptr_t>(it.u) % (4 * sizeof(T))) == 0 &&
-                    (reinterpret_cast<uintptr_t>(it.buf) & 15u) == 0;
-  const int64_t quads = flat ? total / 4 : 0;
-  for (int64_t q = me; q < quads; q += stride) {
-    const Pack<T, 4> g = reinterpret_cast<const Pack<T, 4>*>(it.u)[q];
-    f32x4 u;
+  constexpr int U = 4;                         // quads of a row under way
+  for (int c_first = c0; c_first < c1; c_first += 64 * U) {
+    const int cs = c_first + 4 * (threadIdx.x & 15);
+    f32x4 top[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = (float)g.v[e];
-    if (it.buf) {
-      f32x4* at = reinterpret_cast<f32x4*>(it.buf) + q;
-      const f32x4 b = c.mu * *at + u;
-      *at = b;
-      u = c.nesterov ? u + c.mu * b : b;
+    for (int k = 0; k < U; ++k) top[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = r0 + row; r - row < r1; r += 64) {
+      const T* u = static_cast<const T*>(it.u) + r * it.ldu;
+      float* m = it.buf + (int64_t)r * it.cols;
+      f32x4 g[U], b[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        g[k] = b[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int col = cs + 64 * k;
+        if (r >= r1) continue;
+        if (aligned && col + 4 <= c1) {
+          const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(u + col);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[k][e] = (float)p.v[e];
+          if (it.buf) b[k] = *reinterpret_cast<const f32x4*>(m + col);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < c1) {
+              g[k][e] = (float)u[col + e];
+              if (it.buf) b[k][e] = m[col + e];
+            }
+        }
+      }
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int col = cs + 64 * k;
+        f32x4 v = g[k];
+        if (it.buf && r < r1) {
+          const f32x4 now = c.mu * b[k] + g[k];
+          if (aligned && col + 4 <= c1) {
+            *reinterpret_cast<f32x4*>(m + col) = now;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < c1) m[col + e] = now[e];
+          }
+          v = c.nesterov ? g[k] + c.mu * now : now;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum += (double)v[e] * (double)v[e];
+          top[k][e] = fmaxf(top[k][e], fabsf(v[e]));
+          most = fmaxf(most, fabsf(v[e]));
+        }
+      }
+      most = most_of_16(most);
+      if ((lane & 15) == 0 && r < r1) atomicMax(&row_max[r - r0], __builtin_bit_cast(uint32_t, most));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum += (double)u[e] * (double)u[e];
-  }
-  for (int64_t i = 4 * quads + me; i < total; i += stride) {
-    int64_t at = i;
-    if (it.ldu != it.cols) {
-      const int64_t r = i / it.cols;
-      at = r * it.ldu + (i - r * it.cols);
+    for (int k = 0; k < U; ++k) {
+      if (c_first + 64 * k >= c1) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = cs + 64 * k + e;
+        const float most = top[k][e];      // (a bit cast of a vector's element is one of its first element)
+        if (col < c1) atomicMax(&col_max[col - c0], __builtin_bit_cast(uint32_t, most));
+      }
     }
-    if (it.buf) it.buf[i] = c.mu * it.buf[i] + (float)static_cast<const T*>(it.u)[at];
-    const double u = direction<T>(c, it, at, i);
-    sum += u * u;
   }
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
-  __shared__ double of_wave[4];
-  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = sum;
+  if (lane == 0) of_wave[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) it.norm[blockIdx.x] = (of_wave[0] + of_wave[1]) + (of_wave[2] + of_wave[3]);
+  const int pr = it.flip ? it.np : it.mp, pc = it.flip ? it.mp : it.np;       // padded rows and columns as the caller has them
+  for (int i = threadIdx.x; i < min(it.edge_r, pr - r0); i += kNormThreads)
+    it.row_max[(int64_t)part_c * pr + r0 + i] = __builtin_bit_cast(float, row_max[i]);
+  for (int i = threadIdx.x; i < min(it.edge_c, pc - c0); i += kNormThreads)
+    it.col_max[(int64_t)part_r * pc + c0 + i] = __builtin_bit_cast(float, col_max[i]);
+  if (threadIdx.x == 0) {
+    double total = 0;
+    for (int w = 0; w < kNormThreads / 64; ++w) total += of_wave[w];
+    it.norm[blockIdx.x] = total;
+  }
 }
+
+// Smallest power of two that is not below v, from 2^-100 to 1.
+__device__ __forceinline__ float scale_above(float v) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, fminf(fmaxf(v, 0x1p-100f), 1.f));
+  return __builtin_bit_cast(float, (bits + 0x7fffffu) & 0xff800000u);
+}
+// 1 / v of such a power of two.
+__device__ __forceinline__ float reciprocal(float v) { return __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, v)); }
 
 // --- plane pairs ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t split_pair(float scaled) {       // hi | lo << 16
@@ -141,71 +219,100 @@ __device__ __forceinline__ uint32_t split_pair(float scaled) {       // hi | lo 
 __device__ __forceinline__ int64_t plane_at(int64_t row, int col, int cols) {
   return row * cols * 4 + (col >> 5) * 128 + (col & 31) * 2;
 }
-// A 64 x 64 tile of pairs in LDS, its rows `line` and its columns `step` words apart, to row0, col0 of a plane pair: 256 bytes a
-// row, sixteen bytes a thread and turn, consecutive threads one behind the other (64 bytes a thread: the kernel took 23 us
-// for 1024 x 4096 instead of 17).
-__device__ __forceinline__ void store_tile(char* plane, int row0, int col0, int cols, const uint32_t* pairs, int line, int step) {
+// A 64 x 64 tile of values in LDS, its rows `line` and its columns `step` words apart and each row times its `scale`, to row0, col0
+// of a plane pair: 256 bytes a row, sixteen bytes a thread and turn, consecutive threads one behind the other (64 bytes a thread:
+// the kernel took 23 us for 1024 x 4096 instead of 17).
+__device__ __forceinline__ void store_tile(char* plane, int row0, int col0, int cols, const float* values, int line, int step,
+                                           const float* scale) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int row = k * 16 + (threadIdx.x >> 4), chunk = threadIdx.x & 15;      // chunk: group of 32 columns, hi or lo, 8 columns
     const int col = (chunk >> 3) * 32 + (chunk & 3) * 8, shift = (chunk >> 2 & 1) * 16;
+    const float f = scale[row];
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t* at = pairs + row * line + (col + 2 * e) * step;
-      w[e] = (at[0] >> shift & 0xffffu) | (at[step] >> shift) << 16;
+      const float* at = values + row * line + (col + 2 * e) * step;
+      w[e] = (split_pair(at[0] * f) >> shift & 0xffffu) | (split_pair(at[step] * f) >> shift) << 16;
     }
     *reinterpret_cast<u32x4*>(plane + plane_at(row0 + row, col0, cols) + chunk * 16) = w;
   }
 }
 
-// X and X^T of U / (|U| + eps), 64 x 64 tiles of the padded shape.
+// X of U / (|U| + eps) as planes, turned and straight, and in fp32, and the scales: 64 x 64 tiles of the padded shape.
 template <typename T>
 __global__ __launch_bounds__(256) void split_kernel(Call c) {
-  __shared__ uint32_t tile[64][65];
+  __shared__ float tile[64][65];
   __shared__ double of_wave[4];
+  __shared__ float most[2][4][64], to[2][64];         // of the rows, of the columns
   const Item& it = c.item[blockIdx.y];
   const int pr = it.flip ? it.np : it.mp, pc = it.flip ? it.mp : it.np;       // padded rows and columns as the caller has them
   const int tiles_c = pc / 64, tiles = (pr / 64) * tiles_c;
   if ((int)blockIdx.x >= tiles) return;
   const int r0 = (blockIdx.x / tiles_c) * 64, c0 = (blockIdx.x % tiles_c) * 64;
-  const int col = threadIdx.x & 63;
+  const int col = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // All requests at once and before the norm is added up, from clamped places: one by one they took 15 us.
   const T* gp = static_cast<const T*>(it.u) + min(c0 + col, it.cols - 1);
   const float* bp = it.buf + min(c0 + col, it.cols - 1);
   float u[16];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) u[k] = (float)gp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.ldu];
+  for (int k = 0; k < 16; ++k) u[k] = (float)gp[(int64_t)min(r0 + wave + 4 * k, it.rows - 1) * it.ldu];
   float b[16];
   if (it.buf) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) b[k] = bp[(int64_t)min(r0 + (int)(threadIdx.x >> 6) + 4 * k, it.rows - 1) * it.cols];
+    for (int k = 0; k < 16; ++k) b[k] = bp[(int64_t)min(r0 + wave + 4 * k, it.rows - 1) * it.cols];
   }
-  double total = 0;
+  const int parts = it.parts_r * it.parts_c;
+  double total = it.norm[min((int)threadIdx.x, parts - 1)];
+  float row_top = 0.f, col_top = 0.f;                 // (the last part again past the end)
+  for (int p = wave; p < max(it.parts_r, it.parts_c); p += 16)
 #pragma unroll
-  for (int i = 0; i < kNormBlocks; i += 256) {
-    const double part = it.norm[min(i + (int)threadIdx.x, c.norm_blocks - 1)];
-    total += i + (int)threadIdx.x < c.norm_blocks ? part : 0.0;
-  }
+    for (int k = 0; k < 16; k += 4) {
+      row_top = fmaxf(row_top, it.row_max[(int64_t)min(p + k, it.parts_c - 1) * pr + r0 + col]);
+      col_top = fmaxf(col_top, it.col_max[(int64_t)min(p + k, it.parts_r - 1) * pc + c0 + col]);
+    }
+  if ((int)threadIdx.x >= parts) total = 0.0;
   if (it.buf) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) u[k] = c.nesterov ? u[k] + c.mu * b[k] : b[k];
   }
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) total += __shfl_xor(total, x);
-  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = total;
+  if (col == 0) of_wave[wave] = total;
+  most[0][wave][col] = row_top;
+  most[1][wave][col] = col_top;
   __syncthreads();
-  const double inv = (double)kScaleX / (sqrt((of_wave[0] + of_wave[1]) + (of_wave[2] + of_wave[3])) + (double)c.eps);
+  const double length = sqrt((of_wave[0] + of_wave[1]) + (of_wave[2] + of_wave[3])) + (double)c.eps;
+  const double inv = length == 0.0 ? 0.0 : 1.0 / length;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
-    const int r = (threadIdx.x >> 6) + 4 * k;
-    tile[r][col] = r0 + r < it.rows && c0 + col < it.cols ? split_pair((float)((double)u[k] * inv)) : 0u;
+    const int r = wave + 4 * k;
+    tile[r][col] = r0 + r < it.rows && c0 + col < it.cols ? (float)((double)u[k] * inv) : 0.f;
+  }
+  if (wave < 2) {                        // the scales of the tile's rows (wave 0) and columns
+    const float top = fmaxf(fmaxf(most[wave][0][col], most[wave][1][col]), fmaxf(most[wave][2][col], most[wave][3][col]));
+    const float s = scale_above((float)((double)top * inv * (double)sqrtf((float)(wave ? it.rows : it.cols))));
+    to[wave][col] = kScaleX * reciprocal(s);
+    float* const scales = (wave == 1) != (it.flip != 0) ? it.e : it.d;
+    if ((wave ? r0 : c0) == 0) scales[(wave ? c0 : r0) + col] = s;
   }
   __syncthreads();
   char* straight = it.flip ? it.XT[0] : it.X;          // [pr][pc]
   char* turned = it.flip ? it.X : it.XT[0];            // [pc][pr]
-  store_tile(straight, r0, c0, pc, &tile[0][0], 65, 1);
-  store_tile(turned, c0, r0, pr, &tile[0][0], 1, 65);
+  store_tile(straight, r0, c0, pc, &tile[0][0], 65, 1, to[0]);
+  store_tile(turned, c0, r0, pr, &tile[0][0], 1, 65, to[1]);
+  // (block by block as Linear reads them)
+  const int i0 = it.flip ? c0 : r0, j0 = it.flip ? r0 : c0, lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f32x4 v;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int i = 32 * (k >> 1) + 8 * g + 4 * (lane >> 5) + x, j = 32 * (k & 1) + (lane & 31);
+      v[x] = it.flip ? tile[j][i] : tile[i][j];
+    }
+    *reinterpret_cast<f32x4*>(it.linear_x + ((int64_t)(i0 / 32 + (k >> 1)) * (it.np / 32) + j0 / 32 + (k & 1)) * 1024 + g * 256 + lane * 4) = v;
+  }
 }
 
 // --- products -----------------------------------------------------------------------------------------------------------
@@ -215,17 +322,27 @@ enum Stage { kGram = 0, kPoly = 1, kStep = 2, kLast = 3 };     // A = X X^T;  B 
 // instruction brings them into a wave's registers, whichever its matrix is (see find()).
 struct Job {
   const char *p, *q;          // the operands: rows of k
-  const char* linear;         // of the linear term: A, or X through its transpose
+  char* linear;               // of the linear term: A (written by kGram), or X (kStep writes the next one in its place)
   char *straight, *turned;    // the result, and its transpose
   int rows, cols, depth;      // of the product, padded
   int first, tiles;           // first tile and number of tiles
   int spare;
+  // The scales lie in front of the linear terms: those of the columns, those of the rows, A, X.
+  __host__ __device__ static int64_t scale_bytes(int count) { return ((int64_t)count * 4 + 1023) / 1024 * 1024; }
+  __device__ __forceinline__ const float* row_scales(bool symmetric) const {
+    return reinterpret_cast<const float*>(linear - (symmetric ? 0 : (int64_t)rows * rows * 4) - scale_bytes(rows));
+  }
+  __device__ __forceinline__ const float* col_scales(bool symmetric) const {
+    const float* d = row_scales(symmetric);
+    return symmetric ? d : reinterpret_cast<const float*>(reinterpret_cast<const char*>(d) - scale_bytes(cols));
+  }
 };
 static_assert(sizeof(Job) == 64, "find() counts words");
 struct Jobs {
   Job job[kMax];
   float* partial;             // split products: [tile][split][elements of a tile]
   int splits;                 // workgroups per tile, a range of k each
+  float growth;               // of the scales up to this iteration (see Scales)
 };
 // Where the last product goes.
 struct Final {
@@ -376,51 +493,74 @@ constexpr int kTurnWords = 2 * 32 * kTurnRow;     // two turning areas of a wave
 // Order of a wave's own LDS accesses (nobody else touches its areas).
 __device__ __forceinline__ void own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The linear term of a tile in fp32, as the sums lie in the registers: 4 KB a tile, whole lines in either direction.
 struct Linear {
-  u32x4 chunk[4];
+  f32x4 v[4];
+  static __device__ __forceinline__ f32x4* at(const Task& t, int i0, int j0, int lane) {
+    return reinterpret_cast<f32x4*>(t.linear) + ((int64_t)(i0 >> 5) * (t.cols >> 5) + (j0 >> 5)) * 256 + lane;
+  }
   __device__ __forceinline__ void read(const Task& t, int i0, int j0, int lane) {
-    const char* s = t.linear + plane_at(j0 + (lane >> 3), i0, t.rows) + 16 * (lane & 7);
+    const f32x4* from = at(t, i0, j0, lane);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) chunk[n] = *reinterpret_cast<const u32x4*>(s + (int64_t)n * 8 * t.rows * 4);
+    for (int g = 0; g < 4; ++g) v[g] = from[64 * g];
   }
 };
+
+// Scales.  Row i of X is kept divided by d_i and column j (a row of X^T) by e_j, powers of two that are not below their norms (the
+// largest magnitude times the root of the length, rounded up); rows of A and B are divided by d_i too.  So an entry has its 22 bits
+// relative to its own row, however little that is next to the others.  (One scale for the whole matrix: rows of 10^-6 of the
+// others were 400 times as far off as in fp32, nothing was left of rows of 10^-10.  It took 127 us for the stack of three matrices
+// instead of 132, 351 for 1024 x 4096 instead of 368, 3.52 ms for a step of 4096 x 4096 instead of 3.64: X in fp32 is 4 bytes an
+// element more to write in each step.)  No product needs more than that: with P = D^-1 X, R = D^-1 A, S = D^-1 B and T = E^-1 X^T,
+//   A = D (P P^T) D,   A A = D (R R^T) D,   B X = D (S T^T) E,
+// so the scales meet the sums at a product's end alone.  The linear terms carry no scale of one side: A is kept as D^-1 A D^-1
+// and X as it is, in fp32.  A step multiplies no singular value by more than 3.4445, and so no row's or column's norm: the scales
+// grow by 4 with each step, up to 1.  |P|, |T| <= 1.2, |R| <= 1.45, |S| <= 1.2 * 2.83 by the quintic.
+struct Scales {               // of a tile's rows and columns, in LDS
+  const float *row, *row_to;  // the scale, and kScaleX over the next step's
+  const float *col, *col_to;
+};
+__device__ __forceinline__ float scale_now(float first, float growth) { return fminf(first * growth, 1.f); }
+__device__ __forceinline__ float scale_to(float first, float growth) { return kScaleX * reciprocal(fminf(first * (4.f * growth), 1.f)); }
+
+// Value times scale as hi and lo, two rows at a time.
+__device__ __forceinline__ void split_rows(const f32x4 (&v)[4], half2 (&hi)[8], half2 (&lo)[8]) {
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const float2v x = {v[p / 2][2 * (p & 1)], v[p / 2][2 * (p & 1) + 1]};
+    hi[p] = __builtin_convertvector(x, half2);
+    lo[p] = __builtin_convertvector(x - __builtin_convertvector(hi[p], float2v), half2);
+  }
+}
 
 // What becomes of the tile.  `area`: the wave's turning areas.  `mirror`: also store the transposed tile of a symmetric result.
 template <int STAGE>
 __device__ __forceinline__ void store_tile(const Task& t, const typename EndOf<STAGE>::Mine& end, int i0, int j0, bool mirror,
-                                           const f32x16& sum, const Linear& linear, uint32_t* area, int lane) {
+                                           const f32x16& sum, const Linear& linear, const Scales& scales, uint32_t* area, int lane) {
   const int half = lane >> 5, jc = lane & 31;
   uint32_t* turn = area;
   uint32_t* lines = area + 32 * kTurnRow;
-  float v[16];
-  if (STAGE == kGram) {
+  f32x4 v[4], row[4];
+  const float col = scales.col[jc];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = sum[e] * (kScaleA / (kScaleX * kScaleX));
-  } else {
+  for (int g = 0; g < 4; ++g) row[g] = *reinterpret_cast<const f32x4*>(scales.row + 8 * g + 4 * half);
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      *reinterpret_cast<u32x4*>(lines + ((lane >> 3) + 8 * n) * kTurnRow + 4 * (lane & 7)) = linear.chunk[n];
-    own_lds();
-    const float lin = STAGE == kPoly ? kB * (kScaleB / kScaleA) : STAGE == kStep ? kA : kA / kScaleX;
-    const float quad = STAGE == kPoly ? kC * kScaleB / (kScaleA * kScaleA)
-                       : STAGE == kStep ? 1.f / kScaleB : 1.f / (kScaleB * kScaleX);
-    const char* line = reinterpret_cast<const char*>(lines + jc * kTurnRow) + 8 * half;
+  for (int g = 0; g < 4; ++g)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const half4 hi = *reinterpret_cast<const half4*>(line + 16 * g), lo = *reinterpret_cast<const half4*>(line + 64 + 16 * g);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)      // (two mixed-precision multiply-adds: the planes are not converted)
-        v[4 * g + x] = fmaf((float)hi[x], lin, fmaf((float)lo[x], lin, quad * sum[4 * g + x]));
+    for (int x = 0; x < 4; ++x) {
+      const float s = sum[4 * g + x];
+      v[g][x] = STAGE == kGram   ? s * (1.f / (kScaleX * kScaleX))
+                : STAGE == kPoly ? fmaf(kB, linear.v[g][x], s * (kC / (kScaleA * kScaleA)))
+                                 : fmaf(kA, linear.v[g][x], s * (row[g][x] * (1.f / (kScaleB * kScaleX))) * col);
     }
-  }
   if constexpr (STAGE == kLast) {
     const Final& it = end.f;
     // (places past the matrix are read as its last ones and not stored)
     const int64_t step_row = it.flip ? 1 : it.ld, step_col = it.flip ? it.ld : 1;
-    const int row0 = i0 + 4 * half, col = j0 + jc;
-    const int64_t at_col = min(col, it.n - 1) * step_col;
+    const int row0 = i0 + 4 * half, at_j = j0 + jc;
+    const int64_t at_col = min(at_j, it.n - 1) * step_col;
     auto place = [&](int e) { return min(row0 + 8 * (e / 4) + e % 4, it.m - 1) * step_row + at_col; };
-    auto inside = [&](int e) { return row0 + 8 * (e / 4) + e % 4 < it.m && col < it.n; };
+    auto inside = [&](int e) { return row0 + 8 * (e / 4) + e % 4 < it.m && at_j < it.n; };
     if (end.lr || end.dtype == DTF_F32) {
       float* out = static_cast<float*>(it.out);
       if (end.lr) {                       // the weights: all of them requested before the first store
@@ -429,29 +569,34 @@ __device__ __forceinline__ void store_tile(const Task& t, const typename EndOf<S
 #pragma unroll
         for (int e = 0; e < 16; ++e) old[e] = out[place(e)];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = old[e] - step_size * v[e];
+        for (int e = 0; e < 16; ++e) v[e / 4][e % 4] = old[e] - step_size * v[e / 4][e % 4];
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (inside(e)) out[place(e)] = v[e];
+        if (inside(e)) out[place(e)] = v[e / 4][e % 4];
     } else {
       uint16_t* out = static_cast<uint16_t*>(it.out);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint16_t bits = end.dtype == DTF_BF16 ? __builtin_bit_cast(uint16_t, (bf16_t)v[e]) : __builtin_bit_cast(uint16_t, (f16_t)v[e]);
+        const float x = v[e / 4][e % 4];
+        const uint16_t bits = end.dtype == DTF_BF16 ? __builtin_bit_cast(uint16_t, (bf16_t)x) : __builtin_bit_cast(uint16_t, (f16_t)x);
         if (inside(e)) out[place(e)] = bits;
       }
     }
     return;
   }
-  // hi and lo of two rows at a time
-  half2 hi[8], lo[8];
+  if (STAGE != kPoly) {
+    f32x4* to = Linear::at(t, i0, j0, lane);
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const float2v x = {v[2 * p], v[2 * p + 1]};
-    hi[p] = __builtin_convertvector(x, half2);
-    lo[p] = __builtin_convertvector(x - __builtin_convertvector(hi[p], float2v), half2);
+    for (int g = 0; g < 4; ++g) to[64 * g] = v[g];
   }
+  half2 hi[8], lo[8];
+  f32x4 w[4];
+  constexpr float kSquare = STAGE == kGram ? kScaleA : kScaleB;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    w[g] = STAGE <= kPoly ? v[g] * (col * kSquare) : v[g] * *reinterpret_cast<const f32x4*>(scales.row_to + 8 * g + 4 * half);
+  split_rows(w, hi, lo);
   f16_t* at = reinterpret_cast<f16_t*>(turn + 4 * half * kTurnRow) + jc;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
@@ -461,7 +606,10 @@ __device__ __forceinline__ void store_tile(const Task& t, const typename EndOf<S
   if (mirror) {
     // Line j of the transposed tile: this lane has rows 4 half .. 4 half + 3 of every eight, the lane 32 away the other four.
     // Exchanged between two groups of eight, each lane holds whole chunks.
-    own_lds();                            // (the linear term has been read)
+    const float col_to = STAGE <= kPoly ? 0.f : scales.col_to[jc];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) w[g] = STAGE <= kPoly ? v[g] * (row[g] * kSquare) : v[g] * col_to;
+    split_rows(w, hi, lo);
     uint32_t* line = lines + jc * kTurnRow + 4 * half;
 #pragma unroll
     for (int g = 0; g < 4; g += 2)
@@ -489,6 +637,19 @@ __device__ __forceinline__ void store_tile(const Task& t, const typename EndOf<S
   own_lds();
 }
 
+// A wave's tile of 32: its scales to LDS (`at`, 128 words of the wave's own).  Lanes 0 .. 31 have read a row's, the others a
+// column's (see read_scale).
+template <int STAGE>
+__device__ __forceinline__ float read_scale(const Task& t, int i0, int j0, int lane) {
+  return lane < 32 ? t.row_scales(STAGE <= kPoly)[i0 + lane] : t.col_scales(STAGE <= kPoly)[j0 + lane - 32];
+}
+__device__ __forceinline__ Scales lay_scales(float first, float growth, float* at, int lane) {
+  at[lane] = scale_now(first, growth);
+  at[64 + lane] = scale_to(first, growth);
+  own_lds();
+  return Scales{at, at + 64, at + 32, at + 96};
+}
+
 // Tile `t` of a stage: rows and columns in tiles.  Symmetric results: t = tj (tj + 1) / 2 + ti, ti <= tj.
 template <int STAGE>
 __device__ __forceinline__ void tile_place(const Task& task, int edge, int t, int& ti, int& tj) {
@@ -513,7 +674,7 @@ constexpr int ring_bytes(int tile) {                // (image 0 becomes the turn
   return (2 * tile * 128 < kTurn ? kTurn : 2 * tile * 128) + (ring_of(tile) - 1) * 2 * tile * 128;
 }
 static_assert(ring_bytes(64) == 148 << 10 && ring_bytes(128) == 132 << 10 && ring_bytes(192) == 144 << 10 && ring_bytes(256) == 128 << 10,
-              "a CU has 160 KB");
+              "a CU has 160 KB, and up to 4 KB are for the scales of a tile");
 
 // LDS image I of the ring: the rows of one operand, then the other's.  (One variable each: the compiler must see that a load to
 // one image does not concern the reads of another.)
@@ -692,6 +853,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Jobs jobs, typen
   g.q.init(task.q, tj * 32, task.cols, row_bytes, 0, lane);
   g.wave = wave, g.lane = lane;
   Linear linear{};
+  float scale = 0.f;
+  if (wave == 0) scale = read_scale<STAGE>(task, ti * 32, tj * 32, lane);
   if (STAGE != kGram && wave == 0) linear.read(task, ti * 32, tj * 32, lane);
   f32x16 sums[3][1][1];
 #pragma unroll
@@ -719,11 +882,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void narrow_kernel(Jobs jobs, typen
 #pragma unroll
       for (int x = 0; x < 4; ++x) sum[4 * g4 + x] += v[x];
     }
-  store_tile<STAGE>(task, end, ti * 32, tj * 32, STAGE > kPoly || ti != tj, sum, linear, reinterpret_cast<uint32_t*>(image<128, 0>()), lane);
+  const Scales scales = lay_scales(scale, jobs.growth, reinterpret_cast<float*>(image<128, 2>()), lane);
+  store_tile<STAGE>(task, end, ti * 32, tj * 32, STAGE > kPoly || ti != tj, sum, linear, scales, reinterpret_cast<uint32_t*>(image<128, 0>()), lane);
 }
 
 template <int TILE, int STAGE>
 __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, typename EndOf<STAGE>::Args all_ends) {
+  __shared__ __attribute__((aligned(16))) float scale_of[4][TILE];      // rows and columns: the scales, kScaleX over the next ones
   constexpr int MI = Product<TILE>::MI, NI = Product<TILE>::NI;
   Product<TILE> g;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -740,8 +905,17 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, type
   const int row_p = g.row_p = (wave >> 1) * (TILE / 2), row_q = g.row_q = (wave & 1) * (TILE / 2);
   const int pairs = task.depth / 64;
   const int k_first = 2 * (int)((int64_t)pairs * part / splits), k_last = 2 * (int)((int64_t)pairs * (part + 1) / splits);
-  // 32 x 32 tiles past the matrix are neither read nor stored (dimensions are whole multiples of 64: a wave has none, or full rows)
-  auto there = [&](int i, int j) { return ti * TILE + row_p + 32 * i < task.rows && tj * TILE + row_q + 32 * j < task.cols; };
+  // 32 x 32 tiles past the matrix are neither read nor stored (dimensions are whole multiples of 64: a wave has none, or full rows),
+  // nor those below the diagonal of a symmetric result, which are stored with their mirror images
+  auto there = [&](int i, int j) {
+    const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q + 32 * j;
+    return i0 < task.rows && j0 < task.cols && (STAGE > kPoly || i0 <= j0);
+  };
+  float row_scale = 0.f, col_scale = 0.f;
+  if (threadIdx.x < TILE && splits == 1) {
+    row_scale = task.row_scales(STAGE <= kPoly)[min(ti * TILE + (int)threadIdx.x, task.rows - 1)];
+    col_scale = task.col_scales(STAGE <= kPoly)[min(tj * TILE + (int)threadIdx.x, task.cols - 1)];
+  }
   Linear early{};                         // (of the smallest tile: under way during the product)
   if (MI * NI == 1 && STAGE != kGram && splits == 1 && there(0, 0)) early.read(task, ti * TILE + row_p, tj * TILE + row_q, lane);
   constexpr int kSums = Product<TILE>::kSums;
@@ -774,6 +948,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, type
               f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
     return;
   }
+  if (threadIdx.x < TILE) {
+    scale_of[0][threadIdx.x] = scale_now(row_scale, jobs.growth);
+    scale_of[1][threadIdx.x] = scale_to(row_scale, jobs.growth);
+    scale_of[2][threadIdx.x] = scale_now(col_scale, jobs.growth);
+    scale_of[3][threadIdx.x] = scale_to(col_scale, jobs.growth);
+  }
+  __syncthreads();
   // Nobody reads the images any more: image 0 becomes the waves' turning areas.  The linear terms of a row of tiles are under way
   // while the row before is stored; straight-line code, so that waiting for them does not mean waiting for the stores behind them
   // (a loop over the tiles took 1.7 us for each: its head waited for everything).
@@ -812,9 +993,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, type
       } else {
         sum = acc[i][j];
       }
-      if (there(i, j))
-        store_tile<STAGE>(task, end, ti * TILE + row_p + 32 * i, tj * TILE + row_q + 32 * j, STAGE > kPoly || ti != tj, sum,
-                          linear[i % kRows][j], turn, lane);
+      if (there(i, j)) {
+        const int i0 = ti * TILE + row_p + 32 * i, j0 = tj * TILE + row_q + 32 * j, in_p = row_p + 32 * i, in_q = row_q + 32 * j;
+        store_tile<STAGE>(task, end, i0, j0, STAGE > kPoly || i0 != j0, sum, linear[i % kRows][j],
+                          Scales{scale_of[0] + in_p, scale_of[1] + in_p, scale_of[2] + in_q, scale_of[3] + in_q}, turn, lane);
+      }
       if (kRows == 1 && i + 1 < MI && STAGE != kGram && there(i + 1, j))
         linear[0][j].read(task, ti * TILE + row_p + 32 * (i + 1), tj * TILE + row_q + 32 * j, lane);
     }
@@ -825,6 +1008,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void product_kernel(Jobs jobs, type
 template <int STAGE>
 __global__ __launch_bounds__(256) void finish_kernel(Jobs jobs, typename EndOf<STAGE>::Args ends, int edge, int waves) {
   __shared__ __attribute__((aligned(16))) uint32_t turns[4][kTurnWords];
+  __shared__ __attribute__((aligned(16))) float scale_of[4][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x * 4 + wave;
   if (id >= waves) return;
@@ -836,10 +1020,11 @@ __global__ __launch_bounds__(256) void finish_kernel(Jobs jobs, typename EndOf<S
   int ti, tj;
   tile_place<STAGE>(task, edge, tile, ti, tj);
   const int i0 = ti * edge + (of_wave >> 1) * (edge / 2) + 32 * (ij / side), j0 = tj * edge + (of_wave & 1) * (edge / 2) + 32 * (ij % side);
-  if (i0 >= task.rows || j0 >= task.cols) return;
+  if (i0 >= task.rows || j0 >= task.cols || (STAGE <= kPoly && i0 > j0)) return;
   const int64_t elems = (int64_t)edge * edge;
   const float* from = jobs.partial + (int64_t)(task.first + tile) * splits * elems + of_wave * (elems / 4) + ij * 1024 + lane * 4;
   Linear linear{};
+  const float scale = read_scale<STAGE>(task, i0, j0, lane);
   if (STAGE != kGram) linear.read(task, i0, j0, lane);
   f32x16 sum;
 #pragma unroll
@@ -855,13 +1040,12 @@ __global__ __launch_bounds__(256) void finish_kernel(Jobs jobs, typename EndOf<S
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[e] += s0 + k < splits ? v[k][e / 4][e % 4] : 0.f;
   }
-  store_tile<STAGE>(task, end, i0, j0, STAGE > kPoly || ti != tj, sum, linear, turns[wave], lane);
+  store_tile<STAGE>(task, end, i0, j0, STAGE > kPoly || i0 != j0, sum, linear, lay_scales(scale, jobs.growth, scale_of[wave], lane),
+                    turns[wave], lane);
 }
 
 // --- host ---------------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-constexpr int kMaxDim = 1 << 16;
 
 bool bad_shapes(int count, const int32_t* rows, const int32_t* cols) {
   if (count < 1 || count > kMax || !rows || !cols) return true;
@@ -952,7 +1136,7 @@ struct Layout {
 Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, char* base) {
   Layout l;
   c.count = count;
-  int64_t at = 0, most = 0;
+  int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = base + at;
     at += up(bytes, 1024);
@@ -965,15 +1149,22 @@ Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, cha
     it.m = it.flip ? cols[i] : rows[i];
     it.n = it.flip ? rows[i] : cols[i];
     it.mp = (int)up(it.m, 64), it.np = (int)up(it.n, 64);
-    it.norm = reinterpret_cast<double*>(take(kNormBlocks * 8));
+    // Parts of whole tiles of 64: kBlocks at most, up to 64 of the rows of a narrow matrix or the columns of a flat one.  (Every
+    // tile of split_kernel reads the maxima of all parts of its rows and columns.)
+    const int tiles_r = (rows[i] + 63) / 64, tiles_c = (cols[i] + 63) / 64;
+    const int most_r = std::max(kParts, std::min(64, kBlocks / tiles_c)), most_c = std::max(kParts, std::min(64, kBlocks / tiles_r));
+    it.edge_r = (int)up((rows[i] + most_r - 1) / most_r, 64), it.edge_c = (int)up((cols[i] + most_c - 1) / most_c, 64);
+    it.parts_r = (rows[i] + it.edge_r - 1) / it.edge_r, it.parts_c = (cols[i] + it.edge_c - 1) / it.edge_c;
+    it.norm = reinterpret_cast<double*>(take(kBlocks * 8));
+    it.row_max = reinterpret_cast<float*>(take((int64_t)it.parts_c * up(rows[i], 64) * 4));
+    it.col_max = reinterpret_cast<float*>(take((int64_t)it.parts_r * up(cols[i], 64) * 4));
     const int64_t wide = (int64_t)it.mp * it.np * 4, square = (int64_t)it.mp * it.mp * 4;
     it.X = take(wide), it.XT[0] = take(wide), it.XT[1] = take(wide);
     it.A = take(square), it.B = take(square);
-    const int64_t elements = (int64_t)rows[i] * cols[i];
-    most = elements > most ? elements : most;
+    it.e = reinterpret_cast<float*>(take(Job::scale_bytes(it.np)));        // (in this order: see Job)
+    it.d = reinterpret_cast<float*>(take(Job::scale_bytes(it.mp)));
+    it.linear_a = reinterpret_cast<float*>(take(square)), it.linear_x = reinterpret_cast<float*>(take(wide));
   }
-  const int64_t blocks = (most + 2047) / 2048;           // eight elements a thread
-  c.norm_blocks = (int)(blocks > kNormBlocks ? kNormBlocks : blocks);
   int64_t partial = 0;
   for (int stage = kGram; stage <= kStep; ++stage) {
     l.stage[stage] = plan_stage(c, stage);
@@ -985,11 +1176,13 @@ Layout lay_out(Call& c, const int32_t* rows, const int32_t* cols, int count, cha
 }
 
 template <int STAGE>
-void launch_stage(const Call& c, const Layout& l, int parity, const typename EndOf<STAGE>::Args& ends, hipStream_t s) {
+void launch_stage(const Call& c, const Layout& l, int iteration, const typename EndOf<STAGE>::Args& ends, hipStream_t s) {
+  const int parity = iteration & 1;
   const StagePlan& p = l.stage[STAGE == kLast ? kStep : STAGE];
   Jobs jobs{};
   jobs.partial = l.partial;
   jobs.splits = p.cut.splits;
+  jobs.growth = (float)(1 << 2 * iteration);
   for (int i = 0; i < kMax; ++i) {
     Job& j = jobs.job[i];
     j.first = p.first[i], j.tiles = p.first[i + 1] - p.first[i];
@@ -997,7 +1190,7 @@ void launch_stage(const Call& c, const Layout& l, int parity, const typename End
     const Item& it = c.item[i];
     j.p = STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.B;
     j.q = STAGE == kGram ? it.X : STAGE == kPoly ? it.A : it.XT[parity];
-    j.linear = STAGE == kPoly ? it.A : it.XT[parity];
+    j.linear = reinterpret_cast<char*>(STAGE <= kPoly ? it.linear_a : it.linear_x);
     j.straight = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.X;
     j.turned = STAGE == kGram ? it.A : STAGE == kPoly ? it.B : it.XT[parity ^ 1];
     j.rows = it.mp;
@@ -1020,12 +1213,14 @@ void launch_stage(const Call& c, const Layout& l, int parity, const typename End
 
 template <typename T>
 int run(Call& c, const Layout& l, hipStream_t s) {
-  norm_kernel<T><<<dim3(c.norm_blocks, c.count), 256, 0, s>>>(c);
   int64_t most = 0;
+  int parts = 0;
   for (int i = 0; i < c.count; ++i) {
     const int64_t t = (int64_t)(c.item[i].mp / 64) * (c.item[i].np / 64);
     most = t > most ? t : most;
+    parts = std::max(parts, c.item[i].parts_r * c.item[i].parts_c);
   }
+  norm_kernel<T><<<dim3(parts, c.count), kNormThreads, 0, s>>>(c);
   split_kernel<T><<<dim3((unsigned)most, c.count), 256, 0, s>>>(c);
   Finals finals{};
   for (int i = 0; i < c.count; ++i) {
@@ -1034,10 +1229,10 @@ int run(Call& c, const Layout& l, hipStream_t s) {
   }
   finals.lr = c.lr, finals.dtype = c.dtype;
   for (int k = 0; k < 5; ++k) {
-    launch_stage<kGram>(c, l, k & 1, None{}, s);
-    launch_stage<kPoly>(c, l, k & 1, None{}, s);
-    if (k < 4) launch_stage<kStep>(c, l, k & 1, None{}, s);
-    else launch_stage<kLast>(c, l, k & 1, finals, s);
+    launch_stage<kGram>(c, l, k, None{}, s);
+    launch_stage<kPoly>(c, l, k, None{}, s);
+    if (k < 4) launch_stage<kStep>(c, l, k, None{}, s);
+    else launch_stage<kLast>(c, l, k, finals, s);
   }
   return hipGetLastError() == hipSuccess ? DTF_OK : DTF_ERR_LAUNCH;
 }

@@ -1,7 +1,8 @@
 """Orthogonalised updates of matrices (csrc/muon.hip): the Muon optimiser's step on the matrix cores.
 
 ``orthogonalize(x)`` is the factor alone: five Newton-Schulz steps of the odd quintic (3.4445, -4.7750, 2.0315) on
-``x / (|x|_F + eps)``, with the accuracy of fp32 matrix products for any input type.  ``MuonPlan`` + ``muon_step`` are the optimiser
+``x / (|x|_F + eps)``, with the accuracy of fp32 matrix products for any input type, also in rows and columns that are little next to the
+others (down to 2^-100 of the norm).  ``MuonPlan`` + ``muon_step`` are the optimiser
 step over a fixed list of matrices, momentum and weight update included, every launch shared by all of them;
 ``train.MuonOptimizer`` runs it for the matrices of a graph.
 """
@@ -29,8 +30,7 @@ def _workspace(lib, shapes, device) -> torch.Tensor:
 
 
 def orthogonalize(x: torch.Tensor, eps: float = EPS, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The Newton-Schulz factor of a matrix, in its type; the zero matrix for a zero matrix.  ``out`` may be ``x`` itself.  A matrix
-    whose norm is so far below ``eps`` that ``x / eps`` has entries under 2^-40 gives zeros there."""
+    """The Newton-Schulz factor of a matrix, in its type; the zero matrix for a zero matrix.  ``out`` may be ``x`` itself."""
     lib = hb.require()
     ldx = hb.typed_rows(x, "x")
     if out is None:
