@@ -30,9 +30,8 @@
 // ring of 8, 4, 3 or 2 LDS images filled by direct buffer-to-LDS loads: 148, 132, 144 or 128 KB (ring_bytes()), one workgroup per
 // CU, the loads of a step requested one to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away,
 // against 0.1 to 1.8 us of products per step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at
-// 16 l), so the 16-byte chunks of a row are
-// permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the sixteen rows that a quarter of a fragment
-// read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
+// 16 l), so the 16-byte chunks of a row are permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the
+// sixteen rows that a quarter of a fragment read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
 // A step's two halves of 16 k alternate between two sets of fragment registers: the LDS reads of one half and the loads are
 // spread between the MFMAs of the half before, across the step's single barrier too.  Large tiles matter: per k-step of a
 // tile of edge T the matrix cores are busy for 0.047 T^2 cycles and the LDS for 6 T (reads by four waves of T/2 x T/2, and the
