@@ -69,7 +69,7 @@ class MuonPlan:
         self.params, self.grads, self.momenta = ([t.detach() for t in ts] for ts in (params, grads, momenta))
         self.device = params[0].device
         self._groups = []
-        self._streams = {hb._stream(params[0])}         # whose work the allocator waits for before it gives the memory away
+        self._streams = {torch.cuda.current_stream(self.device).cuda_stream}         # whose work the allocator waits for before it gives the memory away
         for i in range(0, len(params), GROUP):
             ws, gs, bs = params[i:i + GROUP], grads[i:i + GROUP], momenta[i:i + GROUP]
             n = len(ws)
