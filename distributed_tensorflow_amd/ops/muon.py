@@ -68,6 +68,7 @@ class MuonPlan:
         lib = hb.require()
         self.params, self.grads, self.momenta = ([t.detach() for t in ts] for ts in (params, grads, momenta))
         self.device = params[0].device
+        self._written = [hb._span(t) for t in written]
         self._groups = []
         self._streams = {torch.cuda.current_stream(self.device).cuda_stream}         # whose work the allocator waits for before it gives the memory away
         for i in range(0, len(params), GROUP):
@@ -84,6 +85,9 @@ def muon_step(plan: MuonPlan, lr: torch.Tensor, *, momentum: float = 0.95, neste
     lib = hb.require()
     if hb._f32c(lr, "lr").numel() != 1 or lr.device != plan.device:
         raise hb.HipKernelError("muon_step: lr is one float32 on the plan's device")
+    at = lr.data_ptr()
+    if any(first <= at < end for first, end in plan._written):
+        raise hb.HipKernelError("muon_step: the learning rate lies in a weight or momentum that the step writes")
     stream = hb._stream(lr)
     if stream not in plan._streams:
         side = torch.cuda.current_stream(plan.device)
@@ -91,6 +95,6 @@ def muon_step(plan: MuonPlan, lr: torch.Tensor, *, momentum: float = 0.95, neste
             t.record_stream(side)
         plan._streams.add(stream)
     for n, rows, cols, w, g, b, ws in plan._groups:
-        hb._check(lib.dtf_muon_step(n, rows, cols, w, g, b, lr.data_ptr(), float(momentum), int(bool(nesterov)), float(eps),
+        hb._check(lib.dtf_muon_step(n, rows, cols, w, g, b, at, float(momentum), int(bool(nesterov)), float(eps),
                                     ws.data_ptr(), ws.numel(), stream), "dtf_muon_step")
     hb.written(plan.params + plan.momenta)

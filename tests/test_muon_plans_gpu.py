@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from distributed_tensorflow_amd.ops import muon
+from distributed_tensorflow_amd.ops import hip_backend as hb, muon
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,13 @@ def test_a_plan_dropped_while_its_step_is_under_way_on_a_side_stream():
         t.fill_(255)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_learning_rate_that_the_step_would_write_is_refused():
+    w, g, b = (torch.ones(8, 6, device="cuda") for _ in range(3))
+    plan = muon.MuonPlan([w], [g], [b])
+    for at in (w.view(-1)[:1], w.view(-1)[47:], b.view(-1)[5:6]):
+        with pytest.raises(hb.HipKernelError):
+            muon.muon_step(plan, at)
+    assert bool((w == 1).all()) and bool((b == 1).all())
+    muon.muon_step(plan, g.view(-1)[:1])            # (only read)
