@@ -114,7 +114,11 @@ def update_rows(table: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, lr: 
         return lookup_sgd(table, ids, grad, lr, scale)
     flat = ids.reshape(-1).long()
     inside = (flat >= 0) & (flat < table.shape[0])
-    return table.index_add_(0, flat[inside], grad.reshape(-1, table.shape[1])[inside], alpha=-float(lr) * float(scale))
+    rows, step = grad.reshape(-1, table.shape[1])[inside], -float(lr) * float(scale)
+    if table.dtype == torch.float32:
+        return table.index_add_(0, flat[inside], rows, alpha=step)
+    # (sums in fp32 and rounded once; rows that do not occur come back as they were)
+    return table.copy_(table.float().index_add_(0, flat[inside], rows.float(), alpha=step))
 
 
 class _Lookup(torch.autograd.Function):
@@ -136,5 +140,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0)
     if table.is_cuda:
         return _Lookup.apply(hb.with_rows(table), ids, float(scale))
     inside = (ids >= 0) & (ids < table.shape[0])
-    rows = torch.nn.functional.embedding(torch.where(inside, ids, torch.zeros_like(ids)).long(), table) * scale
-    return torch.where(inside.unsqueeze(-1), rows, torch.zeros_like(rows))
+    # (16-bit tables: the gradient's sums in fp32, rounded once)
+    wide = table.float() if table.dtype in (torch.bfloat16, torch.float16) else table
+    rows = torch.nn.functional.embedding(torch.where(inside, ids, torch.zeros_like(ids)).long(), wide) * scale
+    return torch.where(inside.unsqueeze(-1), rows, torch.zeros_like(rows)).to(table.dtype)
