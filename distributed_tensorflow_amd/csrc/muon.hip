@@ -508,8 +508,8 @@ struct Linear {
 // Scales.  Row i of X is kept divided by d_i and column j (a row of X^T) by e_j, powers of two that are not below their norms (the
 // largest magnitude times the root of the length, rounded up); rows of A and B are divided by d_i too.  So an entry has its 22 bits
 // relative to its own row, however little that is next to the others.  (One scale for the whole matrix: rows of 10^-6 of the
-// others were 400 times as far off as in fp32, nothing was left of rows of 10^-10.  It took 127 us for the stack of three matrices
-// instead of 132, 351 for 1024 x 4096 instead of 368, 3.52 ms for a step of 4096 x 4096 instead of 3.64: X in fp32 is 4 bytes an
+// others were 400 times as far off as in fp32, nothing was left of rows of 10^-10.  It took 128 us for the stack of three matrices
+// instead of 132, 365 for 1024 x 4096 instead of 385, 3.52 ms for a step of 4096 x 4096 instead of 3.64: X in fp32 is 4 bytes an
 // element more to write in each step.)  No product needs more than that: with P = D^-1 X, R = D^-1 A, S = D^-1 B and T = E^-1 X^T,
 //   A = D (P P^T) D,   A A = D (R R^T) D,   B X = D (S T^T) E,
 // so the scales meet the sums at a product's end alone.  The linear terms carry no scale of one side: A is kept as D^-1 A D^-1
