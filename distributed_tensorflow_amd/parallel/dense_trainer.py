@@ -345,6 +345,7 @@ class PsDenseResidentTrainer:
         capturable = (self.device.type == "cuda" and not self.use_locking
                       and type(self.store).__name__ in ("IpcVariableStore", "LocalVariableStore"))
         self.use_graph = bool(use_graph) and capturable
+        self.train_op = train_op
         sess.own_gradients(train_op)
         self.params, self.grads = sess.theta, sess.grad
         view = lambda slab, v: None if v is None else sess.layout.view(slab, v.op_name)  # noqa: E731
@@ -423,6 +424,7 @@ class PsDenseResidentTrainer:
     def run_steps(self, n: int):
         bpe = self.engine.batches_per_epoch
         with self.sess.run_lock:            # (the Supervisor's checkpoint thread pulls into the same slab)
+            self.sess.own_gradients(self.train_op)        # (another op may have run through sess.run in between)
             for k in self._schedule(self.engine._host_cursor, n):
                 cur = self.engine._host_cursor
                 if cur % bpe == 0 and cur > 0:

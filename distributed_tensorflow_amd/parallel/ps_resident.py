@@ -62,6 +62,7 @@ class PsResidentTrainer(_BaseTrainer):
                       and not self.use_locking)
         self.use_graph = bool(use_graph) and capturable
         self.layout = sess.layout
+        self.train_op = train_op
         sess.own_gradients(train_op)
         self.params, self.grads = sess.theta, sess.grad
         names = {r: m[r].op_name for r in ("W1", "b1", "W2", "b2")}
@@ -191,6 +192,10 @@ class PsResidentTrainer(_BaseTrainer):
                 self._one_step(pos + i)
         self.engine.parity = parity
         return graph
+
+    def run_steps(self, n: int):
+        self.sess.own_gradients(self.train_op)       # (another op may have run through sess.run in between)
+        super().run_steps(n)
 
     def prepare(self, steps_hint=()):
         try:

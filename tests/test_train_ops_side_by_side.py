@@ -106,6 +106,13 @@ def test_engine_step_beside_another_op_on_a_parameter_server(widths, resident):
         sess.run(aside)
         assert np.array_equal(sess.run(w[0]), after) and abs(float(sess.run(other)[0, 0]) - 0.36) < 1e-6
         assert sess.run(step) == 2
+        kept = sess.run(other).copy()
+        if resident:
+            trainer.run_steps(1)
+        else:
+            sess.run(train, feed_dict=feed)
+        assert np.array_equal(sess.run(other), kept) and not np.array_equal(sess.run(w[0]), after)
+        assert sess.run(step) == 3
         sv.stop()
         sess.close()
     finally:
