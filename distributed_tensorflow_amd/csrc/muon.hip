@@ -31,7 +31,8 @@
 // CU, the loads of a step requested one to seven steps ahead of it (the matrices come from the other XCDs' writes: 0.8 us away,
 // against 0.1 to 1.8 us of products per step).  A load instruction moves eight 128-byte rows; its LDS side is fixed (lane l at
 // 16 l), so the 16-byte chunks of a row are permuted on the GLOBAL side: slot s of row r holds chunk s ^ ((r >> 1) & 7), and the
-// sixteen rows that a quarter of a fragment read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the banks; measured: no conflict).
+// sixteen rows that a quarter of a fragment read touches fill all 64 banks once (rows r and r + 1 lie in the two halves of the
+// banks; measured: no conflict).
 // A step's two halves of 16 k alternate between two sets of fragment registers: the LDS reads of one half and the loads are
 // spread between the MFMAs of the half before, across the step's single barrier too.  Large tiles matter: per k-step of a
 // tile of edge T the matrix cores are busy for 0.047 T^2 cycles and the LDS for 6 T (reads by four waves of T/2 x T/2, and the
@@ -58,7 +59,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kMax = DTF_MUON_MAX;
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleX = 32768.f, kScaleA = 16384.f, kScaleB = 8192.f;    // powers of two: entries stay below 65504
-constexpr int kParts = 16;            // of the rows, and of the columns, for the norm and the maxima: at most, unless there are few of the other
+constexpr int kParts = 16;            // of the rows, and of the columns, for the norm and the maxima (see lay_out())
 constexpr int kBlocks = kParts * kParts;
 constexpr int kMaxDim = 1 << 16;
 constexpr int kNormThreads = 1024;
@@ -99,8 +100,9 @@ __device__ __forceinline__ float most_of_16(float v) {
   return most_of_rotated<1>(most_of_rotated<2>(most_of_rotated<4>(most_of_rotated<8>(v))));
 }
 
-// A part of the matrix per block, 64 x 64 elements at a time, four columns a thread: the momentum, the sum of squares, and the largest
-// magnitude of every row and column (exact, so that their order does not matter).
+// A part of the matrix per block, 64 rows of 256 columns at a time, four quads a thread: the momentum, the sum of squares, and the
+// largest magnitude of every row and column (exact, so that their order does not matter).  (4096 x 4096: 41 us, 4.9 TB/s; the maxima
+// cost 8 of them.)
 template <typename T>
 __global__ __launch_bounds__(kNormThreads) void norm_kernel(Call c) {
   const Item& it = c.item[blockIdx.y];

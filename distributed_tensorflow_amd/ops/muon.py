@@ -1,9 +1,9 @@
 """Orthogonalised updates of matrices (csrc/muon.hip): the Muon optimiser's step on the matrix cores.
 
 ``orthogonalize(x)`` is the factor alone: five Newton-Schulz steps of the odd quintic (3.4445, -4.7750, 2.0315) on
-``x / (|x|_F + eps)``, with the accuracy of fp32 matrix products for any input type, also in rows and columns that are little next to the
-others (down to 2^-100 of the norm).  ``MuonPlan`` + ``muon_step`` are the optimiser
-step over a fixed list of matrices, momentum and weight update included, every launch shared by all of them;
+``x / (|x|_F + eps)``, with the accuracy of fp32 matrix products for any input type, also in rows and columns that are little next
+to the others (down to 2^-100 of the norm).  ``MuonPlan`` + ``muon_step`` are the optimiser step over a fixed list of matrices, momentum
+and weight update included, every launch shared by all of them;
 ``train.MuonOptimizer`` runs it for the matrices of a graph.
 """
 from __future__ import annotations
@@ -70,7 +70,8 @@ class MuonPlan:
         self.device = params[0].device
         self._written = [hb._span(t) for t in written]
         self._groups = []
-        self._streams = {torch.cuda.current_stream(self.device).cuda_stream}         # whose work the allocator waits for before it gives the memory away
+        # streams whose work the allocator waits for before it gives the memory away
+        self._streams = {torch.cuda.current_stream(self.device).cuda_stream}
         for i in range(0, len(params), GROUP):
             ws, gs, bs = params[i:i + GROUP], grads[i:i + GROUP], momenta[i:i + GROUP]
             n = len(ws)
