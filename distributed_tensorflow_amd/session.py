@@ -455,7 +455,9 @@ class Session:
             return v.get()
         if isinstance(v, torch.Tensor):
             a = v.detach().cpu().numpy()
-            return a.item() if a.ndim == 0 else a
+            if a.ndim == 0:
+                return a.item()
+            return a if v.is_cuda else a.copy()        # (host memory: the next step would write into what was fetched)
         return v
 
     def _feed_tensor(self, node, feed):

@@ -232,3 +232,19 @@ def test_muon_leaves_alone_what_its_loss_does_not_read_on_the_cpu(with_table):
 @pytest.mark.parametrize("with_table", [False, True])
 def test_muon_leaves_alone_what_its_loss_does_not_read_on_the_gpu(with_table):
     _muon_leaves_alone_what_its_loss_does_not_read(with_table)
+
+
+def test_a_fetched_variable_stays_as_it_was_fetched():
+    """A CPU session's variables lie in host memory: what ``sess.run`` hands out is a copy of it."""
+    with tf.Graph().as_default(), tf.device("/cpu:0"):
+        ids = tf.placeholder(tf.int64, [None])
+        table = tf.Variable(tf.ones([4, 3]), name="table")
+        train = tf.train.GradientDescentOptimizer(0.5).minimize(tf.reduce_sum(tf.nn.embedding_lookup(table, ids)))
+        with tf.Session() as sess:
+            sess.run(tf.global_variables_initializer())
+            fetched, same = sess.run(table), sess.run(tf.identity(table))
+            sess.run(train, feed_dict={ids: np.array([2])})
+            assert (fetched == 1).all() and (same == 1).all()
+            assert (sess.run(table)[2] == 0.5).all()
+            fetched[:] = 7
+            assert (sess.run(table)[0] == 1).all()
