@@ -92,7 +92,7 @@ def test_engine_step_beside_another_op_on_a_parameter_server(widths, resident):
         sv = tf.train.Supervisor(graph=g, is_chief=True, global_step=step, init_op=init)
         sess = sv.prepare_or_wait_for_session(worker.target)
         sess.run(aside)
-        kept, before = sess.run(other).copy(), sess.run(w[0]).copy()       # (a CPU session hands out its memory)
+        kept, before = sess.run(other), sess.run(w[0])
         if resident:
             ds = DeviceDataset(*feed.values(), sess.device, 8, seed=3)
             trainer = (PsResidentTrainer if len(widths) == 3 else PsDenseResidentTrainer)(sess, train, ds, 8)
@@ -101,12 +101,12 @@ def test_engine_step_beside_another_op_on_a_parameter_server(widths, resident):
             sess.run(train, feed_dict=feed)
             sess.run([train, loss], feed_dict=feed)
         assert np.array_equal(sess.run(other), kept)
-        after = sess.run(w[0]).copy()
+        after = sess.run(w[0])
         assert not np.array_equal(after, before)
         sess.run(aside)
         assert np.array_equal(sess.run(w[0]), after) and abs(float(sess.run(other)[0, 0]) - 0.36) < 1e-6
         assert sess.run(step) == 2
-        kept = sess.run(other).copy()
+        kept = sess.run(other)
         if resident:
             trainer.run_steps(1)
         else:
